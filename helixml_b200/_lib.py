@@ -11,6 +11,8 @@ LIB_PATH = os.path.join(_HERE, "libhelix_b200.so")
 HX_OK = 0
 HX_F32, HX_BF16, HX_U8 = 0, 1, 2
 SCAN_AUTO, SCAN_SIMPLE, SCAN_TILED, SCAN_SEQSPLIT, SCAN_DIRECT, SCAN_LOOKBACK = 0, 1, 2, 3, 4, 5
+GATE_DECAY, GATE_SIGMOID = 0, 1
+GATED_SCAN_STATE_STEPS = 64
 EPI_NONE, EPI_SILU, EPI_SOFTPLUS, EPI_SILU_FAST = 0, 1, 2, 3
 
 STATUS_NAMES = ["Ok", "ShapeMismatch", "InvalidDimension", "DeviceMismatch", "DTypeMismatch", "UnsupportedOperation",
@@ -77,6 +79,37 @@ class MambaStepArgs(C.Structure):
     ]
 
 
+class GatedScanArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seq_len", C.c_int32), ("d_inner", C.c_int32), ("io_dtype", C.c_int32), ("gate", C.c_int32),
+        ("reserved", C.c_int32),
+        ("x", C.c_void_p), ("g", C.c_void_p), ("h", C.c_void_p),
+        ("x_batch_stride", C.c_int64), ("x_row_stride", C.c_int64),
+        ("g_batch_stride", C.c_int64), ("g_row_stride", C.c_int64),
+        ("h_batch_stride", C.c_int64), ("h_row_stride", C.c_int64),
+        ("h0", C.c_void_p), ("h_last", C.c_void_p), ("states", C.c_void_p), ("lengths", C.c_void_p),
+    ]
+
+
+class GatedScanBwdArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seq_len", C.c_int32), ("d_inner", C.c_int32), ("io_dtype", C.c_int32), ("gate", C.c_int32),
+        ("reserved", C.c_int32),
+        ("x", C.c_void_p), ("g", C.c_void_p), ("dh", C.c_void_p), ("dx", C.c_void_p), ("dg", C.c_void_p),
+        ("x_batch_stride", C.c_int64), ("x_row_stride", C.c_int64),
+        ("g_batch_stride", C.c_int64), ("g_row_stride", C.c_int64),
+        ("dh_batch_stride", C.c_int64), ("dh_row_stride", C.c_int64),
+        ("dx_batch_stride", C.c_int64), ("dx_row_stride", C.c_int64),
+        ("dg_batch_stride", C.c_int64), ("dg_row_stride", C.c_int64),
+        ("states", C.c_void_p), ("dh_last", C.c_void_p), ("dh0", C.c_void_p), ("lengths", C.c_void_p),
+    ]
+
+
+class W4MatrixArgs(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("group", C.c_int32), ("scale_dtype", C.c_int32),
+                ("codes", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p)]
+
+
 class GatherArgs(C.Structure):
     _fields_ = [("world", C.c_int32), ("rank", C.c_int32), ("batch", C.c_int32), ("seq_len", C.c_int32),
                 ("d_shard", C.c_int32), ("d_full", C.c_int32), ("col0", C.c_int32), ("io_dtype", C.c_int32),
@@ -119,6 +152,10 @@ _PROTOS = {
                                      C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "hx_s4_diag_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "hx_gated_scan_fwd": (C.c_int, [C.POINTER(GatedScanArgs), C.c_void_p]),
+    "hx_gated_scan_bwd": (C.c_int, [C.POINTER(GatedScanBwdArgs), C.c_void_p]),
+    "hx_gated_scan_step": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                     C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "hx_s4_ref_forward_ssm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
                                         C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t,
                                         C.c_void_p]),
@@ -137,6 +174,12 @@ _PROTOS = {
                                            C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "hx_gemm_simt": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "hx_w4_row_bytes": (C.c_size_t, [C.c_int32]),
+    "hx_w4_quantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.POINTER(W4MatrixArgs), C.c_void_p]),
+    "hx_w4_pack": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(W4MatrixArgs), C.c_void_p]),
+    "hx_w4_dequantize": (C.c_int, [C.POINTER(W4MatrixArgs), C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "hx_gemm_w4": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.POINTER(W4MatrixArgs), C.c_void_p, C.c_void_p, C.c_int64,
+                             C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "hx_rmsnorm_fwd": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64,
                                  C.c_int32, C.c_float, C.c_void_p]),
     "hx_embedding_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_int32,

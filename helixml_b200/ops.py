@@ -162,6 +162,145 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, conv_w=None, conv_b=None, d
     return (y, h) if return_state else y
 
 
+GATES = {"decay": L.GATE_DECAY, "sigmoid": L.GATE_SIGMOID}
+
+
+def _gate(gate) -> int:
+    if gate not in GATES:
+        raise L.HxError(10, f"unknown gate {gate!r}: one of {sorted(GATES)}")
+    return GATES[gate]
+
+
+def _on_device(**tensors):
+    """The one CUDA device all of these (None among them) are on."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda or (dev is not None and t.device != dev):
+            raise L.HxError(3, f"{name} is on {t.device}" + (f", expected {dev}" if dev is not None else ", expected a CUDA device"))
+        dev = t.device
+    return dev
+
+
+def _run_on(dev, fn, *args):
+    """fn(*args, stream) on `dev` and the stream torch uses there, whichever device is the current one."""
+    stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if dev.index == torch.cuda.current_device():
+        L.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(dev):
+            L.check(fn(*args, stream))
+
+
+def _like(name, t, shape, dtype):
+    if t.dtype != dtype:
+        raise L.HxError(4, f"{name} has dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise L.HxError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _dense(name, t, shape, dtype):
+    """An operand the library takes without strides: checked, and copied where it is a strided view."""
+    if t is None:
+        return None
+    _like(name, t, shape, dtype)
+    return t.contiguous()
+
+
+def _dense_out(name, t, shape, dtype):
+    _like(name, t, shape, dtype)
+    if not t.is_contiguous():
+        raise L.HxError(1, f"{name} must be contiguous")
+    return t
+
+
+def gated_scan_states(batch, seq_len, d_inner, device="cuda"):
+    """The buffer in which gated_scan keeps what gated_scan_bwd starts from: the state before every 64th row, fp32."""
+    steps = L.GATED_SCAN_STATE_STEPS
+    return torch.empty((batch, (seq_len + steps - 1) // steps, d_inner), dtype=torch.float32, device=device)
+
+
+def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_state=False, states=None):
+    """Gated linear recurrence (hx_gated_scan_fwd): h_t = g_t h_{t-1} + x_t ("decay"), or a_t h_{t-1} + (1 - a_t) x_t with
+    a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
+    lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
+    states: a gated_scan_states buffer, filled for gated_scan_bwd.  Returns h, or (h, h_last [B, D] fp32) with return_state."""
+    dev = _on_device(x=x, g=g, h0=h0, lengths=lengths, out=out, states=states)
+    _view3(x)
+    Bsz, Lq, Dm = x.shape
+    a = L.GatedScanArgs()
+    a.batch, a.seq_len, a.d_inner, a.io_dtype, a.gate = Bsz, Lq, Dm, _dt(x), _gate(gate)
+    h = out if out is not None else torch.empty((Bsz, Lq, Dm), dtype=x.dtype, device=dev)
+    for name, t in (("x", x), ("g", g), ("h", h)):
+        _like(name, t, (Bsz, Lq, Dm), x.dtype)
+        bs, rs = _view3(t)
+        setattr(a, name, t.data_ptr())
+        setattr(a, f"{name}_batch_stride", bs)
+        setattr(a, f"{name}_row_stride", rs)
+    h0 = _dense("h0", h0, (Bsz, Dm), torch.float32)
+    lengths = _dense("lengths", lengths, (Bsz,), torch.int32)
+    last = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev) if return_state else None
+    if states is not None:
+        steps = L.GATED_SCAN_STATE_STEPS
+        _dense_out("states", states, (Bsz, (Lq + steps - 1) // steps, Dm), torch.float32)
+    for name, t in (("h0", h0), ("h_last", last), ("states", states), ("lengths", lengths)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    _run_on(dev, L.lib().hx_gated_scan_fwd, C.byref(a))
+    return (h, last) if return_state else h
+
+
+def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None, out=None):
+    """Gradients of gated_scan (hx_gated_scan_bwd): (dx, dg, dh0) for dh = dL/dh [B, L, D] and dh_last = dL/dh_last [B, D]
+    fp32 (None: zero).  x, g and lengths as given to gated_scan, states as it filled them; out: (dx, dg) to write into (halves
+    of one buffer, say)."""
+    dx, dg = out if out is not None else (None, None)
+    dev = _on_device(dh=dh, x=x, g=g, states=states, lengths=lengths, dh_last=dh_last, dx=dx, dg=dg)
+    _view3(x)
+    Bsz, Lq, Dm = x.shape
+    a = L.GatedScanBwdArgs()
+    a.batch, a.seq_len, a.d_inner, a.io_dtype, a.gate = Bsz, Lq, Dm, _dt(x), _gate(gate)
+    if out is None:
+        dx, dg = (torch.empty((Bsz, Lq, Dm), dtype=x.dtype, device=dev) for _ in range(2))
+    for name, t in (("x", x), ("g", g), ("dh", dh), ("dx", dx), ("dg", dg)):
+        _like(name, t, (Bsz, Lq, Dm), x.dtype)
+        bs, rs = _view3(t)
+        setattr(a, name, t.data_ptr())
+        setattr(a, f"{name}_batch_stride", bs)
+        setattr(a, f"{name}_row_stride", rs)
+    steps = L.GATED_SCAN_STATE_STEPS
+    states = _dense("states", states, (Bsz, (Lq + steps - 1) // steps, Dm), torch.float32)
+    dh_last = _dense("dh_last", dh_last, (Bsz, Dm), torch.float32)
+    lengths = _dense("lengths", lengths, (Bsz,), torch.int32)
+    dh0 = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev)
+    for name, t in (("states", states), ("dh_last", dh_last), ("dh0", dh0), ("lengths", lengths)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    _run_on(dev, L.lib().hx_gated_scan_bwd, C.byref(a))
+    return dx, dg, dh0
+
+
+def gated_scan_step(x, g, h, gate="sigmoid", h_out=None, out=None):
+    """One token of the gated recurrence for every sequence (hx_gated_scan_step): x, g [B, D] (row strides arbitrary),
+    h [B, D] fp32.  Returns y [B, D]; the new state goes to h_out, or replaces h."""
+    h_out = h if h_out is None else h_out
+    dev = _on_device(x=x, g=g, h=h, h_out=h_out, out=out)
+    if x.dim() != 2:
+        raise L.HxError(1, f"expected a [B, D] tensor, got {tuple(x.shape)}")
+    Bsz, Dm = x.shape
+    y = out if out is not None else torch.empty((Bsz, Dm), dtype=x.dtype, device=dev)
+    for name, t in (("x", x), ("g", g), ("y", y)):
+        _like(name, t, (Bsz, Dm), x.dtype)
+        if t.stride(1) != 1:
+            raise L.HxError(1, f"{name} needs a unit inner stride, has {t.stride()}")
+    for name, t in (("h", h), ("h_out", h_out)):
+        _dense_out(name, t, (Bsz, Dm), torch.float32)
+    _run_on(dev, L.lib().hx_gated_scan_step, _p(x), x.stride(0), _p(g), g.stride(0), _p(h), _p(h_out), _p(y), y.stride(0), Bsz, Dm,
+            _gate(gate), _dt(x))
+    return y
+
+
 def conv1d_silu(x, conv_w, conv_b=None, out=None):
     Bsz, Lq, Dm = x.shape
     u = out if out is not None else torch.empty((Bsz, Lq, Dm), dtype=x.dtype, device=x.device)
@@ -254,6 +393,93 @@ def gemm_acc(a, w, c):
         raise L.HxError(1, f"shapes {tuple(a.shape)}, {tuple(w.shape)}, {tuple(c.shape)} do not fit")
     L.check(L.lib().hx_gemm_bf16_acc(a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(0), c.data_ptr(), c.stride(0), M, N, K,
                                      _stream()))
+    return c
+
+
+class W4Matrix:
+    """A weight matrix [N, K] in 4 bits with one scale per `group` columns of a row (hx_w4_matrix): codes u8
+    [N, row bytes], scale [N, K / group] fp32 or bf16, zero [N, K / group] u8 or None (code 8 stands for zero).  Made by
+    w4_quantize or w4_pack."""
+
+    def __init__(self, rows, cols, group, scale, zero):
+        if group not in (32, 64, 128) or cols % group:
+            raise L.HxError(1, f"{cols} columns in groups of {group}: groups are 32, 64 or 128 and divide the columns")
+        dev = _on_device(scale=scale, zero=zero)
+        if scale.dtype not in (torch.float32, torch.bfloat16):
+            raise L.HxError(4, f"scale has dtype {scale.dtype}, expected float32 or bfloat16")
+        self.rows, self.cols, self.group = rows, cols, group
+        self.scale = _dense("scale", scale, (rows, cols // group), scale.dtype)
+        self.zero = _dense("zero", zero, (rows, cols // group), torch.uint8)
+        self.codes = torch.empty((rows, L.lib().hx_w4_row_bytes(cols)), dtype=torch.uint8, device=dev)
+
+    def _args(self):
+        m = L.W4MatrixArgs()
+        m.rows, m.cols, m.group, m.scale_dtype = self.rows, self.cols, self.group, _dt(self.scale)
+        m.codes, m.scale, m.zero = self.codes.data_ptr(), self.scale.data_ptr(), None if self.zero is None else self.zero.data_ptr()
+        return m
+
+
+def _rows2(name, t):
+    """Row stride in elements of a [rows, columns] view with unit inner stride."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise L.HxError(1, f"{name}: expected a 2-D tensor with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
+    return t.stride(0)
+
+
+def w4_quantize(w, group=64, zero_points=False, scale_dtype=torch.float32) -> W4Matrix:
+    """Weights w [N, K] (fp32 or bf16) in 4 bits (hx_w4_quantize): symmetric about zero, or with a zero point per group."""
+    ldw = _rows2("w", w)
+    dev = _on_device(w=w)
+    if scale_dtype not in (torch.float32, torch.bfloat16):
+        raise L.HxError(4, f"scale dtype {scale_dtype}: float32 or bfloat16")
+    N, K = w.shape
+    if group not in (32, 64, 128) or K % group:
+        raise L.HxError(1, f"{K} columns in groups of {group}: groups are 32, 64 or 128 and divide the columns")
+    scale = torch.empty((N, K // group), dtype=scale_dtype, device=dev)
+    zero = torch.empty((N, K // group), dtype=torch.uint8, device=dev) if zero_points else None
+    m = W4Matrix(N, K, group, scale, zero)
+    _run_on(dev, L.lib().hx_w4_quantize, _p(w), ldw, _dt(w), C.byref(m._args()))
+    return m
+
+
+def w4_pack(codes, scale, zero=None) -> W4Matrix:
+    """A matrix whose codes exist already (hx_w4_pack): codes [N, K] u8 in 0..15, scale [N, K / group], zero like scale or
+    None; the group follows from the shapes."""
+    ldc = _rows2("codes", codes)
+    dev = _on_device(codes=codes, scale=scale, zero=zero)
+    if codes.dtype != torch.uint8:
+        raise L.HxError(4, f"codes have dtype {codes.dtype}, expected uint8")
+    N, K = codes.shape
+    groups = scale.shape[1] if scale.dim() == 2 else 0
+    if groups < 1 or K % groups:
+        raise L.HxError(1, f"scale {tuple(scale.shape)} does not divide codes {tuple(codes.shape)} into groups")
+    m = W4Matrix(N, K, K // groups, scale, zero)
+    _run_on(dev, L.lib().hx_w4_pack, _p(codes), ldc, C.byref(m._args()))
+    return m
+
+
+def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
+    """The values a W4Matrix stands for, [N, K] fp32 or bf16 (hx_w4_dequantize)."""
+    dev = m.codes.device
+    w = out if out is not None else torch.empty((m.rows, m.cols), dtype=dtype, device=dev)
+    _on_device(codes=m.codes, out=w)
+    _like("out", w, (m.rows, m.cols), dtype)
+    _run_on(dev, L.lib().hx_w4_dequantize, C.byref(m._args()), _p(w), _rows2("out", w), _dt(w))
+    return w
+
+
+def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=None):
+    """C = a @ W.T (+ bias) (+ activation) with W in 4 bits (hx_gemm_w4), for the few rows of a decode step.
+    a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's)."""
+    dev = _on_device(a=a, codes=m.codes, bias=bias, out=out)
+    lda = _rows2("a", a)
+    M, K = a.shape
+    if K != m.cols:
+        raise L.HxError(1, f"a is {tuple(a.shape)} but W is {(m.rows, m.cols)}")
+    bias = _dense("bias", bias, (m.rows,), torch.float32)
+    c = out if out is not None else torch.empty((M, m.rows), dtype=out_dtype or a.dtype, device=dev)
+    _like("out", c, (M, m.rows), out_dtype or c.dtype)
+    _run_on(dev, L.lib().hx_gemm_w4, _p(a), lda, _dt(a), C.byref(m._args()), _p(bias), _p(c), _rows2("out", c), _dt(c), M, epilogue)
     return c
 
 

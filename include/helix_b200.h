@@ -300,6 +300,70 @@ HX_API hx_status hx_s4_diag_fwd(const void *u, const float *A, const float *Bp, 
                          int32_t seq_len, int32_t d_model, int32_t d_state, int32_t io_dtype,
                          void *stream);
 
+/* ---- gated linear recurrence: a scan whose decay is an input of its own at every point.  (The reference has no such
+ * layer; it stands beside the scans above.)  Per batch row b and channel d, over t = 0 .. len[b] - 1:
+ *   HX_GATE_DECAY     a_t = g[b,t,d]              h_t = a_t h_{t-1} + x[b,t,d]
+ *   HX_GATE_SIGMOID   a_t = 1 / (1 + exp(-g))     h_t = a_t h_{t-1} + (1 - a_t) x[b,t,d]
+ * h_{-1} = h0[b,d] (zero without h0).  State and arithmetic are fp32 whatever io_dtype is.  A decay may have any sign; sums
+ * are associated over time in an order of the kernel's own (the same for every call of one shape), so with |a| > 1 rounding
+ * grows as it does in any order.  Results for infinite and NaN inputs are those of the sequential recurrence.
+ *   lengths (int32 [batch] on the device, or NULL for seq_len everywhere; values are clamped to 0 .. seq_len): rows of a
+ *   padded batch from len[b] on are not read as numbers (they may hold anything), their outputs are zeros, and h_last is the
+ *   state after row len[b] - 1 (h0 where len[b] is 0).
+ * x, g and dh may be any views with a unit inner stride and strides >= 0; the rows of an output must not overlap one another
+ * or an input. */
+typedef enum hx_gate_kind { HX_GATE_DECAY = 0, HX_GATE_SIGMOID = 1 } hx_gate_kind;
+/* Steps from one state kept for the backward pass to the next. */
+#define HX_GATED_SCAN_STATE_STEPS 64
+typedef struct hx_gated_scan_args {
+    int32_t batch, seq_len, d_inner;
+    int32_t io_dtype;         /* hx_dtype of x, g, h: HX_F32 or HX_BF16 */
+    int32_t gate;             /* hx_gate_kind */
+    int32_t reserved;
+    const void *x, *g;        /* [batch, seq_len, d_inner] */
+    void *h;                  /* [batch, seq_len, d_inner] */
+    int64_t x_batch_stride, x_row_stride;
+    int64_t g_batch_stride, g_row_stride;
+    int64_t h_batch_stride, h_row_stride;
+    const float *h0;          /* [batch, d_inner] fp32 or NULL */
+    float *h_last;            /* [batch, d_inner] fp32 or NULL; may be h0's buffer */
+    float *states;            /* NULL, or [batch, ceil(seq_len / 64), d_inner] fp32: the state before row 64 i, what the
+                                 backward pass starts from */
+    const int32_t *lengths;   /* [batch] or NULL */
+} hx_gated_scan_args;
+HX_API hx_status hx_gated_scan_fwd(const hx_gated_scan_args *args, void *stream);
+
+/* Its gradients.  With dh = dL/dh and dh_last = dL/dh_last, from the end of each sequence:
+ *   delta_t = dh_t + a_{t+1} delta_{t+1}   (behind the last row: dh_last)        dh0 = a_0 delta_0
+ *   HX_GATE_DECAY     dx = delta            dg = delta h_{t-1}
+ *   HX_GATE_SIGMOID   dx = delta (1 - a)    dg = delta (h_{t-1} - x) a (1 - a)
+ * h_{t-1} is recomputed in fp32 from x, g and the forward pass's `states`, so the rounded h is not needed.  Rows from
+ * len[b] on get zero gradients; where len[b] is 0, dh0 = dh_last. */
+typedef struct hx_gated_scan_bwd_args {
+    int32_t batch, seq_len, d_inner;
+    int32_t io_dtype;         /* of x, g, dh, dx, dg */
+    int32_t gate;
+    int32_t reserved;
+    const void *x, *g, *dh;   /* [batch, seq_len, d_inner] */
+    void *dx, *dg;            /* [batch, seq_len, d_inner] */
+    int64_t x_batch_stride, x_row_stride;
+    int64_t g_batch_stride, g_row_stride;
+    int64_t dh_batch_stride, dh_row_stride;
+    int64_t dx_batch_stride, dx_row_stride;
+    int64_t dg_batch_stride, dg_row_stride;
+    const float *states;      /* what hx_gated_scan_fwd wrote for the same x, g, h0 and lengths */
+    const float *dh_last;     /* [batch, d_inner] fp32 or NULL */
+    float *dh0;               /* [batch, d_inner] fp32 or NULL */
+    const int32_t *lengths;
+} hx_gated_scan_bwd_args;
+HX_API hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *args, void *stream);
+
+/* One token per sequence: h_out = a h + x (or (1 - a) x), y = h_out in the io dtype.  x, g, y: [batch, d_inner] with row
+ * strides; h, h_out: [batch, d_inner] fp32, dense; h_out may be h. */
+HX_API hx_status hx_gated_scan_step(const void *x, int64_t x_row_stride, const void *g, int64_t g_row_stride, const float *h,
+                             float *h_out, void *y, int64_t y_row_stride, int32_t batch, int32_t d_inner, int32_t gate,
+                             int32_t io_dtype, void *stream);
+
 /* ---- the reference-literal S4 recurrence (crates/nn/src/ssm.rs:138-186): one shared state vector
  * of d_state entries driven by all d_model inputs.
  *   a = exp(dt A_real) cos(dt A_imag);  state_t = a state_{t-1} + (dt Bm) u_t;  y_t = Cm state_t + Dv u_t
@@ -361,6 +425,42 @@ HX_API hx_status hx_gemm_pair_mode(int32_t mode, int32_t *pairs);
 HX_API hx_status hx_gemm_simt(const void *A, int64_t lda, const void *W, int64_t ldw, const float *bias,
                        void *C, int64_t ldc, int32_t ab_dtype, int32_t c_dtype, int32_t M,
                        int32_t N, int32_t K, int32_t epilogue, void *stream);
+
+/* ---- weights in 4 bits: W[n,k] = scale[n, k / group] * (code[n,k] - zero[n, k / group]) with codes and zero points in 0..15
+ * (zero = 8 everywhere when `zero` is NULL).  A decode step is bound by the bytes of its projections; this form reads a
+ * quarter of what bf16 weights take, plus one scale per group.  (No counterpart in the reference, whose quantize_int8 is a
+ * trait method on whole tensors, crates/tensor-core/src/tensor.rs:236-275.)
+ * A row of codes is hx_w4_row_bytes(cols) bytes: blocks of 64 bytes for 128 columns (the last one filled up with code 8).
+ * With r = k mod 128, code[n,k] is in the 32-bit word at byte 16 ((r mod 32) / 8) + 4 (r / 32) of its block, at bits
+ * 4 p .. 4 p + 3, p = (r mod 8) / 2 + 4 (r mod 2): a lane of the product's kernel finds 8 codes of each of four groups in 16
+ * bytes, and the two halves of a tensor-core operand in the two halves of a word. */
+typedef struct hx_w4_matrix {
+    int32_t rows, cols;       /* out and in features; cols a multiple of `group` */
+    int32_t group;            /* 32, 64 or 128 consecutive columns share a scale */
+    int32_t scale_dtype;      /* HX_F32 or HX_BF16 */
+    uint8_t *codes;           /* [rows, hx_w4_row_bytes(cols)], 16-byte aligned */
+    void *scale;              /* [rows, cols / group] */
+    uint8_t *zero;            /* [rows, cols / group] or NULL */
+} hx_w4_matrix;
+HX_API size_t hx_w4_row_bytes(int32_t cols);
+/* Quantises W [rows, cols] (fp32 or bf16, row stride ldw) into m's codes, scale and, where m->zero is given, zero points:
+ *   without zero points  scale = max|w| / 7 over the group, code = clamp(round(w / scale), -7, 7) + 8
+ *   with zero points     lo = min(w, 0), hi = max(w, 0) over the group, scale = (hi - lo) / 15, zero = clamp(round(-lo / scale),
+ *                        0, 15), code = clamp(round(w / scale) + zero, 0, 15)
+ * `scale` is rounded to fp32, then to scale_dtype, before it divides; quotients are decided as in exact arithmetic, ties to
+ * even.  A group of zeros (or one whose scale rounds to zero) gets scale 0, codes and zero point 8; a group that holds an
+ * infinity or a NaN gets a NaN scale. */
+HX_API hx_status hx_w4_quantize(const void *W, int64_t ldw, int32_t w_dtype, const hx_w4_matrix *m, void *stream);
+/* Lays out codes that exist already: in [rows, cols] u8 (the low four bits count, row stride ldc) -> m->codes. */
+HX_API hx_status hx_w4_pack(const uint8_t *in, int64_t ldc, const hx_w4_matrix *m, void *stream);
+/* The values the matrix stands for: W [rows, cols] fp32 or bf16, row stride ldw. */
+HX_API hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t w_dtype, void *stream);
+/* C[M,N] = A[M,K] . W^T (+ bias[N]) (+ activation: 0 none, 1 SiLU, 2 softplus) with N = m->rows, K = m->cols; A and C fp32 or
+ * bf16 with row strides in elements, bias fp32.  Every product and sum is fp32 or wider than its operands: codes are exact,
+ * the sum over a group is scaled in fp32.  Made for the few rows of a decode step (any M is right; beyond 64 rows the weights
+ * are read once per 64 rows, and hx_w4_dequantize with hx_gemm_bf16 is the faster way). */
+HX_API hx_status hx_gemm_w4(const void *A, int64_t lda, int32_t a_dtype, const hx_w4_matrix *m, const float *bias, void *C,
+                     int64_t ldc, int32_t c_dtype, int32_t M, int32_t epilogue, void *stream);
 
 /* ---- RMSNorm over the last axis with optional fused residual add.  The residual stream is fp32:
  *   if (residual) { residual += x (x may be NULL: nothing added); src = residual } else src = x
