@@ -12,7 +12,7 @@ HX_OK = 0
 HX_F32, HX_BF16, HX_U8 = 0, 1, 2
 SCAN_AUTO, SCAN_SIMPLE, SCAN_TILED, SCAN_SEQSPLIT, SCAN_DIRECT, SCAN_LOOKBACK = 0, 1, 2, 3, 4, 5
 GATE_DECAY, GATE_SIGMOID = 0, 1
-GATED_SCAN_STATE_STEPS = 64
+GATED_SCAN_STATE_STEPS = 16
 EPI_NONE, EPI_SILU, EPI_SOFTPLUS, EPI_SILU_FAST = 0, 1, 2, 3
 
 STATUS_NAMES = ["Ok", "ShapeMismatch", "InvalidDimension", "DeviceMismatch", "DTypeMismatch", "UnsupportedOperation",
@@ -88,6 +88,7 @@ class GatedScanArgs(C.Structure):
         ("g_batch_stride", C.c_int64), ("g_row_stride", C.c_int64),
         ("h_batch_stride", C.c_int64), ("h_row_stride", C.c_int64),
         ("h0", C.c_void_p), ("h_last", C.c_void_p), ("states", C.c_void_p), ("lengths", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -102,6 +103,7 @@ class GatedScanBwdArgs(C.Structure):
         ("dx_batch_stride", C.c_int64), ("dx_row_stride", C.c_int64),
         ("dg_batch_stride", C.c_int64), ("dg_row_stride", C.c_int64),
         ("states", C.c_void_p), ("dh_last", C.c_void_p), ("dh0", C.c_void_p), ("lengths", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -153,6 +155,7 @@ _PROTOS = {
     "hx_s4_diag_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "hx_gated_scan_fwd": (C.c_int, [C.POINTER(GatedScanArgs), C.c_void_p]),
+    "hx_gated_scan_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
     "hx_gated_scan_bwd": (C.c_int, [C.POINTER(GatedScanBwdArgs), C.c_void_p]),
     "hx_gated_scan_step": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                      C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),

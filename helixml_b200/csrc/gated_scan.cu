@@ -1,112 +1,557 @@
 // Gated linear recurrence h_t = a_t h_{t-1} + b_t over [batch, seq_len, d_inner], its gradients, and its single-token step.
-// One thread per (batch row, channel) walks the sequence; neighbouring lanes hold neighbouring channels.
+//
+// The work per point is a handful of instructions, so both directions are bound by HBM: x and g read and h written once, or x, g
+// and dh read and dx and dg written once.  A warp owns 64 neighbouring channels of one batch row (two a lane) and walks the steps;
+// its rows arrive through a ring of cp.async fetches in its own part of shared memory, so warps never wait for one another.
+// Where the chains alone are too few warps to keep HBM busy, the sequence is cut into segments: run t..t' composes to the affine map
+// h -> A h + B (A the product of its decays, B its result from zero), a first launch writes the map of every segment but the last,
+// and the second folds the maps before its segment onto h0 and walks the segment with outputs.  That reads x and g twice, the second
+// time from L2 as far as they fit: the first launch walks every segment from its end (a map can be built from either side), so what
+// it read last is what the second needs first.  The order of the sums is a function of the shape alone.
+// The backward pass is the same recurrence from the end, e_t = a_t (dh_t + e_{t+1}); h_{t-1} is recomputed from the state that the
+// forward pass saved every 16 steps, so h itself, rounded to the io type, is not needed.
+//
+// Folding maps is not the recurrence where numbers leave the format: a product of decays that underflows times an infinite state
+// would be NaN, one that overflows times a state of zero too.  Where a map's A or a folded state is not finite, the warp walks the
+// steps from there to its segment instead.
+#include <algorithm>
+#include <initializer_list>
+
 #include "hx_common.cuh"
+#include "hx_tma.cuh"
 
 namespace hx {
 namespace gated {
 
-constexpr int kStateSteps = HX_GATED_SCAN_STATE_STEPS;
+constexpr int kC = 64;                    // channels of a warp, two a lane
+constexpr int kRun = 8;                   // steps of a forward fetch
+constexpr int kBlock = HX_GATED_SCAN_STATE_STEPS;   // steps of a backward fetch: from one saved state to the next
+constexpr int kWarps = 4;                 // warps of a CTA, each on its own
+constexpr int kStages = 6, kBlockStages = 3;        // fetches a ring of runs, of blocks holds: all but one are under way
+constexpr int kOccupancy = 4, kBlockOccupancy = 3;  // CTAs an SM is to hold (registers)
+static_assert(kBlock == 2 * kRun, "segments are multiples of both");
 
-// a = sigmoid(g) and rest = 1 - a, both to full relative precision: exp is taken of -|g|, so it neither overflows nor cancels.
-__device__ __forceinline__ void sigmoid_pair(float g, float &a, float &rest) {
-    const float e = expf(-fabsf(g));
-    const float big = 1.0f / (1.0f + e), small = e * big;
-    a = g >= 0.f ? big : small;   // a NaN goes through as NaN
-    rest = g >= 0.f ? small : big;
+template <int BYTES> __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One tensor's way into a warp's ring: pieces of ROWS rows of kC channels, from row `t` of src on.  `cols` channels exist, those
+// behind them are zeros.  PIECE: what every address is a multiple of, in bytes; two-byte pieces go through registers.
+template <int ROWS, int PIECE, typename T> struct Feed {
+    static constexpr int per = PIECE >= 4 ? PIECE / (int)sizeof(T) : 1, across = kC / per;   // elements of a piece, pieces of a row
+    static constexpr int wide = across < 32 ? across : 32, high = 32 / wide;    // one instruction of the warp: high rows x wide pieces
+    static constexpr int turns = across / wide;
+    const T *from;        // this lane's first piece of the next fetch
+    int64_t row_stride, advance;
+    int cols, bytes[turns];
+    uint32_t offset;      // of that piece in a slot
+    __device__ __forceinline__ Feed(const T *src, int64_t t, int64_t rs, int steps, int cols_, int lane) {
+        const int r0 = lane / wide, col = lane % wide * per;
+        row_stride = rs;
+        advance = steps * rs;
+        cols = cols_;
+        from = src + t * rs + r0 * rs + col;
+        offset = (uint32_t)(r0 * kC + col) * (uint32_t)sizeof(T);
+#pragma unroll
+        for (int q = 0; q < turns; ++q) bytes[q] = min(max(cols - col - q * wide * per, 0), per) * (int)sizeof(T);
+    }
+    // all ROWS rows exist
+    __device__ __forceinline__ void whole(uint32_t slot) {
+        const T *f = from;
+        from += advance;
+        if constexpr (PIECE >= 4) {
+#pragma unroll
+            for (int r = 0; r < ROWS; r += high) {
+#pragma unroll
+                for (int q = 0; q < turns; ++q)
+                    cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, bytes[q]);
+                f += high * row_stride;
+            }
+        } else {
+            copy(slot, f, ROWS);
+        }
+    }
+    // `rows` of them do
+    __device__ __forceinline__ void part(uint32_t slot, int rows) {
+        const T *f = from;
+        from += advance;
+        if constexpr (PIECE >= 4) {
+            const int r0 = (threadIdx.x & 31) / wide;
+#pragma unroll
+            for (int r = 0; r < ROWS; r += high) {
+#pragma unroll
+                for (int q = 0; q < turns; ++q) {
+                    const int n = r0 + r < rows ? bytes[q] : 0;   // nothing is read where n is 0
+                    cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, n);
+                }
+                f += high * row_stride;
+            }
+        } else {
+            copy(slot, f, rows);
+        }
+    }
+    // two-byte elements at any address: the lane's columns are lane and lane + 32
+    __device__ __forceinline__ void copy(uint32_t slot, const T *f, int rows) {
+        const int lane = threadIdx.x & 31;
+        f -= lane % wide * per;   // across = 64 elements: wide = 32, high = 1
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int k = 0; k < kC / 32; ++k) {
+                const int col = lane + 32 * k;
+                const T v = r < rows && col < cols ? f[r * row_stride + col] : T(0.f);
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(slot + (r * kC + col) * 2), "h"(*reinterpret_cast<const uint16_t *>(&v)) : "memory");
+            }
+    }
+};
+
+// A lane's two channels.
+__device__ __forceinline__ float2 load2(const float *p) { return *reinterpret_cast<const float2 *>(p); }
+__device__ __forceinline__ float2 load2(const __nv_bfloat16 *p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ void store2(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
+__device__ __forceinline__ void store2(__nv_bfloat16 *p, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y); }
+// the first n of them, at any alignment
+template <typename T> __device__ __forceinline__ float2 load_some(const T *p, int n) {
+    return make_float2(n > 0 ? ld_f32(p) : 0.f, n > 1 ? ld_f32(p + 1) : 0.f);
+}
+template <typename T> __device__ __forceinline__ void store_some(T *p, float2 v, int n) {
+    if (n > 0) st_f32(p, v.x);
+    if (n > 1) st_f32(p + 1, v.y);
 }
 
-template <int GATE> __device__ __forceinline__ void decay_and_input(float g, float x, float &a, float &b) {
-    if constexpr (GATE == HX_GATE_DECAY) {
+// A pair of gates -> decays a = sigmoid(g) and 1 - a, both to full relative precision: with e = exp(-g), a = 1 / (1 + e) and
+// 1 - a = e a, neither of which cancels.  e is held to about 2^126, where a is the smallest normal number and 1 - a comes out as 1;
+// taking 2^-126 off a makes it the zero it should be there and is below the rounding of any a that matters.  A NaN goes through.
+// FAST, for bf16 results: one exp2 and one reciprocal of the special-function unit, off by (|g| + 9) 2^-24, far below 2^-9.
+// Otherwise e = 2^t (1 + (t' - t) ln 2), t the rounded and t' the exact product -g log2(e), and one Newton step on the reciprocal.
+template <bool FAST> __device__ __forceinline__ void sigmoid2(float2 g, float2 &a, float2 &rest) {
+    float2 e;
+    if constexpr (FAST) {
+        float2 t = mul2(g, make_float2(-kLog2e, -kLog2e));
+        asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.x));   // 126
+        asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.y));
+        e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+    } else {
+        constexpr float kLog2eLow = (float)(1.44269504088896340736 - (double)kLog2e);
+        asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g.x));   // -126 ln 2
+        asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g.y));
+        asm("min.NaN.f32 %0, %0, 0f43480000;" : "+f"(g.x));   // 200: e is zero there, and t finite
+        asm("min.NaN.f32 %0, %0, 0f43480000;" : "+f"(g.y));
+        const float2 t = mul2(g, splat2(-kLog2e));
+        const float2 low = fma2(g, splat2(-kLog2eLow), fma2(g, splat2(-kLog2e), make_float2(-t.x, -t.y)));
+        e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+        e = fma2(e, mul2(low, splat2(kLn2)), e);
+    }
+    const float2 d = add2(e, splat2(1.f));
+    float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    if constexpr (!FAST) r = fma2(r, fma2(make_float2(-d.x, -d.y), r, splat2(1.f)), r);
+    rest = mul2(e, r);
+    a = add2(r, splat2(-0x1p-126f));
+}
+
+__device__ __forceinline__ bool finite(float2 v) { return fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f; }
+
+// One step's decay and input from its gate and x; `rest` is 1 - a (sigmoid only).
+template <int GATE, bool FAST> __device__ __forceinline__ void gate_step(float2 g, float2 x, float2 &a, float2 &b, float2 &rest) {
+    if constexpr (GATE == HX_GATE_SIGMOID) {
+        sigmoid2<FAST>(g, a, rest);
+        b = mul2(rest, x);
+    } else {
         a = g;
         b = x;
-    } else {
-        float rest;
-        sigmoid_pair(g, a, rest);
-        b = rest * x;
     }
 }
 
-template <typename T, int GATE>
-__global__ void __launch_bounds__(128) gated_scan_kernel(const hx_gated_scan_args p) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (int64_t)p.batch * p.d_inner) return;
-    const int b = (int)(i / p.d_inner), d = (int)(i % p.d_inner);
-    const T *x = static_cast<const T *>(p.x) + b * p.x_batch_stride + d;
-    const T *g = static_cast<const T *>(p.g) + b * p.g_batch_stride + d;
-    T *out = static_cast<T *>(p.h) + b * p.h_batch_stride + d;
-    const int len = p.lengths ? min(max(p.lengths[b], 0), p.seq_len) : p.seq_len;
-    const int64_t tiles = (p.seq_len + (int64_t)kStateSteps - 1) / kStateSteps;
-    float h = p.h0 ? p.h0[i] : 0.f;
-    for (int t = 0; t < len; ++t) {
-        if (p.states && t % kStateSteps == 0) p.states[(b * tiles + t / kStateSteps) * p.d_inner + d] = h;
-        float a, in;
-        decay_and_input<GATE>(ld_f32(g + t * p.g_row_stride), ld_f32(x + t * p.x_row_stride), a, in);
-        h = fmaf(a, h, in);
-        st_f32(out + t * p.h_row_stride, h);
-    }
-    for (int64_t t = len; t < p.seq_len; ++t) st_f32(out + t * p.h_row_stride, 0.f);
-    if (p.h_last) p.h_last[i] = h;
+// What one warp works on.
+struct Part {
+    int b, d0, seg, lane, c, n, cols;   // batch row, first channel of the tile, segment; the lane's channels c.. and how many exist
+    int len;                            // of the batch row
+    int t0, t1;                         // the segment's steps, inside len
+    bool live;
+};
+__device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, const int32_t *lengths, int seg_len, int segs) {
+    Part q;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int tiles = (d_inner + kC - 1) / kC;
+    const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
+    q.live = w < (int64_t)tiles * batch * segs;
+    const int64_t row = q.live ? w / tiles : 0;
+    q.d0 = q.live ? (int)(w % tiles) * kC : 0;
+    q.b = (int)(row % batch);
+    q.seg = (int)(row / batch);
+    q.lane = threadIdx.x & 31;
+    q.c = q.d0 + 2 * q.lane;
+    q.cols = d_inner - q.d0;
+    q.n = min(max(d_inner - q.c, 0), 2);
+    q.len = lengths ? min(max(lengths[q.b], 0), seq_len) : seq_len;
+    q.t0 = (int)min((int64_t)q.seg * seg_len, (int64_t)q.len);
+    q.t1 = (int)min((int64_t)(q.seg + 1) * seg_len, (int64_t)q.len);
+    return q;
+}
+// maps: [segment][batch][d_inner rounded up to 2] pairs (A, B) of a channel
+__device__ __forceinline__ float4 *map_at(float2 *maps, int seg, int b, int c, int batch, int d_inner) {
+    return reinterpret_cast<float4 *>(maps + ((int64_t)seg * batch + b) * ((d_inner + 1) & ~1) + c);
 }
 
-template <typename T, int GATE>
-__global__ void __launch_bounds__(128) gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (int64_t)p.batch * p.d_inner) return;
-    const int b = (int)(i / p.d_inner), d = (int)(i % p.d_inner);
-    const T *x = static_cast<const T *>(p.x) + b * p.x_batch_stride + d;
-    const T *g = static_cast<const T *>(p.g) + b * p.g_batch_stride + d;
-    const T *dh = static_cast<const T *>(p.dh) + b * p.dh_batch_stride + d;
-    T *dx = static_cast<T *>(p.dx) + b * p.dx_batch_stride + d;
-    T *dg = static_cast<T *>(p.dg) + b * p.dg_batch_stride + d;
-    const int len = p.lengths ? min(max(p.lengths[b], 0), p.seq_len) : p.seq_len;
-    const int64_t tiles = (p.seq_len + (int64_t)kStateSteps - 1) / kStateSteps;
-    for (int64_t t = len; t < p.seq_len; ++t) {
-        st_f32(dx + t * p.dx_row_stride, 0.f);
-        st_f32(dg + t * p.dg_row_stride, 0.f);
-    }
-    float e = p.dh_last ? p.dh_last[i] : 0.f;   // a_{t+1} delta_{t+1}
-    float before[kStateSteps];
-    for (int tile = (len + kStateSteps - 1) / kStateSteps - 1; tile >= 0; --tile) {
-        const int t0 = tile * kStateSteps, n = min(kStateSteps, len - t0);
-        float h = p.states[(b * tiles + tile) * p.d_inner + d];
-        for (int k = 0; k < n; ++k) {
-            before[k] = h;
-            float a, in;
-            decay_and_input<GATE>(ld_f32(g + (t0 + k) * p.g_row_stride), ld_f32(x + (t0 + k) * p.x_row_stride), a, in);
-            h = fmaf(a, h, in);
-        }
-        for (int k = n - 1; k >= 0; --k) {
-            const int64_t t = t0 + k;
-            const float delta = ld_f32(dh + t * p.dh_row_stride) + e;
-            const float gv = ld_f32(g + t * p.g_row_stride);
-            if constexpr (GATE == HX_GATE_DECAY) {
-                st_f32(dx + t * p.dx_row_stride, delta);
-                st_f32(dg + t * p.dg_row_stride, delta * before[k]);
-                e = gv * delta;
+// ---------------------------------------------------------------- forward
+// MAP: writes the maps of segments 0 .. segs - 2.  Otherwise: outputs of all segments.
+template <typename T, int GATE, int PIECE, bool MAP>
+__global__ void __launch_bounds__(32 * kWarps, kOccupancy)
+gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int segs) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr int STAGES = kStages;
+    extern __shared__ __align__(16) unsigned char smem[];
+    using Ring = T[STAGES][2][kRun][kC];
+    Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
+    if constexpr (MAP) chain_trigger();
+    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, seg_len, MAP ? segs - 1 : segs);
+    if (!q.live) return;
+    const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
+    const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
+    const int runs = (q.t1 - q.t0 + kRun - 1) / kRun;
+    // MAP walks from the last run to the first
+    const int64_t first = q.t0 + (int64_t)(MAP ? runs - 1 : 0) * kRun;
+    Feed<kRun, PIECE, T> feed_g(g, first, p.g_row_stride, MAP ? -kRun : kRun, q.cols, q.lane);
+    Feed<kRun, PIECE, T> feed_x(x, first, p.x_row_stride, MAP ? -kRun : kRun, q.cols, q.lane);
+    constexpr uint32_t slot_bytes = sizeof(ring[0]), ring_bytes = sizeof(ring);
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(&ring[0][0][0][0]);
+    const int ragged = (q.t1 - q.t0) % kRun;   // rows of the last run, 0: all
+    uint32_t to = 0;                           // slot that is filled next
+    auto issue = [&](int r) {                  // the r-th run of the walk
+        if (r < runs) {
+            __syncwarp();   // the warp is done with what the slot held
+            const uint32_t slot = ring0 + to;
+            if (ragged && r == (MAP ? 0 : runs - 1)) {
+                feed_g.part(slot, ragged);
+                feed_x.part(slot + slot_bytes / 2, ragged);
             } else {
-                float a, rest;
-                sigmoid_pair(gv, a, rest);
-                st_f32(dx + t * p.dx_row_stride, delta * rest);
-                st_f32(dg + t * p.dg_row_stride, delta * (before[k] - ld_f32(x + t * p.x_row_stride)) * a * rest);
-                e = a * delta;
+                feed_g.whole(slot);
+                feed_x.whole(slot + slot_bytes / 2);
+            }
+            to = to + slot_bytes == ring_bytes ? 0 : to + slot_bytes;
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int r = 0; r < STAGES - 1; ++r) issue(r);
+
+    float2 h = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);   // MAP: B and A of the steps walked so far
+    T *out = static_cast<T *>(p.h) + q.b * p.h_batch_stride + q.c;
+    const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
+    float *states = !MAP && p.states ? p.states + q.b * blocks * p.d_inner + q.c : nullptr;
+    const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2, even = p.d_inner % 2 == 0;
+    if constexpr (!MAP) {
+        if (p.h0) h = load_some(p.h0 + (int64_t)q.b * p.d_inner + q.c, q.n);
+        if (segs > 1) {
+            chain_wait();
+            bool odd = false;
+            int j = 0;
+            for (; j < q.seg && !odd; j += 4) {
+                float4 m[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    m[k] = j + k < q.seg && q.n ? *map_at(maps, j + k, q.b, q.c, p.batch, p.d_inner) : make_float4(1.f, 0.f, 1.f, 0.f);
+                float2 next = h;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    next = make_float2(fmaf(m[k].x, next.x, m[k].y), fmaf(m[k].z, next.y, m[k].w));
+                    odd |= !finite(next) || !finite(make_float2(m[k].x, m[k].z));
+                }
+                odd = __any_sync(0xffffffffu, odd);
+                if (odd) break;   // h is the state before segment j
+                h = next;
+            }
+            if (odd)
+                for (int64_t t = (int64_t)j * seg_len; t < q.t0; ++t) {
+                    float2 a, b, rest;
+                    gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), load_some(x + t * p.x_row_stride + 2 * q.lane, q.n), a, b, rest);
+                    h = fma2(a, h, b);
+                }
+        }
+    }
+    const T *slot_g = &ring[0][0][0][2 * q.lane], *const slot_end = slot_g + STAGES * 2 * kRun * kC;
+    T *o = out + q.t0 * p.h_row_stride;
+    float *st = states ? states + (int64_t)(q.t0 / kBlock) * p.d_inner : nullptr;
+    bool keep = states != nullptr;   // every other run starts at a state to be kept
+    for (int r = 0; r < runs; ++r) {
+        cp_wait<STAGES - 2>();
+        __syncwarp();
+        float2 a[kRun], v[kRun];
+#pragma unroll
+        for (int s = 0; s < kRun; ++s) {
+            float2 rest;
+            gate_step<GATE, FAST>(load2(slot_g + s * kC), load2(slot_g + (kRun + s) * kC), a[s], v[s], rest);
+        }
+        slot_g += 2 * kRun * kC;
+        if (slot_g == slot_end) slot_g = &ring[0][0][0][2 * q.lane];
+        issue(r + STAGES - 1);
+        const int rows = ragged && r == (MAP ? 0 : runs - 1) ? ragged : kRun;
+        if constexpr (MAP) {
+            if (rows == kRun) {
+#pragma unroll
+                for (int s = kRun - 1; s >= 0; --s) {
+                    h = fma2(A, v[s], h);
+                    A = mul2(A, a[s]);
+                }
+            } else {
+#pragma unroll
+                for (int s = kRun - 1; s >= 0; --s)
+                    if (s < rows) {
+                        h = fma2(A, v[s], h);
+                        A = mul2(A, a[s]);
+                    }
+            }
+        } else {
+            if (keep) {
+                if (even && q.n == 2) store2(st, h);
+                else store_some(st, h, q.n);
+                st += p.d_inner;
+            }
+            keep = !keep && states;
+            if (rows == kRun && whole) {
+#pragma unroll
+                for (int s = 0; s < kRun; ++s) {
+                    h = fma2(a[s], h, v[s]);
+                    store2(o, h);
+                    o += p.h_row_stride;
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kRun; ++s)
+                    if (s < rows) {
+                        h = fma2(a[s], h, v[s]);
+                        store_some(o, h, q.n);
+                        o += p.h_row_stride;
+                    }
             }
         }
     }
-    if (p.dh0) p.dh0[i] = e;
+    if constexpr (MAP) {
+        if (q.n) *map_at(maps, q.seg, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, h.x, A.y, h.y);
+    } else {
+        const int64_t end = q.seg == segs - 1 ? p.seq_len : min((int64_t)(q.seg + 1) * seg_len, (int64_t)p.seq_len);
+        for (int64_t t = max((int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) store_some(out + t * p.h_row_stride, make_float2(0.f, 0.f), q.n);
+        if (p.h_last && q.seg == segs - 1) store_some(p.h_last + (int64_t)q.b * p.d_inner + q.c, h, q.n);
+    }
 }
 
+// ---------------------------------------------------------------- backward
+// MAP: writes the maps e behind the segment -> e before it, of segments 1 .. segs - 1, walking forward.  Otherwise: the gradients,
+// walking from the end.
+template <typename T, int GATE, int PIECE, bool MAP>
+__global__ void __launch_bounds__(32 * kWarps, MAP ? kOccupancy : kBlockOccupancy)
+gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len, int segs) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr int STAGES = MAP ? kStages : kBlockStages, ROWS = MAP ? kRun : kBlock, TENSORS = MAP ? 2 : 3;
+    extern __shared__ __align__(16) unsigned char smem[];
+    using Ring = T[STAGES][TENSORS][ROWS][kC];   // g, dh, x
+    Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
+    if constexpr (MAP) chain_trigger();
+    Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, seg_len, MAP ? segs - 1 : segs);
+    if (!q.live) return;
+    if constexpr (MAP) {
+        ++q.seg;
+        q.t0 = (int)min((int64_t)q.seg * seg_len, (int64_t)q.len);
+        q.t1 = (int)min((int64_t)(q.seg + 1) * seg_len, (int64_t)q.len);
+    }
+    const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
+    const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
+    const T *dh = static_cast<const T *>(p.dh) + q.b * p.dh_batch_stride + q.d0;
+    const int runs = (q.t1 - q.t0 + ROWS - 1) / ROWS;
+    const int64_t first = q.t0 + (int64_t)(MAP ? 0 : runs - 1) * ROWS;
+    constexpr int way = MAP ? ROWS : -ROWS;
+    Feed<ROWS, PIECE, T> feed_g(g, first, p.g_row_stride, way, q.cols, q.lane);
+    Feed<ROWS, PIECE, T> feed_d(dh, first, p.dh_row_stride, way, q.cols, q.lane);
+    Feed<ROWS, PIECE, T> feed_x(x, first, p.x_row_stride, way, q.cols, q.lane);
+    constexpr uint32_t part_bytes = sizeof(ring[0][0]), slot_bytes = sizeof(ring[0]), ring_bytes = sizeof(ring);
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(&ring[0][0][0][0]);
+    const int ragged = (q.t1 - q.t0) % ROWS;
+    uint32_t to = 0;
+    auto issue = [&](int r) {
+        if (r < runs) {
+            __syncwarp();
+            const uint32_t slot = ring0 + to;
+            if (ragged && r == (MAP ? runs - 1 : 0)) {
+                feed_g.part(slot, ragged);
+                feed_d.part(slot + part_bytes, ragged);
+                if constexpr (!MAP) feed_x.part(slot + 2 * part_bytes, ragged);
+            } else {
+                feed_g.whole(slot);
+                feed_d.whole(slot + part_bytes);
+                if constexpr (!MAP) feed_x.whole(slot + 2 * part_bytes);
+            }
+            to = to + slot_bytes == ring_bytes ? 0 : to + slot_bytes;
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int r = 0; r < STAGES - 1; ++r) issue(r);
+    const T *slot = &ring[0][0][0][2 * q.lane], *const slot_end = slot + STAGES * TENSORS * ROWS * kC;
+
+    if constexpr (MAP) {
+        float2 E = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);
+        for (int r = 0; r < runs; ++r) {
+            cp_wait<STAGES - 2>();
+            __syncwarp();
+            float2 a[kRun], v[kRun];
+#pragma unroll
+            for (int s = 0; s < kRun; ++s) {
+                float2 rest, b;
+                v[s] = load2(slot + (ROWS + s) * kC);
+                gate_step<GATE, FAST>(load2(slot + s * kC), v[s], a[s], b, rest);
+            }
+            slot += TENSORS * ROWS * kC;
+            if (slot == slot_end) slot = &ring[0][0][0][2 * q.lane];
+            issue(r + STAGES - 1);
+            if (ragged && r == runs - 1) {
+#pragma unroll
+                for (int s = 0; s < kRun; ++s)
+                    if (s < ragged) {
+                        A = mul2(A, a[s]);
+                        E = fma2(A, v[s], E);
+                    }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kRun; ++s) {
+                    A = mul2(A, a[s]);
+                    E = fma2(A, v[s], E);
+                }
+            }
+        }
+        if (q.n) *map_at(maps, q.seg - 1, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, E.x, A.y, E.y);
+    } else {
+        float2 e = p.dh_last ? load_some(p.dh_last + (int64_t)q.b * p.d_inner + q.c, q.n) : make_float2(0.f, 0.f);
+        const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
+        const bool even = p.d_inner % 2 == 0;
+        auto state_of = [&](int r) {   // the state before the r-th block of the walk
+            if (r >= runs) return make_float2(0.f, 0.f);
+            const float *st = p.states + (q.b * blocks + q.t0 / kBlock + (runs - 1 - r)) * p.d_inner + q.c;
+            return even && q.n == 2 ? load2(st) : load_some(st, q.n);
+        };
+        float2 state = state_of(0);
+        if (segs > 1) {
+            chain_wait();
+            bool odd = false;
+            int j = segs - 1;
+            for (; j > q.seg && !odd; j -= 4) {
+                float4 m[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    m[k] = j - k > q.seg && q.n ? *map_at(maps, j - k - 1, q.b, q.c, p.batch, p.d_inner) : make_float4(1.f, 0.f, 1.f, 0.f);
+                float2 next = e;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    next = make_float2(fmaf(m[k].x, next.x, m[k].y), fmaf(m[k].z, next.y, m[k].w));
+                    odd |= !finite(next) || !finite(make_float2(m[k].x, m[k].z));
+                }
+                odd = __any_sync(0xffffffffu, odd);
+                if (odd) break;   // e is the one behind segment j
+                e = next;
+            }
+            if (odd)
+                for (int64_t t = min((int64_t)(j + 1) * seg_len, (int64_t)q.len) - 1; t >= q.t1; --t) {
+                    float2 a, b, rest;
+                    const float2 d = load_some(dh + t * p.dh_row_stride + 2 * q.lane, q.n);
+                    gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), d, a, b, rest);
+                    e = mul2(a, add2(e, d));
+                }
+        }
+        const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2;
+        T *dx = static_cast<T *>(p.dx) + q.b * p.dx_batch_stride + q.c;
+        T *dg = static_cast<T *>(p.dg) + q.b * p.dg_batch_stride + q.c;
+        T *ox = dx + ((int64_t)q.t1 - 1) * p.dx_row_stride, *og = dg + ((int64_t)q.t1 - 1) * p.dg_row_stride;
+        for (int r = 0; r < runs; ++r) {
+            cp_wait<STAGES - 2>();
+            __syncwarp();
+            const int rows = ragged && r == 0 ? ragged : kBlock;
+            float2 a[kBlock], rest[kBlock], before[kBlock];
+            const float2 next_state = state_of(r + 1);
+#pragma unroll
+            for (int s = 0; s < kBlock; ++s) {   // rows behind the end are zeros here: what they give is not used
+                float2 b;
+                gate_step<GATE, FAST>(load2(slot + s * kC), load2(slot + (2 * kBlock + s) * kC), a[s], b, rest[s]);
+                before[s] = state;
+                state = fma2(a[s], state, b);
+            }
+            state = next_state;
+            issue(r + STAGES - 1);
+            auto gradients = [&](int s, float2 &dxv, float2 &dgv) {
+                const float2 d = add2(load2(slot + (kBlock + s) * kC), e);   // delta
+                e = mul2(a[s], d);
+                if constexpr (GATE == HX_GATE_SIGMOID) {
+                    dxv = mul2(d, rest[s]);
+                    // delta (h - x) a (1 - a), with e = a delta
+                    dgv = mul2(mul2(e, rest[s]), fma2(load2(slot + (2 * kBlock + s) * kC), make_float2(-1.f, -1.f), before[s]));
+                } else {
+                    dxv = d;
+                    dgv = mul2(d, before[s]);
+                }
+            };
+            float2 dxv, dgv;
+            if (rows == kBlock && whole) {
+#pragma unroll
+                for (int s = kBlock - 1; s >= 0; --s) {
+                    gradients(s, dxv, dgv);
+                    store2(ox, dxv);
+                    store2(og, dgv);
+                    ox -= p.dx_row_stride;
+                    og -= p.dg_row_stride;
+                }
+            } else {
+#pragma unroll
+                for (int s = kBlock - 1; s >= 0; --s)
+                    if (s < rows) {
+                        gradients(s, dxv, dgv);
+                        store_some(ox, dxv, q.n);
+                        store_some(og, dgv, q.n);
+                        ox -= p.dx_row_stride;
+                        og -= p.dg_row_stride;
+                    }
+            }
+            slot += TENSORS * ROWS * kC;
+            if (slot == slot_end) slot = &ring[0][0][0][2 * q.lane];
+        }
+        const int64_t end = q.seg == segs - 1 ? p.seq_len : min((int64_t)(q.seg + 1) * seg_len, (int64_t)p.seq_len);
+        for (int64_t t = max((int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) {
+            store_some(dx + t * p.dx_row_stride, make_float2(0.f, 0.f), q.n);
+            store_some(dg + t * p.dg_row_stride, make_float2(0.f, 0.f), q.n);
+        }
+        if (p.dh0 && q.seg == 0) store_some(p.dh0 + (int64_t)q.b * p.d_inner + q.c, e, q.n);
+    }
+}
+
+// ---------------------------------------------------------------- one token
+// Two channels a thread, so that a row's halves of a projection are read in words where they are aligned (`pairs`).
 template <typename T, int GATE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 gated_step_kernel(const T *x, int64_t x_stride, const T *g, int64_t g_stride, const float *h, float *h_out, T *y, int64_t y_stride,
-                  int batch, int d_inner) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (int64_t)batch * d_inner) return;
-    const int b = (int)(i / d_inner), d = (int)(i % d_inner);
-    float a, in;
-    decay_and_input<GATE>(ld_f32(g + b * g_stride + d), ld_f32(x + b * x_stride + d), a, in);
-    const float v = fmaf(a, h[i], in);
-    h_out[i] = v;
-    st_f32(y + b * y_stride + d, v);
+                  int batch, int d_inner, bool pairs) {
+    const int half = (d_inner + 1) / 2;
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (i >= (int64_t)batch * half) return;
+    const int b = (int)(i / half), d = (int)(i % half) * 2, n = min(d_inner - d, 2);
+    const int64_t at = (int64_t)b * d_inner + d;
+    x += b * x_stride + d;
+    g += b * g_stride + d;
+    y += b * y_stride + d;
+    float2 a, in, rest;
+    if (pairs) {
+        gate_step<GATE, false>(load2(g), load2(x), a, in, rest);
+        const float2 v = fma2(a, load2(h + at), in);
+        store2(h_out + at, v);
+        store2(y, v);
+    } else {
+        gate_step<GATE, false>(load_some(g, n), load_some(x, n), a, in, rest);
+        const float2 v = fma2(a, load_some(h + at, n), in);
+        store_some(h_out + at, v, n);
+        store_some(y, v, n);
+    }
 }
 
 // Rows of an output [B, L, D] with these strides do not overlap.
@@ -126,21 +571,107 @@ static hx_status check_common(const char *who, int batch, int seq_len, int d_inn
     return HX_OK;
 }
 
+// The largest of 16, 4 and the element size that divides every address the kernel forms.
+static int piece_of(size_t element, std::initializer_list<const void *> bases, std::initializer_list<int64_t> strides) {
+    uint64_t bits = 0;
+    for (const void *p : bases) bits |= (uint64_t)(uintptr_t)p;
+    for (int64_t s : strides) bits |= (uint64_t)s * element;
+    return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : (int)element;
+}
+
+// How the sequence is cut.  One segment where a step's channels are at least kStepBytes: a warp takes about 0.04 us a step however
+// little else runs, so from there on a single pass is done before two passes (five tensors instead of three, seven instead of five)
+// have moved their bytes.  16 x 2048 x 1536 fp32 sigmoid: 111 us whole, 144 in two; 4 x 4096 x 1024 bf16: 182 whole, 40 in 27.
+// Otherwise as many segments as give an SM kWarpBytes / element size warps (1 x 16384 x 1536 bf16: 60 us with 64 segments, 67 with
+// 32 or 128; 1 x 32768 x 1536 fp32: 169, 166, 175 us with 16, 32, 64).
+constexpr int64_t kStepBytes = 45000, kWarpBytes = 24;
+struct Plan { int segs, seg_len; };
+static Plan plan_of(int batch, int seq_len, int d_inner, int io_dtype) {
+    const int64_t chains = (int64_t)batch * ((d_inner + kC - 1) / kC), e = (int64_t)dtype_size(io_dtype);
+    int64_t segs = 1;
+    if ((int64_t)batch * d_inner * e < kStepBytes) segs = std::max<int64_t>(kWarpBytes / e * sm_count() / chains, 1);
+    int64_t seg_len = (seq_len + segs - 1) / segs;
+    seg_len = std::max<int64_t>((seg_len + kBlock - 1) / kBlock * kBlock, 2 * kBlock);
+    segs = std::max<int64_t>((seq_len + seg_len - 1) / seg_len, 1);
+    return {(int)segs, (int)std::min<int64_t>(seg_len, 0x7fffffff / kBlock * kBlock)};
+}
+static size_t map_bytes(int batch, int d_inner, const Plan &plan) {
+    return (size_t)(plan.segs - 1) * batch * ((d_inner + 1) & ~1) * sizeof(float2);
+}
+
+template <typename K, typename Args>
+static hx_status launch(K kernel, size_t ring, bool chained, int64_t warps, const Args &args, const Plan &plan, const char *name, cudaStream_t st) {
+    const int64_t ctas = (warps + kWarps - 1) / kWarps;
+    HX_REQUIRE(ctas <= 0x7fffffff, HX_ERR_INVALID_DIMENSION, "%s: batch * d_inner is too large for one launch", name);
+    HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kWarps * ring)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = kWarps * ring;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = chained ? 1 : 0;
+    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args, static_cast<float2 *>(args.workspace), plan.seg_len, plan.segs));
+    return check_launch(name);
+}
+template <typename T, int GATE, int PIECE> static hx_status launch_fwd(const hx_gated_scan_args &a, const Plan &plan, cudaStream_t st) {
+    const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
+    const size_t ring = sizeof(T[kStages][2][kRun][kC]);
+    if (plan.segs > 1) {
+        const hx_status s = launch(gated_scan_kernel<T, GATE, PIECE, true>, ring, false, chains * (plan.segs - 1), a, plan, "gated_scan_kernel", st);
+        if (s != HX_OK) return s;
+    }
+    return launch(gated_scan_kernel<T, GATE, PIECE, false>, ring, plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_kernel", st);
+}
+template <typename T, int GATE, int PIECE> static hx_status launch_bwd(const hx_gated_scan_bwd_args &a, const Plan &plan, cudaStream_t st) {
+    const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
+    if (plan.segs > 1) {
+        const hx_status s = launch(gated_scan_bwd_kernel<T, GATE, PIECE, true>, sizeof(T[kStages][2][kRun][kC]), false, chains * (plan.segs - 1), a, plan, "gated_scan_bwd_kernel", st);
+        if (s != HX_OK) return s;
+    }
+    return launch(gated_scan_bwd_kernel<T, GATE, PIECE, false>, sizeof(T[kBlockStages][3][kBlock][kC]), plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_bwd_kernel", st);
+}
+// The plan a call may use: one segment where it brings no workspace.
+template <typename Args> static hx_status choose_plan(const char *who, const Args &a, Plan *plan) {
+    *plan = plan_of(a.batch, a.seq_len, a.d_inner, a.io_dtype);
+    if (plan->segs == 1) return HX_OK;
+    if (a.workspace == nullptr) {
+        plan->segs = 1;
+        plan->seg_len = 0x7fffffff / kBlock * kBlock;
+        return HX_OK;
+    }
+    const size_t need = map_bytes(a.batch, a.d_inner, *plan);
+    HX_REQUIRE(a.workspace_bytes >= need, HX_ERR_INVALID_INPUT, "%s: a workspace of %zu bytes, %zu are needed", who, a.workspace_bytes, need);
+    HX_REQUIRE(((uintptr_t)a.workspace & 15) == 0, HX_ERR_INVALID_INPUT, "%s: the workspace must be 16-byte aligned", who);
+    return HX_OK;
+}
+
 }  // namespace gated
 }  // namespace hx
 
 using namespace hx;
 using namespace hx::gated;
 
-#define HX_GATED_LAUNCH(KERNEL, GATE, DTYPE, ...)                                                              \
-    do {                                                                                                       \
-        if ((DTYPE) == HX_BF16) {                                                                              \
-            if ((GATE) == HX_GATE_DECAY) KERNEL<__nv_bfloat16, HX_GATE_DECAY> __VA_ARGS__;                     \
-            else KERNEL<__nv_bfloat16, HX_GATE_SIGMOID> __VA_ARGS__;                                           \
-        } else {                                                                                               \
-            if ((GATE) == HX_GATE_DECAY) KERNEL<float, HX_GATE_DECAY> __VA_ARGS__;                             \
-            else KERNEL<float, HX_GATE_SIGMOID> __VA_ARGS__;                                                   \
-        }                                                                                                      \
+// Picks the instance for a type, a gate and an alignment.
+#define HX_GATED_PIECE(FN, T, GATE, PIECE, ...)                                                              \
+    do {                                                                                                     \
+        if ((PIECE) == 16) return FN<T, GATE, 16>(__VA_ARGS__);                                              \
+        if ((PIECE) >= 4) return FN<T, GATE, 4>(__VA_ARGS__);                                                \
+        if constexpr (sizeof(T) == 2) return FN<T, GATE, 2>(__VA_ARGS__);                                    \
+    } while (0)
+#define HX_GATED_LAUNCH(FN, GATE, DTYPE, PIECE, ...)                                                         \
+    do {                                                                                                     \
+        if ((DTYPE) == HX_BF16) {                                                                            \
+            if ((GATE) == HX_GATE_DECAY) HX_GATED_PIECE(FN, __nv_bfloat16, HX_GATE_DECAY, PIECE, __VA_ARGS__); \
+            else HX_GATED_PIECE(FN, __nv_bfloat16, HX_GATE_SIGMOID, PIECE, __VA_ARGS__);                     \
+        } else {                                                                                             \
+            if ((GATE) == HX_GATE_DECAY) HX_GATED_PIECE(FN, float, HX_GATE_DECAY, PIECE, __VA_ARGS__);       \
+            else HX_GATED_PIECE(FN, float, HX_GATE_SIGMOID, PIECE, __VA_ARGS__);                             \
+        }                                                                                                    \
+        return HX_ERR_BACKEND;                                                                               \
     } while (0)
 
 extern "C" {
@@ -157,9 +688,20 @@ hx_status hx_gated_scan_fwd(const hx_gated_scan_args *a, void *stream) {
                HX_ERR_INVALID_INPUT, "hx_gated_scan_fwd: negative stride");
     HX_REQUIRE(rows_apart(a->h_batch_stride, a->h_row_stride, a->batch, a->seq_len, a->d_inner), HX_ERR_SHAPE_MISMATCH,
                "hx_gated_scan_fwd: rows of h overlap (strides %lld, %lld)", (long long)a->h_batch_stride, (long long)a->h_row_stride);
-    const dim3 grid((unsigned)((chains + 127) / 128));
-    HX_GATED_LAUNCH(gated_scan_kernel, a->gate, a->io_dtype, <<<grid, 128, 0, (cudaStream_t)stream>>>(*a));
-    return check_launch("gated_scan_kernel");
+    const int piece = piece_of(dtype_size(a->io_dtype), {a->x, a->g, a->h},
+                               {a->x_batch_stride, a->x_row_stride, a->g_batch_stride, a->g_row_stride, a->h_batch_stride, a->h_row_stride});
+    Plan plan;
+    const hx_status ps = choose_plan("hx_gated_scan_fwd", *a, &plan);
+    if (ps != HX_OK) return ps;
+    HX_GATED_LAUNCH(launch_fwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
+}
+
+hx_status hx_gated_scan_workspace_bytes(int32_t batch, int32_t seq_len, int32_t d_inner, int32_t io_dtype, size_t *bytes) {
+    HX_REQUIRE(bytes != nullptr, HX_ERR_INVALID_INPUT, "hx_gated_scan_workspace_bytes: bytes is NULL");
+    const hx_status s = check_common("hx_gated_scan_workspace_bytes", batch, seq_len, d_inner, HX_GATE_DECAY, io_dtype);
+    if (s != HX_OK) return s;
+    *bytes = (int64_t)batch * d_inner == 0 ? 0 : map_bytes(batch, d_inner, plan_of(batch, seq_len, d_inner, io_dtype));
+    return HX_OK;
 }
 
 hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *a, void *stream) {
@@ -177,9 +719,13 @@ hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *a, void *stream) {
     HX_REQUIRE(rows_apart(a->dx_batch_stride, a->dx_row_stride, a->batch, a->seq_len, a->d_inner) &&
                    rows_apart(a->dg_batch_stride, a->dg_row_stride, a->batch, a->seq_len, a->d_inner),
                HX_ERR_SHAPE_MISMATCH, "hx_gated_scan_bwd: rows of dx or dg overlap");
-    const dim3 grid((unsigned)((chains + 127) / 128));
-    HX_GATED_LAUNCH(gated_scan_bwd_kernel, a->gate, a->io_dtype, <<<grid, 128, 0, (cudaStream_t)stream>>>(*a));
-    return check_launch("gated_scan_bwd_kernel");
+    const int piece = piece_of(dtype_size(a->io_dtype), {a->x, a->g, a->dh, a->dx, a->dg},
+                               {a->x_batch_stride, a->x_row_stride, a->g_batch_stride, a->g_row_stride, a->dh_batch_stride,
+                                a->dh_row_stride, a->dx_batch_stride, a->dx_row_stride, a->dg_batch_stride, a->dg_row_stride});
+    Plan plan;
+    const hx_status ps = choose_plan("hx_gated_scan_bwd", *a, &plan);
+    if (ps != HX_OK) return ps;
+    HX_GATED_LAUNCH(launch_bwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
 }
 
 hx_status hx_gated_scan_step(const void *x, int64_t x_row_stride, const void *g, int64_t g_row_stride, const float *h, float *h_out,
@@ -193,22 +739,23 @@ hx_status hx_gated_scan_step(const void *x, int64_t x_row_stride, const void *g,
     HX_REQUIRE(x_row_stride >= 0 && g_row_stride >= 0, HX_ERR_INVALID_INPUT, "hx_gated_scan_step: negative stride");
     HX_REQUIRE(batch <= 1 || y_row_stride >= d_inner, HX_ERR_SHAPE_MISMATCH, "hx_gated_scan_step: rows of y overlap (stride %lld)",
                (long long)y_row_stride);
-    const unsigned grid = (unsigned)((n + 255) / 256);
+    const int64_t grid = ((int64_t)batch * ((d_inner + 1) / 2) + 127) / 128;
+    HX_REQUIRE(grid <= 0x7fffffff, HX_ERR_INVALID_DIMENSION, "hx_gated_scan_step: batch * d_inner is too large for one launch");
+    const size_t e = dtype_size(io_dtype);
+    const uint64_t io = (uintptr_t)x | (uintptr_t)g | (uintptr_t)y | (uint64_t)(x_row_stride | g_row_stride | y_row_stride) * e;
+    const bool pairs = d_inner % 2 == 0 && io % (2 * e) == 0 && ((uintptr_t)h | (uintptr_t)h_out) % 8 == 0;
+#define HX_GATED_STEP(T, GATE)                                                                                               \
+    gated_step_kernel<T, GATE><<<(unsigned)grid, 128, 0, (cudaStream_t)stream>>>(                                            \
+        static_cast<const T *>(x), x_row_stride, static_cast<const T *>(g), g_row_stride, h, h_out, static_cast<T *>(y),     \
+        y_row_stride, batch, d_inner, pairs)
     if (io_dtype == HX_BF16) {
-        auto xp = static_cast<const __nv_bfloat16 *>(x), gp = static_cast<const __nv_bfloat16 *>(g);
-        auto yp = static_cast<__nv_bfloat16 *>(y);
-        if (gate == HX_GATE_DECAY)
-            gated_step_kernel<__nv_bfloat16, HX_GATE_DECAY><<<grid, 256, 0, (cudaStream_t)stream>>>(xp, x_row_stride, gp, g_row_stride, h, h_out, yp, y_row_stride, batch, d_inner);
-        else
-            gated_step_kernel<__nv_bfloat16, HX_GATE_SIGMOID><<<grid, 256, 0, (cudaStream_t)stream>>>(xp, x_row_stride, gp, g_row_stride, h, h_out, yp, y_row_stride, batch, d_inner);
+        if (gate == HX_GATE_DECAY) HX_GATED_STEP(__nv_bfloat16, HX_GATE_DECAY);
+        else HX_GATED_STEP(__nv_bfloat16, HX_GATE_SIGMOID);
     } else {
-        auto xp = static_cast<const float *>(x), gp = static_cast<const float *>(g);
-        auto yp = static_cast<float *>(y);
-        if (gate == HX_GATE_DECAY)
-            gated_step_kernel<float, HX_GATE_DECAY><<<grid, 256, 0, (cudaStream_t)stream>>>(xp, x_row_stride, gp, g_row_stride, h, h_out, yp, y_row_stride, batch, d_inner);
-        else
-            gated_step_kernel<float, HX_GATE_SIGMOID><<<grid, 256, 0, (cudaStream_t)stream>>>(xp, x_row_stride, gp, g_row_stride, h, h_out, yp, y_row_stride, batch, d_inner);
+        if (gate == HX_GATE_DECAY) HX_GATED_STEP(float, HX_GATE_DECAY);
+        else HX_GATED_STEP(float, HX_GATE_SIGMOID);
     }
+#undef HX_GATED_STEP
     return check_launch("gated_step_kernel");
 }
 

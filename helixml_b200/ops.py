@@ -183,14 +183,18 @@ def _on_device(**tensors):
     return dev
 
 
-def _run_on(dev, fn, *args):
-    """fn(*args, stream) on `dev` and the stream torch uses there, whichever device is the current one."""
-    stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+def _on(dev, fn, *args):
+    """fn(*args) with `dev` as the current device."""
     if dev.index == torch.cuda.current_device():
-        L.check(fn(*args, stream))
+        L.check(fn(*args))
     else:
         with torch.cuda.device(dev):
-            L.check(fn(*args, stream))
+            L.check(fn(*args))
+
+
+def _run_on(dev, fn, *args):
+    """fn(*args, stream) on `dev` and the stream torch uses there, whichever device is the current one."""
+    _on(dev, fn, *args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
 
 
 def _like(name, t, shape, dtype):
@@ -216,9 +220,20 @@ def _dense_out(name, t, shape, dtype):
 
 
 def gated_scan_states(batch, seq_len, d_inner, device="cuda"):
-    """The buffer in which gated_scan keeps what gated_scan_bwd starts from: the state before every 64th row, fp32."""
+    """The buffer in which gated_scan keeps what gated_scan_bwd starts from: the state before every 16th row, fp32."""
     steps = L.GATED_SCAN_STATE_STEPS
     return torch.empty((batch, (seq_len + steps - 1) // steps, d_inner), dtype=torch.float32, device=device)
+
+
+def _gated_scan_workspace(a, dev):
+    """The memory a call whose sequence is cut into segments needs; kept alive by the caller until the call is queued."""
+    n = C.c_size_t(0)
+    _on(dev, L.lib().hx_gated_scan_workspace_bytes, a.batch, a.seq_len, a.d_inner, a.io_dtype, C.byref(n))
+    if n.value == 0:
+        return None
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+    return ws
 
 
 def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_state=False, states=None):
@@ -247,6 +262,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     for name, t in (("h0", h0), ("h_last", last), ("states", states), ("lengths", lengths)):
         if t is not None:
             setattr(a, name, t.data_ptr())
+    ws = _gated_scan_workspace(a, dev)  # noqa: F841
     _run_on(dev, L.lib().hx_gated_scan_fwd, C.byref(a))
     return (h, last) if return_state else h
 
@@ -277,6 +293,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     for name, t in (("states", states), ("dh_last", dh_last), ("dh0", dh0), ("lengths", lengths)):
         if t is not None:
             setattr(a, name, t.data_ptr())
+    ws = _gated_scan_workspace(a, dev)  # noqa: F841
     _run_on(dev, L.lib().hx_gated_scan_bwd, C.byref(a))
     return dx, dg, dh0
 

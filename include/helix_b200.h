@@ -314,7 +314,7 @@ HX_API hx_status hx_s4_diag_fwd(const void *u, const float *A, const float *Bp, 
  * or an input. */
 typedef enum hx_gate_kind { HX_GATE_DECAY = 0, HX_GATE_SIGMOID = 1 } hx_gate_kind;
 /* Steps from one state kept for the backward pass to the next. */
-#define HX_GATED_SCAN_STATE_STEPS 64
+#define HX_GATED_SCAN_STATE_STEPS 16
 typedef struct hx_gated_scan_args {
     int32_t batch, seq_len, d_inner;
     int32_t io_dtype;         /* hx_dtype of x, g, h: HX_F32 or HX_BF16 */
@@ -326,12 +326,18 @@ typedef struct hx_gated_scan_args {
     int64_t g_batch_stride, g_row_stride;
     int64_t h_batch_stride, h_row_stride;
     const float *h0;          /* [batch, d_inner] fp32 or NULL */
-    float *h_last;            /* [batch, d_inner] fp32 or NULL; may be h0's buffer */
-    float *states;            /* NULL, or [batch, ceil(seq_len / 64), d_inner] fp32: the state before row 64 i, what the
-                                 backward pass starts from */
+    float *h_last;            /* [batch, d_inner] fp32 or NULL; not h0's buffer */
+    float *states;            /* NULL, or [batch, ceil(seq_len / 16), d_inner] fp32: the state before row 16 i, what the
+                                 backward pass starts from (rows of blocks behind len[b] are not written) */
     const int32_t *lengths;   /* [batch] or NULL */
+    void *workspace;          /* 16-byte aligned device memory of hx_gated_scan_workspace_bytes() bytes, in use until the call
+                                 has run; NULL: the sequence is not cut, which is slower where chains are few */
+    size_t workspace_bytes;
 } hx_gated_scan_args;
 HX_API hx_status hx_gated_scan_fwd(const hx_gated_scan_args *args, void *stream);
+/* Bytes of `workspace` for the forward and the backward pass of these sizes on the current device: 8 bytes per channel, batch row
+ * and segment the sequence is cut into (0: it is not). */
+HX_API hx_status hx_gated_scan_workspace_bytes(int32_t batch, int32_t seq_len, int32_t d_inner, int32_t io_dtype, size_t *bytes);
 
 /* Its gradients.  With dh = dL/dh and dh_last = dL/dh_last, from the end of each sequence:
  *   delta_t = dh_t + a_{t+1} delta_{t+1}   (behind the last row: dh_last)        dh0 = a_0 delta_0
@@ -353,8 +359,10 @@ typedef struct hx_gated_scan_bwd_args {
     int64_t dg_batch_stride, dg_row_stride;
     const float *states;      /* what hx_gated_scan_fwd wrote for the same x, g, h0 and lengths */
     const float *dh_last;     /* [batch, d_inner] fp32 or NULL */
-    float *dh0;               /* [batch, d_inner] fp32 or NULL */
+    float *dh0;               /* [batch, d_inner] fp32 or NULL; not dh_last's buffer */
     const int32_t *lengths;
+    void *workspace;          /* as in hx_gated_scan_args */
+    size_t workspace_bytes;
 } hx_gated_scan_bwd_args;
 HX_API hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *args, void *stream);
 

@@ -173,9 +173,17 @@ def test_without_state_and_optional_operands():
     for a, b in zip(ops.gated_scan_bwd(dh, x, g, states), ops.gated_scan_bwd(dh, x, g, states, dh_last=zero)):
         assert torch.equal(a, b)
     tol = 1e-5
-    for t, row in ((0, 0), (64, 1), (128, 2)):
+    for t, row in ((0, 0), (16, 1), (64, 4), (144, 9)):
         want = zero if t == 0 else h[:, t - 1]
         assert (states[:, row] - want).abs().max().item() <= tol
+
+
+@pytest.mark.parametrize("gate", ["decay", "sigmoid"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_without_workspace_the_sequence_is_walked_whole(dtype, gate, monkeypatch):
+    x, g, h0, dh, dh_last = inputs(18, 2, 777, 70, dtype, gate)
+    monkeypatch.setattr(ops, "_gated_scan_workspace", lambda a, dev: None)
+    check(x, g, h0, dh, dh_last, gate)
 
 
 @pytest.mark.parametrize("empty", [(0, 5, 8), (2, 0, 8), (2, 5, 0)])

@@ -66,6 +66,23 @@ def test_gated_scan_argument_errors():
             assert fn(gated(kind, **{empty: 0}), None) == 0
 
 
+def test_gated_scan_workspace():
+    lib = L.lib()
+    n = C.c_size_t(7)
+    q = lambda *a: (lib.hx_gated_scan_workspace_bytes(*a, C.byref(n)), n.value)
+    assert q(32, 2048, 1536, L.HX_BF16) == (0, 0)          # enough chains: the sequence is not cut
+    st, size = q(1, 4096, 257, L.HX_F32)
+    assert st == 0 and size > 0 and size % (8 * 258) == 0   # maps of whole pairs of channels
+    assert q(0, 4096, 257, L.HX_F32) == (0, 0) and q(1, 32, 257, L.HX_F32) == (0, 0)
+    assert q(-1, 5, 5, L.HX_F32)[0] == 2 and q(1, 5, 5, L.HX_U8)[0] == 4
+    assert lib.hx_gated_scan_workspace_bytes(1, 5, 5, L.HX_F32, None) == 10
+    for fn, kind in ((lib.hx_gated_scan_fwd, L.GatedScanArgs), (lib.hx_gated_scan_bwd, L.GatedScanBwdArgs)):
+        big = dict(batch=1, seq_len=4096, d_inner=8, workspace=256)
+        need = q(1, 4096, 8, L.HX_F32)[1]
+        assert fn(gated(kind, workspace_bytes=need - 1, **big), None) == 10 and b"needed" in lib.hx_last_error()
+        assert fn(gated(kind, workspace_bytes=need, **{**big, "workspace": 264}), None) == 10
+
+
 def test_gated_step_argument_errors():
     lib = L.lib()
 
