@@ -3,6 +3,7 @@ the C ABI on torch's current stream.  torch is used for device memory and stream
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -163,77 +164,93 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, conv_w=None, conv_b=None, d
 
 
 GATES = {"decay": L.GATE_DECAY, "sigmoid": L.GATE_SIGMOID}
+_FLOATS = {torch.float32: L.HX_F32, torch.bfloat16: L.HX_BF16}
+
+# The calls below are a few microseconds of GPU work each when one token is decoded, so what the host does for them counts: tensors
+# are checked by their own attributes, structures filled in one go, addresses handed over as plain integers.
 
 
 def _gate(gate) -> int:
-    if gate not in GATES:
+    code = GATES.get(gate)
+    if code is None:
         raise L.HxError(10, f"unknown gate {gate!r}: one of {sorted(GATES)}")
-    return GATES[gate]
+    return code
 
 
-def _on_device(**tensors):
-    """The one CUDA device all of these (None among them) are on."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda or (dev is not None and t.device != dev):
-            raise L.HxError(3, f"{name} is on {t.device}" + (f", expected {dev}" if dev is not None else ", expected a CUDA device"))
-        dev = t.device
+def _float(name, t) -> int:
+    code = _FLOATS.get(t.dtype)
+    if code is None:
+        raise L.HxError(4, f"{name} has dtype {t.dtype}, expected float32 or bfloat16")
+    return code
+
+
+def _cuda(name, t) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        raise L.HxError(3, f"{name} is on {t.device}, expected a CUDA device")
     return dev
 
 
-def _on(dev, fn, *args):
-    """fn(*args) with `dev` as the current device."""
-    if dev.index == torch.cuda.current_device():
-        L.check(fn(*args))
-    else:
-        with torch.cuda.device(dev):
-            L.check(fn(*args))
-
-
-def _run_on(dev, fn, *args):
-    """fn(*args, stream) on `dev` and the stream torch uses there, whichever device is the current one."""
-    _on(dev, fn, *args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-
-
-def _like(name, t, shape, dtype):
+def _like(name, t, shape, dtype, dev):
+    if t.get_device() != dev:
+        raise L.HxError(3, f"{name} is on {t.device}, expected cuda:{dev}")
     if t.dtype != dtype:
         raise L.HxError(4, f"{name} has dtype {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise L.HxError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _dense(name, t, shape, dtype):
+def _dense(name, t, shape, dtype, dev):
     """An operand the library takes without strides: checked, and copied where it is a strided view."""
     if t is None:
         return None
-    _like(name, t, shape, dtype)
+    _like(name, t, shape, dtype, dev)
     return t.contiguous()
 
 
-def _dense_out(name, t, shape, dtype):
-    _like(name, t, shape, dtype)
+def _dense_out(name, t, shape, dtype, dev):
+    _like(name, t, shape, dtype, dev)
     if not t.is_contiguous():
         raise L.HxError(1, f"{name} must be contiguous")
-    return t
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(dev, fn, *args):
+    """fn(*args, stream) on device `dev` and the stream torch uses there, whichever device is the current one."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)   # what torch.cuda.current_stream(dev).cuda_stream holds, at a tenth of its cost
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, stream)
+    if status:
+        L.check(status)
+
+
+@functools.lru_cache(maxsize=1024)
+def _gated_scan_workspace_bytes(dev, batch, seq_len, d_inner, dtype) -> int:
+    n = C.c_size_t(0)
+    with torch.cuda.device(dev):
+        L.check(L.lib().hx_gated_scan_workspace_bytes(batch, seq_len, d_inner, dtype, C.byref(n)))
+    return n.value
+
+
+def _gated_scan_workspace(dev, batch, seq_len, d_inner, dtype):
+    """The memory a call needs whose sequence is cut into segments."""
+    n = _gated_scan_workspace_bytes(dev, batch, seq_len, d_inner, dtype)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _state_rows(seq_len):
+    return (seq_len + L.GATED_SCAN_STATE_STEPS - 1) // L.GATED_SCAN_STATE_STEPS
 
 
 def gated_scan_states(batch, seq_len, d_inner, device="cuda"):
     """The buffer in which gated_scan keeps what gated_scan_bwd starts from: the state before every 16th row, fp32."""
-    steps = L.GATED_SCAN_STATE_STEPS
-    return torch.empty((batch, (seq_len + steps - 1) // steps, d_inner), dtype=torch.float32, device=device)
-
-
-def _gated_scan_workspace(a, dev):
-    """The memory a call whose sequence is cut into segments needs; kept alive by the caller until the call is queued."""
-    n = C.c_size_t(0)
-    _on(dev, L.lib().hx_gated_scan_workspace_bytes, a.batch, a.seq_len, a.d_inner, a.io_dtype, C.byref(n))
-    if n.value == 0:
-        return None
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-    return ws
+    return torch.empty((batch, _state_rows(seq_len), d_inner), dtype=torch.float32, device=device)
 
 
 def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_state=False, states=None):
@@ -241,29 +258,27 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
     lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
     states: a gated_scan_states buffer, filled for gated_scan_bwd.  Returns h, or (h, h_last [B, D] fp32) with return_state."""
-    dev = _on_device(x=x, g=g, h0=h0, lengths=lengths, out=out, states=states)
-    _view3(x)
-    Bsz, Lq, Dm = x.shape
-    a = L.GatedScanArgs()
-    a.batch, a.seq_len, a.d_inner, a.io_dtype, a.gate = Bsz, Lq, Dm, _dt(x), _gate(gate)
-    h = out if out is not None else torch.empty((Bsz, Lq, Dm), dtype=x.dtype, device=dev)
-    for name, t in (("x", x), ("g", g), ("h", h)):
-        _like(name, t, (Bsz, Lq, Dm), x.dtype)
-        bs, rs = _view3(t)
-        setattr(a, name, t.data_ptr())
-        setattr(a, f"{name}_batch_stride", bs)
-        setattr(a, f"{name}_row_stride", rs)
-    h0 = _dense("h0", h0, (Bsz, Dm), torch.float32)
-    lengths = _dense("lengths", lengths, (Bsz,), torch.int32)
+    dev, shape = _cuda("x", x), x.shape
+    xb, xr = _view3(x)
+    dt = _float("x", x)
+    _like("g", g, shape, x.dtype, dev)
+    gb, gr = _view3(g)
+    Bsz, Lq, Dm = shape
+    if out is None:
+        h = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        h = out
+        _like("out", h, shape, x.dtype, dev)
+    hb, hr = _view3(h)
+    h0 = _dense("h0", h0, (Bsz, Dm), torch.float32, dev)
+    lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
     last = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev) if return_state else None
     if states is not None:
-        steps = L.GATED_SCAN_STATE_STEPS
-        _dense_out("states", states, (Bsz, (Lq + steps - 1) // steps, Dm), torch.float32)
-    for name, t in (("h0", h0), ("h_last", last), ("states", states), ("lengths", lengths)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    ws = _gated_scan_workspace(a, dev)  # noqa: F841
-    _run_on(dev, L.lib().hx_gated_scan_fwd, C.byref(a))
+        _dense_out("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
+    ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
+    a = L.GatedScanArgs(Bsz, Lq, Dm, dt, _gate(gate), 0, x.data_ptr(), g.data_ptr(), h.data_ptr(), xb, xr, gb, gr, hb, hr, _at(h0),
+                        _at(last), _at(states), _at(lengths), _at(ws), 0 if ws is None else ws.numel())
+    _call(dev, L.lib().hx_gated_scan_fwd, C.byref(a))
     return (h, last) if return_state else h
 
 
@@ -271,50 +286,57 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     """Gradients of gated_scan (hx_gated_scan_bwd): (dx, dg, dh0) for dh = dL/dh [B, L, D] and dh_last = dL/dh_last [B, D]
     fp32 (None: zero).  x, g and lengths as given to gated_scan, states as it filled them; out: (dx, dg) to write into (halves
     of one buffer, say)."""
-    dx, dg = out if out is not None else (None, None)
-    dev = _on_device(dh=dh, x=x, g=g, states=states, lengths=lengths, dh_last=dh_last, dx=dx, dg=dg)
-    _view3(x)
-    Bsz, Lq, Dm = x.shape
-    a = L.GatedScanBwdArgs()
-    a.batch, a.seq_len, a.d_inner, a.io_dtype, a.gate = Bsz, Lq, Dm, _dt(x), _gate(gate)
+    dev, shape = _cuda("x", x), x.shape
+    xb, xr = _view3(x)
+    dt = _float("x", x)
+    _like("g", g, shape, x.dtype, dev)
+    _like("dh", dh, shape, x.dtype, dev)
+    gb, gr = _view3(g)
+    db, dr = _view3(dh)
+    Bsz, Lq, Dm = shape
     if out is None:
-        dx, dg = (torch.empty((Bsz, Lq, Dm), dtype=x.dtype, device=dev) for _ in range(2))
-    for name, t in (("x", x), ("g", g), ("dh", dh), ("dx", dx), ("dg", dg)):
-        _like(name, t, (Bsz, Lq, Dm), x.dtype)
-        bs, rs = _view3(t)
-        setattr(a, name, t.data_ptr())
-        setattr(a, f"{name}_batch_stride", bs)
-        setattr(a, f"{name}_row_stride", rs)
-    steps = L.GATED_SCAN_STATE_STEPS
-    states = _dense("states", states, (Bsz, (Lq + steps - 1) // steps, Dm), torch.float32)
-    dh_last = _dense("dh_last", dh_last, (Bsz, Dm), torch.float32)
-    lengths = _dense("lengths", lengths, (Bsz,), torch.int32)
+        dx, dg = torch.empty(shape, dtype=x.dtype, device=dev), torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        dx, dg = out
+        _like("dx", dx, shape, x.dtype, dev)
+        _like("dg", dg, shape, x.dtype, dev)
+    dxb, dxr = _view3(dx)
+    dgb, dgr = _view3(dg)
+    states = _dense("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
+    dh_last = _dense("dh_last", dh_last, (Bsz, Dm), torch.float32, dev)
+    lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
     dh0 = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev)
-    for name, t in (("states", states), ("dh_last", dh_last), ("dh0", dh0), ("lengths", lengths)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    ws = _gated_scan_workspace(a, dev)  # noqa: F841
-    _run_on(dev, L.lib().hx_gated_scan_bwd, C.byref(a))
+    ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
+    a = L.GatedScanBwdArgs(Bsz, Lq, Dm, dt, _gate(gate), 0, x.data_ptr(), g.data_ptr(), dh.data_ptr(), dx.data_ptr(), dg.data_ptr(), xb,
+                           xr, gb, gr, db, dr, dxb, dxr, dgb, dgr, _at(states), _at(dh_last), _at(dh0), _at(lengths), _at(ws),
+                           0 if ws is None else ws.numel())
+    _call(dev, L.lib().hx_gated_scan_bwd, C.byref(a))
     return dx, dg, dh0
 
 
 def gated_scan_step(x, g, h, gate="sigmoid", h_out=None, out=None):
     """One token of the gated recurrence for every sequence (hx_gated_scan_step): x, g [B, D] (row strides arbitrary),
     h [B, D] fp32.  Returns y [B, D]; the new state goes to h_out, or replaces h."""
-    h_out = h if h_out is None else h_out
-    dev = _on_device(x=x, g=g, h=h, h_out=h_out, out=out)
-    if x.dim() != 2:
-        raise L.HxError(1, f"expected a [B, D] tensor, got {tuple(x.shape)}")
-    Bsz, Dm = x.shape
-    y = out if out is not None else torch.empty((Bsz, Dm), dtype=x.dtype, device=dev)
-    for name, t in (("x", x), ("g", g), ("y", y)):
-        _like(name, t, (Bsz, Dm), x.dtype)
-        if t.stride(1) != 1:
-            raise L.HxError(1, f"{name} needs a unit inner stride, has {t.stride()}")
-    for name, t in (("h", h), ("h_out", h_out)):
-        _dense_out(name, t, (Bsz, Dm), torch.float32)
-    _run_on(dev, L.lib().hx_gated_scan_step, _p(x), x.stride(0), _p(g), g.stride(0), _p(h), _p(h_out), _p(y), y.stride(0), Bsz, Dm,
-            _gate(gate), _dt(x))
+    dev, shape = _cuda("x", x), x.shape
+    if len(shape) != 2:
+        raise L.HxError(1, f"expected a [B, D] tensor, got {tuple(shape)}")
+    dt, code = _float("x", x), _gate(gate)
+    _like("g", g, shape, x.dtype, dev)
+    _dense_out("h", h, shape, torch.float32, dev)
+    if h_out is None:
+        h_out = h
+    else:
+        _dense_out("h_out", h_out, shape, torch.float32, dev)
+    if out is None:
+        y = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        y = out
+        _like("out", y, shape, x.dtype, dev)
+    (xr, xi), (gr, gi), (yr, yi) = x.stride(), g.stride(), y.stride()
+    if xi != 1 or gi != 1 or yi != 1:
+        raise L.HxError(1, f"x, g and out need a unit inner stride, have {x.stride()}, {g.stride()}, {y.stride()}")
+    _call(dev, L.lib().hx_gated_scan_step, x.data_ptr(), xr, g.data_ptr(), gr, h.data_ptr(), h_out.data_ptr(), y.data_ptr(), yr, shape[0],
+          shape[1], code, dt)
     return y
 
 
@@ -421,19 +443,16 @@ class W4Matrix:
     def __init__(self, rows, cols, group, scale, zero):
         if group not in (32, 64, 128) or cols % group:
             raise L.HxError(1, f"{cols} columns in groups of {group}: groups are 32, 64 or 128 and divide the columns")
-        dev = _on_device(scale=scale, zero=zero)
-        if scale.dtype not in (torch.float32, torch.bfloat16):
-            raise L.HxError(4, f"scale has dtype {scale.dtype}, expected float32 or bfloat16")
+        dev = _cuda("scale", scale)
+        _float("scale", scale)
         self.rows, self.cols, self.group = rows, cols, group
-        self.scale = _dense("scale", scale, (rows, cols // group), scale.dtype)
-        self.zero = _dense("zero", zero, (rows, cols // group), torch.uint8)
+        self.scale = _dense("scale", scale, (rows, cols // group), scale.dtype, dev)
+        self.zero = _dense("zero", zero, (rows, cols // group), torch.uint8, dev)
         self.codes = torch.empty((rows, L.lib().hx_w4_row_bytes(cols)), dtype=torch.uint8, device=dev)
 
     def _args(self):
-        m = L.W4MatrixArgs()
-        m.rows, m.cols, m.group, m.scale_dtype = self.rows, self.cols, self.group, _dt(self.scale)
-        m.codes, m.scale, m.zero = self.codes.data_ptr(), self.scale.data_ptr(), None if self.zero is None else self.zero.data_ptr()
-        return m
+        return L.W4MatrixArgs(self.rows, self.cols, self.group, _FLOATS[self.scale.dtype], self.codes.data_ptr(), self.scale.data_ptr(),
+                              _at(self.zero))
 
 
 def _rows2(name, t):
@@ -446,8 +465,8 @@ def _rows2(name, t):
 def w4_quantize(w, group=64, zero_points=False, scale_dtype=torch.float32) -> W4Matrix:
     """Weights w [N, K] (fp32 or bf16) in 4 bits (hx_w4_quantize): symmetric about zero, or with a zero point per group."""
     ldw = _rows2("w", w)
-    dev = _on_device(w=w)
-    if scale_dtype not in (torch.float32, torch.bfloat16):
+    dev, dt = _cuda("w", w), _float("w", w)
+    if scale_dtype not in _FLOATS:
         raise L.HxError(4, f"scale dtype {scale_dtype}: float32 or bfloat16")
     N, K = w.shape
     if group not in (32, 64, 128) or K % group:
@@ -455,7 +474,7 @@ def w4_quantize(w, group=64, zero_points=False, scale_dtype=torch.float32) -> W4
     scale = torch.empty((N, K // group), dtype=scale_dtype, device=dev)
     zero = torch.empty((N, K // group), dtype=torch.uint8, device=dev) if zero_points else None
     m = W4Matrix(N, K, group, scale, zero)
-    _run_on(dev, L.lib().hx_w4_quantize, _p(w), ldw, _dt(w), C.byref(m._args()))
+    _call(dev, L.lib().hx_w4_quantize, w.data_ptr(), ldw, dt, C.byref(m._args()))
     return m
 
 
@@ -463,40 +482,49 @@ def w4_pack(codes, scale, zero=None) -> W4Matrix:
     """A matrix whose codes exist already (hx_w4_pack): codes [N, K] u8 in 0..15, scale [N, K / group], zero like scale or
     None; the group follows from the shapes."""
     ldc = _rows2("codes", codes)
-    dev = _on_device(codes=codes, scale=scale, zero=zero)
+    dev = _cuda("codes", codes)
     if codes.dtype != torch.uint8:
         raise L.HxError(4, f"codes have dtype {codes.dtype}, expected uint8")
     N, K = codes.shape
     groups = scale.shape[1] if scale.dim() == 2 else 0
     if groups < 1 or K % groups:
         raise L.HxError(1, f"scale {tuple(scale.shape)} does not divide codes {tuple(codes.shape)} into groups")
+    if scale.get_device() != dev:
+        raise L.HxError(3, f"scale is on {scale.device}, codes on {codes.device}")
     m = W4Matrix(N, K, K // groups, scale, zero)
-    _run_on(dev, L.lib().hx_w4_pack, _p(codes), ldc, C.byref(m._args()))
+    _call(dev, L.lib().hx_w4_pack, codes.data_ptr(), ldc, C.byref(m._args()))
     return m
 
 
 def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
     """The values a W4Matrix stands for, [N, K] fp32 or bf16 (hx_w4_dequantize)."""
-    dev = m.codes.device
-    w = out if out is not None else torch.empty((m.rows, m.cols), dtype=dtype, device=dev)
-    _on_device(codes=m.codes, out=w)
-    _like("out", w, (m.rows, m.cols), dtype)
-    _run_on(dev, L.lib().hx_w4_dequantize, C.byref(m._args()), _p(w), _rows2("out", w), _dt(w))
+    dev = m.codes.get_device()
+    w = torch.empty((m.rows, m.cols), dtype=dtype, device=dev) if out is None else out
+    dt = _float("out", w)
+    _like("out", w, (m.rows, m.cols), dtype, dev)
+    _call(dev, L.lib().hx_w4_dequantize, C.byref(m._args()), w.data_ptr(), _rows2("out", w), dt)
     return w
 
 
 def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=None):
     """C = a @ W.T (+ bias) (+ activation) with W in 4 bits (hx_gemm_w4), for the few rows of a decode step.
     a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's)."""
-    dev = _on_device(a=a, codes=m.codes, bias=bias, out=out)
-    lda = _rows2("a", a)
+    dev, lda = _cuda("a", a), _rows2("a", a)
+    adt = _float("a", a)
     M, K = a.shape
     if K != m.cols:
         raise L.HxError(1, f"a is {tuple(a.shape)} but W is {(m.rows, m.cols)}")
-    bias = _dense("bias", bias, (m.rows,), torch.float32)
-    c = out if out is not None else torch.empty((M, m.rows), dtype=out_dtype or a.dtype, device=dev)
-    _like("out", c, (M, m.rows), out_dtype or c.dtype)
-    _run_on(dev, L.lib().hx_gemm_w4, _p(a), lda, _dt(a), C.byref(m._args()), _p(bias), _p(c), _rows2("out", c), _dt(c), M, epilogue)
+    if m.codes.get_device() != dev:
+        raise L.HxError(3, f"a is on {a.device}, W on {m.codes.device}")
+    bias = _dense("bias", bias, (m.rows,), torch.float32, dev)
+    if out is None:
+        c = torch.empty((M, m.rows), dtype=out_dtype or a.dtype, device=dev)
+        ldc = m.rows
+    else:
+        c = out
+        _like("out", c, (M, m.rows), out_dtype or c.dtype, dev)
+        ldc = _rows2("out", c)
+    _call(dev, L.lib().hx_gemm_w4, a.data_ptr(), lda, adt, C.byref(m._args()), _at(bias), c.data_ptr(), ldc, _float("out", c), M, epilogue)
     return c
 
 
