@@ -1,0 +1,365 @@
+// The product of a few rows with a 4-bit matrix.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "w4.cuh"
+
+namespace hx {
+namespace w4 {
+
+// ---------------------------------------------------------------- C = A W^T for a few rows
+// A stream over the codes: HBM gives an SM about 23 bytes = 46 codes a cycle, each of which has to become a tensor-core operand, so
+// instructions per code are what the kernel is made of.  W is the left operand (16 outputs x 16 columns), the rows of A the right one
+// (8 rows a tile).  Which column a k index of the MMA stands for does not matter as long as both operands agree; the layout of the
+// codes is such that lane (g, c) = (lane / 4, lane mod 4) finds in its 16 bytes of row g four words, word j holding the columns
+// 32 j + 8 c .. + 7 of the block, as the four k-pairs of two MMAs.  So the MMAs of word j cover columns 32 j .. 32 j + 31 whatever
+// the group size, one LDG.128 brings a lane's share of 128 columns, and the matching piece of A is 16 consecutive bytes.
+// A pair of codes becomes two bf16 numbers with (w >> 4 p & 0x000f000f) | 0x43004300, which is 128 + code exactly, minus 128 + zero,
+// also exact.  Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut
+// into three bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
+// A CTA works through tiles of 16 RT outputs, its 16 warps on different blocks of 128 columns, the codes of the next kAhead blocks
+// (of the next tiles too) under way; a tile's partial sums are added in the order of the warps.  Where the tiles are fewer than the
+// SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of their shared memory.
+constexpr int kAhead = 4;
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_codes(const uint8_t *p) {   // read once
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+// codes 2 p and 2 p + 1 of a word, less the zero point: two bf16.  mask and magic are 0x000f000f and 0x43004300 in registers: one
+// logic instruction takes (shifted & mask) | magic.
+__device__ __forceinline__ uint32_t two_weights(uint32_t word, int p, uint32_t mask, uint32_t magic, uint32_t zero) {
+    uint32_t u;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(u) : "r"(word >> (4 * p)), "r"(mask), "r"(magic));
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), *reinterpret_cast<const __nv_bfloat162 *>(&zero));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Eight consecutive elements of a row of A as MMA operands: one part (bf16) or three that add up to them (fp32).
+template <typename TA> struct Operand;
+template <> struct Operand<__nv_bfloat16> {
+    static constexpr int kParts = 1;
+    uint32_t r[1][4];
+    template <bool VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+        if constexpr (VEC) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            r[0][0] = v.x, r[0][1] = v.y, r[0][2] = v.z, r[0][3] = v.w;
+        } else {
+            const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[0][i] = (uint32_t)u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+        }
+    }
+};
+template <> struct Operand<float> {
+    static constexpr int kParts = 3;
+    uint32_t r[3][4];
+    // v = high 8 bits + rest; the rest is exact, and zero for an infinity
+    static __device__ __forceinline__ float take(float &v) {
+        const float high = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+        v = v == high ? 0.f : v - high;
+        return high;
+    }
+    template <bool VEC> __device__ __forceinline__ void load(const float *p) {
+        float v[8];
+        load8(p, VEC, v);
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a = __float_as_uint(take(v[2 * i])), b = __float_as_uint(take(v[2 * i + 1]));
+                r[part][i] = __byte_perm(a, b, 0x7632);
+            }
+    }
+};
+
+__device__ __forceinline__ void finish(float v, int n, int row, const float *bias, void *C, int64_t ldc, int c_dtype, int epilogue) {
+    if (bias) v += bias[n];
+    if (epilogue == gemm::kEpiSilu) v = silu_acc(v);
+    else if (epilogue == gemm::kEpiSoftplus) v = softplus_acc(v);
+    if (c_dtype == HX_BF16) static_cast<__nv_bfloat16 *>(C)[row * ldc + n] = __float2bfloat16_rn(v);
+    else static_cast<float *>(C)[row * ldc + n] = v;
+}
+
+// NT tiles of 8 rows of A, RT of 16 outputs, WARPS of a CTA.  XB > 0: a warp has XB blocks of every tile, whose pieces of A stay in
+// its registers; 0: they are read again for each tile.
+template <typename TA, int NT, int RT, int GROUP, int WARPS, int XB, bool VEC>
+__global__ void __launch_bounds__(32 * WARPS, 1)
+gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
+               int64_t ldc, int c_dtype, int M, int blocks, int epilogue) {
+    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = RT * NT * 128;
+    static_assert(XB == 0 || kAhead % (XB > 0 ? XB : 1) == 0, "the blocks of a tile meet the same registers every time");
+    constexpr int kBuffers = 2 * WARPS * kSums * sizeof(float) <= 48 * 1024 ? 2 : 1;
+    __shared__ __align__(16) float partial[kBuffers][WARPS][kSums];
+    const auto cluster = cooperative_groups::this_cluster();
+    const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();   // CTAs of a tile
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int m0 = blockIdx.y * 8 * NT;
+    const int64_t row_bytes = (int64_t)blocks * kBlockBytes;
+    const int groups = m.cols / GROUP, tiles = (m.rows + 16 * RT - 1) / (16 * RT), stride = gridDim.x / share;
+    const int first = rank * WARPS + warp, apart = share * WARPS;   // blocks of this warp: first, first + apart, ...
+    const int rounds = (blocks + apart - 1) / apart;                // of a tile, the last one not for all warps
+
+    uint32_t mask, magic;   // opaque to the compiler, which would otherwise fold them into two instructions
+    asm volatile("mov.u32 %0, 0x000f000f; mov.u32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
+    const TA *rows[NT];     // this lane's rows of A; past the last one the last, whose sums are then not stored
+#pragma unroll
+    for (int t = 0; t < NT; ++t) rows[t] = A + (int64_t)min(m0 + t * 8 + g, M - 1) * lda + 8 * c;
+    // the fetched side: tile, round, and where its rows of codes and scales are
+    int ahead_tile = blockIdx.x / share, ahead_round = 0;
+    const uint8_t *codes[RT][2];
+    int64_t at[RT][2];
+    auto rows_of = [&](int tile) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int n = min(tile * 16 * RT + r * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
+                codes[r][half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
+                at[r][half] = (int64_t)n * groups + first * kGroups;
+            }
+    };
+    // what is under way stays as it is loaded: any arithmetic on it here would wait for it
+    uint4 w[kAhead][RT][2];
+    uint32_t s[kAhead][RT][2][kGroups];   // scales, to be shifted by scale_shift
+    uint32_t z[kAhead][RT][2];            // zero points, a byte a group
+    const bool scale_bf16 = m.scale_dtype == HX_BF16;
+    const int scale_shift = scale_bf16 ? 16 : 0;
+    // the zero points of a block are one aligned load where the rows are whole blocks
+    const bool zero_word = GROUP == kBlockCols || (m.cols % kBlockCols == 0 && ((uintptr_t)m.zero & (kGroups - 1)) == 0);
+    auto fetch = [&](int u) {
+        if (ahead_tile >= tiles) return;
+        const int block = first + ahead_round * apart;
+        if (block < blocks) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    w[u][r][half] = load_codes(codes[r][half]);
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q) {
+                        const bool in = GROUP == kBlockCols || block * kGroups + q < groups;
+                        s[u][r][half][q] = 0;
+                        if (in && scale_bf16) s[u][r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
+                        else if (in) s[u][r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
+                    }
+                    if (!m.zero) {
+                        z[u][r][half] = 0x08080808u;
+                    } else if (zero_word) {
+                        const uint8_t *p = m.zero + at[r][half];
+                        if constexpr (kGroups == 4) z[u][r][half] = *reinterpret_cast<const uint32_t *>(p);
+                        else if constexpr (kGroups == 2) z[u][r][half] = *reinterpret_cast<const uint16_t *>(p);
+                        else z[u][r][half] = *p;
+                    } else {
+                        z[u][r][half] = 0;
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q)
+                            if (block * kGroups + q < groups) z[u][r][half] |= (uint32_t)m.zero[at[r][half] + q] << (8 * q);
+                    }
+                }
+        }
+        if (++ahead_round == rounds) {
+            ahead_round = 0;
+            ahead_tile += stride;
+            rows_of(ahead_tile);
+        } else {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    codes[r][half] += (int64_t)apart * kBlockBytes;
+                    at[r][half] += apart * kGroups;
+                }
+        }
+    };
+    rows_of(ahead_tile);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) fetch(u);
+
+    Operand<TA> kept[XB > 0 ? XB : 1][NT][4];
+    if constexpr (XB > 0) {
+#pragma unroll
+        for (int x = 0; x < XB; ++x)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = (first + x * apart) * kBlockCols + j * 32;
+                    if (k < m.cols) kept[x][t][j].template load<VEC>(rows[t] + k);
+                }
+    }
+    float total[RT][NT][4];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
+
+    int round = 0, buffer = 0;
+    for (int tile = blockIdx.x / share; tile < tiles;) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (tile >= tiles) break;
+            const int block = first + round * apart;
+            if (block < blocks) {
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    float sum[RT][NT][4] = {};
+                    uint32_t zero[RT][2];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) zero[r][half] = __byte_perm(z[u][r][half], 0x43u, 0x4040u + 0x0101u * q);   // 128 + zero, twice
+#pragma unroll
+                    for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
+                        if (GROUP < kBlockCols && block * kBlockCols + j * 32 >= m.cols) break;   // the filled-up end of a row
+                        uint32_t a[RT][2][4];
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const uint4 v = w[u][r][half];
+                                const uint32_t word = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+#pragma unroll
+                                for (int p = 0; p < 4; ++p) a[r][half][p] = two_weights(word, p, mask, magic, zero[r][half]);
+                            }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            Operand<TA> b;
+                            if constexpr (XB > 0) b = kept[u % (XB > 0 ? XB : 1)][t][j];
+                            else b.template load<VEC>(rows[t] + block * kBlockCols + j * 32);
+#pragma unroll
+                            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                                for (int r = 0; r < RT; ++r) {
+                                    mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
+                                    mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
+                                }
+                        }
+                    }
+                    // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(__uint_as_float(s[u][r][i >> 1][q] << scale_shift), sum[r][t][i], total[r][t][i]);
+                }
+            }
+            fetch(u);
+            if (++round < rounds) continue;
+            round = 0;
+            // the tile's sums: every warp's into this round's buffer, then added in the order of the warps
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    *reinterpret_cast<float4 *>(&partial[buffer][warp][((r * NT + t) * 32 + lane) * 4]) =
+                        make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
+                }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+            for (int i = threadIdx.x; i < kSums; i += 32 * WARPS) {
+                const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
+                const int n = tile * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
+                if (n >= m.rows || row >= M) continue;
+                float v = 0.f;
+#pragma unroll
+                for (int q = 0; q < WARPS; ++q) v += partial[buffer][q][i];
+                if (share > 1) {
+                    partial[buffer][0][i] = v;   // for the cluster's first CTA
+                    continue;
+                }
+                finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
+            }
+            tile += stride;
+            if constexpr (kBuffers == 2) buffer ^= 1;
+            else asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+        }
+    }
+    if (share > 1) {   // one tile a cluster (its sums are in buffer 0)
+        cluster.sync();
+        if (rank == 0)
+            for (int i = threadIdx.x; i < kSums; i += 32 * WARPS) {
+                const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
+                const int n = blockIdx.x / share * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
+                if (n >= m.rows || row >= M) continue;
+                float v = 0.f;
+                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(&partial[0][0][i], q);
+                finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
+            }
+        cluster.sync();   // the others' shared memory stays until it has been read
+    }
+}
+
+// CTAs that share a tile of `outs` outputs: where SMs are left over and a warp would have more than one block.
+static int share_of(const hx_w4_matrix &m, int outs, int warps) {
+    const int64_t tiles = ((int64_t)m.rows + outs - 1) / outs;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sm_count() / tiles, (blocks_of(m.cols) + warps - 1) / warps), 8));
+}
+
+template <typename TA, int NT, int RT, int GROUP, int WARPS, int XB, bool VEC>
+static hx_status launch_gemm_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                                int epilogue, cudaStream_t st) {
+    const int blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + 16 * RT - 1) / (16 * RT));
+    const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
+    HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
+    const int sms = sm_count(), share = share_of(m, 16 * RT, WARPS);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min(tiles, sms) * share), (unsigned)down);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)share;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = share > 1 ? 1 : 0;
+    HX_CUDA(cudaLaunchKernelEx(&cfg, gemm_w4_kernel<TA, NT, RT, GROUP, WARPS, XB, VEC>, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M,
+                               blocks, epilogue));
+    return check_launch("gemm_w4_kernel");
+}
+template <typename TA, int NT, int RT, int WARPS>
+static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                             int epilogue, cudaStream_t st) {
+    const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
+    const int blocks = blocks_of(m.cols), share = share_of(m, 16 * RT, WARPS), kept = (blocks + share * WARPS - 1) / (share * WARPS);
+#define HX_W4_AS(G, XB, VEC) return launch_gemm_as<TA, NT, RT, G, WARPS, XB, VEC>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st)
+#define HX_W4_GROUP(G)                                                             \
+    do {                                                                           \
+        if constexpr (NT == 1 && sizeof(TA) == 2) {                                \
+            if (vec && kept == 1) HX_W4_AS(G, 1, true);                            \
+            if (vec && kept == 2) HX_W4_AS(G, 2, true);                            \
+        }                                                                          \
+        if (vec) HX_W4_AS(G, 0, true);                                             \
+        HX_W4_AS(G, 0, false);                                                     \
+    } while (0)
+    if (m.group == 32) HX_W4_GROUP(32);
+    if (m.group == 64) HX_W4_GROUP(64);
+    HX_W4_GROUP(128);
+#undef HX_W4_GROUP
+#undef HX_W4_AS
+}
+
+template <typename TA>
+static hx_status gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
+                      cudaStream_t st) {
+    if (M <= 8) return launch_gemm<TA, 1, 1, 16>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 16) return launch_gemm<TA, 2, 1, 16>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 32) return launch_gemm<TA, 4, 1, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_gemm<TA, 8, 1, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+}
+
+}  // namespace w4
+}  // namespace hx
