@@ -20,15 +20,21 @@ namespace w4 {
 // A pair of codes becomes two bf16 numbers with (w >> 4 p & 0x000f000f) | 0x43004300, which is 128 + code exactly, minus 128 + zero,
 // also exact.  Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut
 // into three bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
-// A CTA works through tiles of 16 RT outputs, its 16 warps on different blocks of 128 columns, the codes of the next kAhead blocks
-// (of the next tiles too) under way; a tile's partial sums are added in the order of the warps.  Where the tiles are fewer than the
-// SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of their shared memory.
-constexpr int kAhead = 4;
+// A CTA works through tiles of 16 RT outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
+// block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  The four lanes of a row
+// need the same scales, so lane c loads those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are
+// added in the order of the warps.  Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first
+// one adds the others' sums out of their shared memory.
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint4 load_codes(const uint8_t *p) {   // read once
     uint4 v;
@@ -43,6 +49,8 @@ __device__ __forceinline__ uint32_t two_weights(uint32_t word, int p, uint32_t m
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), *reinterpret_cast<const __nv_bfloat162 *>(&zero));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
+
+constexpr int max_warps(int NT) { return NT == 1 ? 16 : 8; }   // of a CTA, by its registers
 
 // Eight consecutive elements of a row of A as MMA operands: one part (bf16) or three that add up to them (fp32).
 template <typename TA> struct Operand;
@@ -90,32 +98,33 @@ __device__ __forceinline__ void finish(float v, int n, int row, const float *bia
     else static_cast<float *>(C)[row * ldc + n] = v;
 }
 
-// NT tiles of 8 rows of A, RT of 16 outputs, WARPS of a CTA.  XB > 0: a warp has XB blocks of every tile, whose pieces of A stay in
-// its registers; 0: they are read again for each tile.
-template <typename TA, int NT, int RT, int GROUP, int WARPS, int XB, bool VEC>
-__global__ void __launch_bounds__(32 * WARPS, 1)
+// NT tiles of 8 rows of A, RT of 16 outputs, CH blocks of a chunk.
+template <typename TA, int NT, int RT, int GROUP, int CH, bool VEC>
+__global__ void __launch_bounds__(32 * max_warps(NT), 1)
 gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
                int64_t ldc, int c_dtype, int M, int blocks, int epilogue) {
     constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = RT * NT * 128;
-    static_assert(XB == 0 || kAhead % (XB > 0 ? XB : 1) == 0, "the blocks of a tile meet the same registers every time");
-    constexpr int kBuffers = 2 * WARPS * kSums * sizeof(float) <= 48 * 1024 ? 2 : 1;
-    __shared__ __align__(16) float partial[kBuffers][WARPS][kSums];
+    extern __shared__ __align__(16) float partial[];   // [2][warps][kSums]
     const auto cluster = cooperative_groups::this_cluster();
     const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();   // CTAs of a tile
+    const int warps = blockDim.x / 32, threads = blockDim.x;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int m0 = blockIdx.y * 8 * NT;
     const int64_t row_bytes = (int64_t)blocks * kBlockBytes;
     const int groups = m.cols / GROUP, tiles = (m.rows + 16 * RT - 1) / (16 * RT), stride = gridDim.x / share;
-    const int first = rank * WARPS + warp, apart = share * WARPS;   // blocks of this warp: first, first + apart, ...
-    const int rounds = (blocks + apart - 1) / apart;                // of a tile, the last one not for all warps
+    const int first = (rank * warps + warp) * CH, apart = share * warps * CH;   // first block of this warp's chunks
+    const int chunks = (blocks + apart - 1) / apart;                            // of a tile, the last one not for all warps
+    const bool scale_bf16 = m.scale_dtype == HX_BF16;
+    const int scale_shift = scale_bf16 ? 16 : 0;
 
     uint32_t mask, magic;   // opaque to the compiler, which would otherwise fold them into two instructions
     asm volatile("mov.u32 %0, 0x000f000f; mov.u32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
     const TA *rows[NT];     // this lane's rows of A; past the last one the last, whose sums are then not stored
 #pragma unroll
     for (int t = 0; t < NT; ++t) rows[t] = A + (int64_t)min(m0 + t * 8 + g, M - 1) * lda + 8 * c;
-    // the fetched side: tile, round, and where its rows of codes and scales are
-    int ahead_tile = blockIdx.x / share, ahead_round = 0;
+
+    // the chunk that is asked for: its tile, its number there, where its rows of codes and scales are
+    int ahead_tile = blockIdx.x / share, ahead = 0;
     const uint8_t *codes[RT][2];
     int64_t at[RT][2];
     auto rows_of = [&](int tile) {
@@ -125,50 +134,40 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
             for (int half = 0; half < 2; ++half) {
                 const int n = min(tile * 16 * RT + r * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
                 codes[r][half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
-                at[r][half] = (int64_t)n * groups + first * kGroups;
+                at[r][half] = (int64_t)n * groups + (first + c) * kGroups;
             }
     };
-    // what is under way stays as it is loaded: any arithmetic on it here would wait for it
-    uint4 w[kAhead][RT][2];
-    uint32_t s[kAhead][RT][2][kGroups];   // scales, to be shifted by scale_shift
-    uint32_t z[kAhead][RT][2];            // zero points, a byte a group
-    const bool scale_bf16 = m.scale_dtype == HX_BF16;
-    const int scale_shift = scale_bf16 ? 16 : 0;
-    // the zero points of a block are one aligned load where the rows are whole blocks
-    const bool zero_word = GROUP == kBlockCols || (m.cols % kBlockCols == 0 && ((uintptr_t)m.zero & (kGroups - 1)) == 0);
-    auto fetch = [&](int u) {
-        if (ahead_tile >= tiles) return;
-        const int block = first + ahead_round * apart;
-        if (block < blocks) {
+    // What is under way stays as it is loaded: any arithmetic on it would wait for it.
+    uint4 w[CH][RT][2];
+    uint32_t scale[2][RT][2][kGroups], zero[2][RT][2][kGroups];   // of block c of this chunk and of the next
+    auto fetch_codes = [&](int u) {
+        if (ahead_tile < tiles && first + ahead * apart + u < blocks)
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    w[u][r][half] = load_codes(codes[r][half]);
+                for (int half = 0; half < 2; ++half) w[u][r][half] = load_codes(codes[r][half] + u * kBlockBytes);
+    };
+    auto fetch_scales = [&](uint32_t (&s)[RT][2][kGroups], uint32_t (&z)[RT][2][kGroups]) {
+        const int block = first + ahead * apart + c;
 #pragma unroll
-                    for (int q = 0; q < kGroups; ++q) {
-                        const bool in = GROUP == kBlockCols || block * kGroups + q < groups;
-                        s[u][r][half][q] = 0;
-                        if (in && scale_bf16) s[u][r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
-                        else if (in) s[u][r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
-                    }
-                    if (!m.zero) {
-                        z[u][r][half] = 0x08080808u;
-                    } else if (zero_word) {
-                        const uint8_t *p = m.zero + at[r][half];
-                        if constexpr (kGroups == 4) z[u][r][half] = *reinterpret_cast<const uint32_t *>(p);
-                        else if constexpr (kGroups == 2) z[u][r][half] = *reinterpret_cast<const uint16_t *>(p);
-                        else z[u][r][half] = *p;
-                    } else {
-                        z[u][r][half] = 0;
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-                        for (int q = 0; q < kGroups; ++q)
-                            if (block * kGroups + q < groups) z[u][r][half] |= (uint32_t)m.zero[at[r][half] + q] << (8 * q);
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    const bool in = ahead_tile < tiles && c < CH && block * kGroups + q < groups;
+                    s[r][half][q] = 0;
+                    z[r][half][q] = 8;
+                    if (in) {
+                        if (scale_bf16) s[r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
+                        else s[r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
+                        if (m.zero) z[r][half][q] = m.zero[at[r][half] + q];
                     }
                 }
-        }
-        if (++ahead_round == rounds) {
-            ahead_round = 0;
+    };
+    auto advance = [&]() {
+        if (++ahead == chunks) {
+            ahead = 0;
             ahead_tile += stride;
             rows_of(ahead_tile);
         } else {
@@ -177,173 +176,176 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     codes[r][half] += (int64_t)apart * kBlockBytes;
-                    at[r][half] += apart * kGroups;
+                    at[r][half] += (int64_t)apart * kGroups;
                 }
         }
     };
     rows_of(ahead_tile);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) fetch(u);
+    for (int u = 0; u < CH; ++u) fetch_codes(u);
+    fetch_scales(scale[0], zero[0]);
+    advance();
 
-    Operand<TA> kept[XB > 0 ? XB : 1][NT][4];
-    if constexpr (XB > 0) {
+    float total[RT][NT][4] = {};
+    int buffer = 0;
+    for (int tile = blockIdx.x / share; tile < tiles; tile += stride) {
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            fetch_scales(scale[1], zero[1]);
 #pragma unroll
-        for (int x = 0; x < XB; ++x)
+            for (int u = 0; u < CH; ++u) {
+                const int block = first + chunk * apart + u;
+                if (block < blocks) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k = (first + x * apart) * kBlockCols + j * 32;
-                    if (k < m.cols) kept[x][t][j].template load<VEC>(rows[t] + k);
-                }
-    }
-    float total[RT][NT][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
-
-    int round = 0, buffer = 0;
-    for (int tile = blockIdx.x / share; tile < tiles;) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (tile >= tiles) break;
-            const int block = first + round * apart;
-            if (block < blocks) {
-#pragma unroll
-                for (int q = 0; q < kGroups; ++q) {
-                    float sum[RT][NT][4] = {};
-                    uint32_t zero[RT][2];
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) zero[r][half] = __byte_perm(z[u][r][half], 0x43u, 0x4040u + 0x0101u * q);   // 128 + zero, twice
-#pragma unroll
-                    for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
-                        if (GROUP < kBlockCols && block * kBlockCols + j * 32 >= m.cols) break;   // the filled-up end of a row
-                        uint32_t a[RT][2][4];
+                    for (int q = 0; q < kGroups; ++q) {
+                        if (GROUP < kBlockCols && block * kGroups + q >= groups) break;   // the filled-up end of a row
+                        float sum[RT][NT][4], by[RT][2];
+                        uint32_t offset[RT][2];   // 128 + zero point, twice
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
-                                const uint4 v = w[u][r][half];
-                                const uint32_t word = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
-#pragma unroll
-                                for (int p = 0; p < 4; ++p) a[r][half][p] = two_weights(word, p, mask, magic, zero[r][half]);
+                                by[r][half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][r][half][q], u, 4) << scale_shift);
+                                offset[r][half] = 0x43084308u;
+                                if (m.zero) offset[r][half] = __byte_perm(__shfl_sync(0xffffffffu, zero[0][r][half][q], u, 4), 0x43u, 0x4040u);
                             }
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            Operand<TA> b;
-                            if constexpr (XB > 0) b = kept[u % (XB > 0 ? XB : 1)][t][j];
-                            else b.template load<VEC>(rows[t] + block * kBlockCols + j * 32);
+                        for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
+                            uint32_t a[RT][2][4];
 #pragma unroll
-                            for (int part = 0; part < kParts; ++part)
+                            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                                for (int r = 0; r < RT; ++r) {
-                                    mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
-                                    mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
+                                for (int half = 0; half < 2; ++half) {
+                                    const uint4 v = w[u][r][half];
+                                    const uint32_t word = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+#pragma unroll
+                                    for (int p = 0; p < 4; ++p) a[r][half][p] = two_weights(word, p, mask, magic, offset[r][half]);
                                 }
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                Operand<TA> b;
+                                b.template load<VEC>(rows[t] + block * kBlockCols + j * 32);
+#pragma unroll
+                                for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                                    for (int r = 0; r < RT; ++r) {
+                                        if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
+                                        else mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
+                                        mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
+                                    }
+                            }
                         }
+                        // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(by[r][i >> 1], sum[r][t][i], total[r][t][i]);
                     }
-                    // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(__uint_as_float(s[u][r][i >> 1][q] << scale_shift), sum[r][t][i], total[r][t][i]);
                 }
+                fetch_codes(u);
             }
-            fetch(u);
-            if (++round < rounds) continue;
-            round = 0;
-            // the tile's sums: every warp's into this round's buffer, then added in the order of the warps
+            advance();
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    *reinterpret_cast<float4 *>(&partial[buffer][warp][((r * NT + t) * 32 + lane) * 4]) =
-                        make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
-                }
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
-            for (int i = threadIdx.x; i < kSums; i += 32 * WARPS) {
-                const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
-                const int n = tile * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
-                if (n >= m.rows || row >= M) continue;
-                float v = 0.f;
-#pragma unroll
-                for (int q = 0; q < WARPS; ++q) v += partial[buffer][q][i];
-                if (share > 1) {
-                    partial[buffer][0][i] = v;   // for the cluster's first CTA
-                    continue;
-                }
-                finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
-            }
-            tile += stride;
-            if constexpr (kBuffers == 2) buffer ^= 1;
-            else asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+                    for (int q = 0; q < kGroups; ++q) scale[0][r][half][q] = scale[1][r][half][q], zero[0][r][half][q] = zero[1][r][half][q];
         }
+        // the tile's sums: every warp's into this tile's buffer, then added in the order of the warps
+        float *mine = partial + (buffer * warps + warp) * kSums;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                *reinterpret_cast<float4 *>(mine + ((r * NT + t) * 32 + lane) * 4) = make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < kSums; i += threads) {
+            const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
+            const int n = tile * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
+            if (n >= m.rows || row >= M) continue;
+            float *p = partial + buffer * warps * kSums + i;
+            float v = 0.f;
+            for (int q = 0; q < warps; ++q) v += p[q * kSums];
+            if (share > 1) *p = v;   // for the cluster's first CTA
+            else finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
+        }
+        buffer ^= 1;
     }
-    if (share > 1) {   // one tile a cluster (its sums are in buffer 0)
+    if (share > 1) {   // one tile a cluster: its sums are in buffer 0
         cluster.sync();
         if (rank == 0)
-            for (int i = threadIdx.x; i < kSums; i += 32 * WARPS) {
+            for (int i = threadIdx.x; i < kSums; i += threads) {
                 const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
                 const int n = blockIdx.x / share * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
                 if (n >= m.rows || row >= M) continue;
                 float v = 0.f;
-                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(&partial[0][0][i], q);
+                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + i, q);
                 finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
             }
         cluster.sync();   // the others' shared memory stays until it has been read
     }
 }
 
-// CTAs that share a tile of `outs` outputs: where SMs are left over and a warp would have more than one block.
-static int share_of(const hx_w4_matrix &m, int outs, int warps) {
-    const int64_t tiles = ((int64_t)m.rows + outs - 1) / outs;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sm_count() / tiles, (blocks_of(m.cols) + warps - 1) / warps), 8));
+// How a product is laid out on the SMs.
+struct Plan { int tiles, share, warps, chunk, grid; };
+static Plan plan_of(const hx_w4_matrix &m, int outs, int most) {
+    const int sms = sm_count(), blocks = blocks_of(m.cols);
+    Plan p;
+    p.tiles = (int)(((int64_t)m.rows + outs - 1) / outs);
+    p.share = std::max(1, std::min({sms / p.tiles, (blocks + most - 1) / most, 8}));
+    const int part = (blocks + p.share - 1) / p.share;   // blocks of a CTA
+    if (p.tiles > sms) {   // a stream of tiles: chunks of four, two CTAs of half the warps on an SM
+        p.chunk = part >= 4 ? 4 : part >= 2 ? 2 : 1;
+        most = std::max(most / 2, 1);
+        p.warps = std::min(most, (part + p.chunk - 1) / p.chunk);
+        p.grid = std::min(p.tiles, 2 * most / p.warps * sms);
+    } else {               // one tile a CTA: as many warps as there are blocks
+        p.chunk = part <= most ? 1 : part <= 2 * most ? 2 : 4;
+        p.warps = std::min(most, (part + p.chunk - 1) / p.chunk);
+        p.grid = p.tiles * p.share;
+    }
+    return p;
 }
 
-template <typename TA, int NT, int RT, int GROUP, int WARPS, int XB, bool VEC>
-static hx_status launch_gemm_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
-                                int epilogue, cudaStream_t st) {
-    const int blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + 16 * RT - 1) / (16 * RT));
+template <typename TA, int NT, int RT, int GROUP, int CH, bool VEC>
+static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                           int epilogue, const Plan &p, cudaStream_t st) {
     const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
     HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
-    const int sms = sm_count(), share = share_of(m, 16 * RT, WARPS);
+    auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, VEC>;
+    const size_t smem = (size_t)2 * p.warps * RT * NT * 128 * sizeof(float);
+    if (smem > 48 * 1024) HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min(tiles, sms) * share), (unsigned)down);
-    cfg.blockDim = dim3(32 * WARPS);
+    cfg.gridDim = dim3((unsigned)p.grid, (unsigned)down);
+    cfg.blockDim = dim3(32 * p.warps);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)share;
+    attr.val.clusterDim.x = (unsigned)p.share;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = share > 1 ? 1 : 0;
-    HX_CUDA(cudaLaunchKernelEx(&cfg, gemm_w4_kernel<TA, NT, RT, GROUP, WARPS, XB, VEC>, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M,
-                               blocks, epilogue));
+    cfg.numAttrs = p.share > 1 ? 1 : 0;
+    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue));
     return check_launch("gemm_w4_kernel");
 }
-template <typename TA, int NT, int RT, int WARPS>
+template <typename TA, int NT, int RT>
 static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                              int epilogue, cudaStream_t st) {
     const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
-    const int blocks = blocks_of(m.cols), share = share_of(m, 16 * RT, WARPS), kept = (blocks + share * WARPS - 1) / (share * WARPS);
-#define HX_W4_AS(G, XB, VEC) return launch_gemm_as<TA, NT, RT, G, WARPS, XB, VEC>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st)
-#define HX_W4_GROUP(G)                                                             \
-    do {                                                                           \
-        if constexpr (NT == 1 && sizeof(TA) == 2) {                                \
-            if (vec && kept == 1) HX_W4_AS(G, 1, true);                            \
-            if (vec && kept == 2) HX_W4_AS(G, 2, true);                            \
-        }                                                                          \
-        if (vec) HX_W4_AS(G, 0, true);                                             \
-        HX_W4_AS(G, 0, false);                                                     \
+    const Plan p = plan_of(m, 16 * RT, max_warps(NT));
+#define HX_W4_AS(G, CH, VEC) return launch_as<TA, NT, RT, G, CH, VEC>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, st)
+#define HX_W4_GROUP(G)                              \
+    do {                                            \
+        if (!vec) HX_W4_AS(G, 2, false);            \
+        if (p.chunk == 1) HX_W4_AS(G, 1, true);     \
+        if (p.chunk == 2) HX_W4_AS(G, 2, true);     \
+        HX_W4_AS(G, 4, true);                       \
     } while (0)
     if (m.group == 32) HX_W4_GROUP(32);
     if (m.group == 64) HX_W4_GROUP(64);
@@ -355,10 +357,10 @@ static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, 
 template <typename TA>
 static hx_status gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                       cudaStream_t st) {
-    if (M <= 8) return launch_gemm<TA, 1, 1, 16>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 16) return launch_gemm<TA, 2, 1, 16>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 32) return launch_gemm<TA, 4, 1, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    return launch_gemm<TA, 8, 1, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 8) return launch_gemm<TA, 1, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 16) return launch_gemm<TA, 2, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 32) return launch_gemm<TA, 4, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_gemm<TA, 8, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
 }
 
 }  // namespace w4
