@@ -16,39 +16,51 @@ namespace w4 {
 // (8 rows a tile).  Which column a k index of the MMA stands for does not matter as long as both operands agree; the layout of the
 // codes is such that lane (g, c) = (lane / 4, lane mod 4) finds in its 16 bytes of row g four words, word j holding the columns
 // 32 j + 8 c .. + 7 of the block, as the four k-pairs of two MMAs.  So the MMAs of word j cover columns 32 j .. 32 j + 31 whatever
-// the group size, one LDG.128 brings a lane's share of 128 columns, and the matching piece of A is 16 consecutive bytes.
-// A pair of codes becomes two bf16 numbers with (w >> 4 p & 0x000f000f) | 0x43004300, which is 128 + code exactly, minus 128 + zero,
-// also exact.  Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut
-// into three bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
-// A CTA works through tiles of 16 RT outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
-// block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  The four lanes of a row
-// need the same scales, so lane c loads those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are
-// added in the order of the warps.  Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first
-// one adds the others' sums out of their shared memory.
+// the group size, one 16-byte load brings a lane's share of 128 columns, and the matching piece of A is 8 consecutive elements.
+// Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut into three
+// bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
+//
+// A CTA works through tiles of 16 outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
+// block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  Codes come by cp.async
+// into the lane's own slots and A waits in shared memory (STAGED), so that no load in the loop but the next scales is waited for by
+// scoreboard: loads that miss and loads that hit would share one.  The four lanes of a row need the same scales, so lane c loads
+// those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are added in the order of the warps.
+// Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of
+// their shared memory.
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ uint4 load_codes(const uint8_t *p) {   // read once
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
-// codes 2 p and 2 p + 1 of a word, less the zero point: two bf16.  mask and magic are 0x000f000f and 0x43004300 in registers: one
-// logic instruction takes (shifted & mask) | magic.
-__device__ __forceinline__ uint32_t two_weights(uint32_t word, int p, uint32_t mask, uint32_t magic, uint32_t zero) {
-    uint32_t u;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(u) : "r"(word >> (4 * p)), "r"(mask), "r"(magic));
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), *reinterpret_cast<const __nv_bfloat162 *>(&zero));
-    return *reinterpret_cast<const uint32_t *>(&v);
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The eight codes of a word as four pairs of bf16, each (code - zero) / 64.  The bits of a bf16 whose exponent field is 0 or 1 read
+// as an integer times 2^-133, so a code in bits 0 .. 3 or in bits 4 .. 7 of a half is a number as it stands; one fused multiply-add
+// by 2^127 or 2^123 makes it code / 64 and takes the zero point off, exactly.
+__device__ __forceinline__ uint32_t fma_pair(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
 }
+__device__ __forceinline__ void eight_weights(uint32_t word, uint32_t minus_zero, uint32_t (&a)[4]) {
+    constexpr uint32_t low = 0x7f007f00u, high = 0x7d007d00u;   // 2^127, 2^123
+    const uint32_t next = word >> 8;
+    a[0] = fma_pair(word & 0x000f000fu, low, minus_zero);
+    a[1] = fma_pair(word & 0x00f000f0u, high, minus_zero);
+    a[2] = fma_pair(next & 0x000f000fu, low, minus_zero);
+    a[3] = fma_pair(next & 0x00f000f0u, high, minus_zero);
+}
+constexpr float kSumScale = 64.f;   // what the sums have to be multiplied by in the end
 
 constexpr int max_warps(int NT) { return NT == 1 ? 16 : 8; }   // of a CTA, by its registers
 
@@ -98,72 +110,100 @@ __device__ __forceinline__ void finish(float v, int n, int row, const float *bia
     else static_cast<float *>(C)[row * ldc + n] = v;
 }
 
-// NT tiles of 8 rows of A, RT of 16 outputs, CH blocks of a chunk.
-template <typename TA, int NT, int RT, int GROUP, int CH, bool VEC>
+// Where a warp's partial sum of output n of the tile and row `row` of A lies: [NT][lane][i].
+__device__ __forceinline__ int place(int n, int row) {
+    return ((row >> 3) * 32 + (n & 7) * 4 + ((row & 7) >> 1)) * 4 + (n >> 3) * 2 + (row & 1);
+}
+
+// Bytes from one staged row of A to the next: rows g and g + 1 fall on different banks.
+template <typename TA> __host__ __device__ constexpr size_t staged_pitch(int cols) {
+    return ((size_t)cols * sizeof(TA) + 127) / 128 * 128 + (sizeof(TA) == 2 ? 64 : 16);
+}
+
+enum Rows { kStaged, kDirect, kDirectAny };   // A from shared memory; from global memory in 16-byte loads; at any alignment
+
+// NT tiles of 8 rows of A, CH blocks of a chunk.
+template <typename TA, int NT, int GROUP, int CH, int ROWS>
 __global__ void __launch_bounds__(32 * max_warps(NT), 1)
 gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
-               int64_t ldc, int c_dtype, int M, int blocks, int epilogue) {
-    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = RT * NT * 128;
-    extern __shared__ __align__(16) float partial[];   // [2][warps][kSums]
+               int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
+    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = NT * 128;
+    extern __shared__ __align__(16) float partial[];   // [2][warps][kSums], then the codes' slots, then A
     const auto cluster = cooperative_groups::this_cluster();
     const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();   // CTAs of a tile
     const int warps = blockDim.x / 32, threads = blockDim.x;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int m0 = blockIdx.y * 8 * NT;
+    const int m0 = blockIdx.y * 8 * NT, here = min(M - m0, 8 * NT);                 // rows of A
     const int64_t row_bytes = (int64_t)blocks * kBlockBytes;
-    const int groups = m.cols / GROUP, tiles = (m.rows + 16 * RT - 1) / (16 * RT), stride = gridDim.x / share;
+    const int groups = m.cols / GROUP, tiles = (m.rows + 15) / 16, stride = gridDim.x / share;
     const int first = (rank * warps + warp) * CH, apart = share * warps * CH;   // first block of this warp's chunks
     const int chunks = (blocks + apart - 1) / apart;                            // of a tile, the last one not for all warps
     const bool scale_bf16 = m.scale_dtype == HX_BF16;
     const int scale_shift = scale_bf16 ? 16 : 0;
+    uint4 *slots = reinterpret_cast<uint4 *>(partial + 2 * warps * kSums) + warp * CH * 64 + lane;
 
-    uint32_t mask, magic;   // opaque to the compiler, which would otherwise fold them into two instructions
-    asm volatile("mov.u32 %0, 0x000f000f; mov.u32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
-    const TA *rows[NT];     // this lane's rows of A; past the last one the last, whose sums are then not stored
+    if constexpr (ROWS == kStaged) {
+        unsigned char *staged = reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * 1024;
+        const size_t pitch = staged_pitch<TA>(m.cols);
+        constexpr int per = 16 / (int)sizeof(TA);
+        const int pieces = m.cols / per;
+        for (int i = threadIdx.x; i < here * pieces; i += threads) {
+            const int row = i / pieces, k = i % pieces * per;
+            TA *to = reinterpret_cast<TA *>(staged + row * pitch) + k;
+            const TA *from = A + (int64_t)(m0 + row) * lda + k;
+            if (vec) {
+                cp_async16(to, from);
+            } else {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) rows[t] = A + (int64_t)min(m0 + t * 8 + g, M - 1) * lda + 8 * c;
+                for (int e = 0; e < per; ++e) to[e] = from[e];
+            }
+        }
+        cp_commit();
+    }
+    const TA *rows[NT];   // this lane's rows of A; past the last one the last, whose sums are then not stored
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = min(t * 8 + g, here - 1);
+        if constexpr (ROWS == kStaged)
+            rows[t] = reinterpret_cast<const TA *>(reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * 1024 +
+                                                   row * staged_pitch<TA>(m.cols)) + 8 * c;
+        else rows[t] = A + (int64_t)(m0 + row) * lda + 8 * c;
+    }
 
     // the chunk that is asked for: its tile, its number there, where its rows of codes and scales are
     int ahead_tile = blockIdx.x / share, ahead = 0;
-    const uint8_t *codes[RT][2];
-    int64_t at[RT][2];
+    const uint8_t *codes[2];
+    int64_t at[2];
     auto rows_of = [&](int tile) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int n = min(tile * 16 * RT + r * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
-                codes[r][half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
-                at[r][half] = (int64_t)n * groups + (first + c) * kGroups;
-            }
+        for (int half = 0; half < 2; ++half) {
+            const int n = min(tile * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
+            codes[half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
+            at[half] = (int64_t)n * groups + (first + c) * kGroups;
+        }
     };
-    // What is under way stays as it is loaded: any arithmetic on it would wait for it.
-    uint4 w[CH][RT][2];
-    uint32_t scale[2][RT][2][kGroups], zero[2][RT][2][kGroups];   // of block c of this chunk and of the next
     auto fetch_codes = [&](int u) {
         if (ahead_tile < tiles && first + ahead * apart + u < blocks)
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) w[u][r][half] = load_codes(codes[r][half] + u * kBlockBytes);
+            for (int half = 0; half < 2; ++half) cp_async16(slots + (u * 2 + half) * 32, codes[half] + u * kBlockBytes);
+        cp_commit();
     };
-    auto fetch_scales = [&](uint32_t (&s)[RT][2][kGroups], uint32_t (&z)[RT][2][kGroups]) {
+    // Scales and zero points under way stay as they are loaded: any arithmetic on them would wait for them.
+    uint32_t scale[2][2][kGroups], zero[2][2][kGroups];   // of block c of this chunk and of the next
+    auto fetch_scales = [&](uint32_t (&s)[2][kGroups], uint32_t (&z)[2][kGroups]) {
         const int block = first + ahead * apart + c;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int q = 0; q < kGroups; ++q) {
-                    const bool in = ahead_tile < tiles && c < CH && block * kGroups + q < groups;
-                    s[r][half][q] = 0;
-                    z[r][half][q] = 8;
-                    if (in) {
-                        if (scale_bf16) s[r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
-                        else s[r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
-                        if (m.zero) z[r][half][q] = m.zero[at[r][half] + q];
-                    }
+            for (int q = 0; q < kGroups; ++q) {
+                s[half][q] = 0;
+                z[half][q] = 8;
+                if (ahead_tile < tiles && c < CH && block * kGroups + q < groups) {
+                    if (scale_bf16) s[half][q] = static_cast<const uint16_t *>(m.scale)[at[half] + q];
+                    else s[half][q] = static_cast<const uint32_t *>(m.scale)[at[half] + q];
+                    if (m.zero) z[half][q] = m.zero[at[half] + q];
                 }
+            }
     };
     auto advance = [&]() {
         if (++ahead == chunks) {
@@ -172,12 +212,10 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
             rows_of(ahead_tile);
         } else {
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    codes[r][half] += (int64_t)apart * kBlockBytes;
-                    at[r][half] += (int64_t)apart * kGroups;
-                }
+            for (int half = 0; half < 2; ++half) {
+                codes[half] += (int64_t)apart * kBlockBytes;
+                at[half] += (int64_t)apart * kGroups;
+            }
         }
     };
     rows_of(ahead_tile);
@@ -185,8 +223,12 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
     for (int u = 0; u < CH; ++u) fetch_codes(u);
     fetch_scales(scale[0], zero[0]);
     advance();
+    if constexpr (ROWS == kStaged) {
+        cp_wait<CH>();
+        __syncthreads();
+    }
 
-    float total[RT][NT][4] = {};
+    float total[NT][4] = {};
     int buffer = 0;
     for (int tile = blockIdx.x / share; tile < tiles; tile += stride) {
         for (int chunk = 0; chunk < chunks; ++chunk) {
@@ -194,131 +236,118 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
 #pragma unroll
             for (int u = 0; u < CH; ++u) {
                 const int block = first + chunk * apart + u;
+                cp_wait<CH - 1>();   // the lane's own slots: nobody else to wait for
                 if (block < blocks) {
+                    const uint4 w[2] = {slots[(u * 2) * 32], slots[(u * 2 + 1) * 32]};
 #pragma unroll
                     for (int q = 0; q < kGroups; ++q) {
                         if (GROUP < kBlockCols && block * kGroups + q >= groups) break;   // the filled-up end of a row
-                        float sum[RT][NT][4], by[RT][2];
-                        uint32_t offset[RT][2];   // 128 + zero point, twice
+                        float sum[NT][4], by[2];
+                        uint32_t offset[2];   // -(zero point) / 64, twice
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                by[r][half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][r][half][q], u, 4) << scale_shift);
-                                offset[r][half] = 0x43084308u;
-                                if (m.zero) offset[r][half] = __byte_perm(__shfl_sync(0xffffffffu, zero[0][r][half][q], u, 4), 0x43u, 0x4040u);
-                            }
+                        for (int half = 0; half < 2; ++half) {
+                            by[half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][half][q], u, 4) << scale_shift);
+                            offset[half] = 0xbe00be00u;
+                            if (m.zero) offset[half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
+                        }
 #pragma unroll
                         for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
-                            uint32_t a[RT][2][4];
+                            uint32_t a[2][4];
 #pragma unroll
-                            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                                for (int half = 0; half < 2; ++half) {
-                                    const uint4 v = w[u][r][half];
-                                    const uint32_t word = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
-#pragma unroll
-                                    for (int p = 0; p < 4; ++p) a[r][half][p] = two_weights(word, p, mask, magic, offset[r][half]);
-                                }
+                            for (int half = 0; half < 2; ++half)
+                                eight_weights(j == 0 ? w[half].x : j == 1 ? w[half].y : j == 2 ? w[half].z : w[half].w, offset[half], a[half]);
 #pragma unroll
                             for (int t = 0; t < NT; ++t) {
                                 Operand<TA> b;
-                                b.template load<VEC>(rows[t] + block * kBlockCols + j * 32);
+                                b.template load<ROWS != kDirectAny>(rows[t] + block * kBlockCols + j * 32);
 #pragma unroll
-                                for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                                    for (int r = 0; r < RT; ++r) {
-                                        if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
-                                        else mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
-                                        mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
-                                    }
+                                for (int part = 0; part < kParts; ++part) {
+                                    if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.r[part][0], b.r[part][1]);
+                                    else mma_bf16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.r[part][0], b.r[part][1]);
+                                    mma_bf16(sum[t], a[0][2], a[1][2], a[0][3], a[1][3], b.r[part][2], b.r[part][3]);
+                                }
                             }
                         }
                         // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
+                        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(by[r][i >> 1], sum[r][t][i], total[r][t][i]);
+                            for (int i = 0; i < 4; ++i) total[t][i] = fmaf(by[i >> 1], sum[t][i], total[t][i]);
                     }
                 }
                 fetch_codes(u);
             }
             advance();
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q) scale[0][r][half][q] = scale[1][r][half][q], zero[0][r][half][q] = zero[1][r][half][q];
+                for (int q = 0; q < kGroups; ++q) scale[0][half][q] = scale[1][half][q], zero[0][half][q] = zero[1][half][q];
         }
         // the tile's sums: every warp's into this tile's buffer, then added in the order of the warps
-        float *mine = partial + (buffer * warps + warp) * kSums;
+        float *mine = partial + (buffer * warps + warp) * kSums + lane * 4;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int t = 0; t < NT; ++t) {
+            *reinterpret_cast<float4 *>(mine + t * 128) = make_float4(total[t][0], total[t][1], total[t][2], total[t][3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                *reinterpret_cast<float4 *>(mine + ((r * NT + t) * 32 + lane) * 4) = make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
-            }
+            for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
+        }
         __syncthreads();
-        for (int i = threadIdx.x; i < kSums; i += threads) {
-            const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
-            const int n = tile * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
-            if (n >= m.rows || row >= M) continue;
-            float *p = partial + buffer * warps * kSums + i;
+        for (int i = threadIdx.x; i < 16 * here; i += threads) {   // output i mod 16 of the tile, row i / 16 of A
+            const int n = i & 15, row = i >> 4;
+            if (tile * 16 + n >= m.rows) continue;
+            float *p = partial + buffer * warps * kSums + place(n, row);
             float v = 0.f;
             for (int q = 0; q < warps; ++q) v += p[q * kSums];
             if (share > 1) *p = v;   // for the cluster's first CTA
-            else finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
+            else finish(kSumScale * v, tile * 16 + n, m0 + row, bias, C, ldc, c_dtype, epilogue);
         }
         buffer ^= 1;
     }
     if (share > 1) {   // one tile a cluster: its sums are in buffer 0
         cluster.sync();
         if (rank == 0)
-            for (int i = threadIdx.x; i < kSums; i += threads) {
-                const int ln = (i >> 2) & 31, r = i / (NT * 128), t = i / 128 % NT;
-                const int n = blockIdx.x / share * 16 * RT + r * 16 + ((i >> 1) & 1) * 8 + (ln >> 2), row = m0 + t * 8 + 2 * (ln & 3) + (i & 1);
-                if (n >= m.rows || row >= M) continue;
+            for (int i = threadIdx.x; i < 16 * here; i += threads) {
+                const int n = i & 15, row = i >> 4, out = blockIdx.x / share * 16 + n;
+                if (out >= m.rows) continue;
                 float v = 0.f;
-                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + i, q);
-                finish(v, n, row, bias, C, ldc, c_dtype, epilogue);
+                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + place(n, row), q);
+                finish(kSumScale * v, out, m0 + row, bias, C, ldc, c_dtype, epilogue);
             }
         cluster.sync();   // the others' shared memory stays until it has been read
     }
 }
 
-// How a product is laid out on the SMs.
-struct Plan { int tiles, share, warps, chunk, grid; };
-static Plan plan_of(const hx_w4_matrix &m, int outs, int most) {
-    const int sms = sm_count(), blocks = blocks_of(m.cols);
+// How a product is laid out on the SMs.  More tiles than SMs: chunks of four blocks, and 16 warps' worth of CTAs on an SM, as many
+// as the staged rows of A leave room for; of fewer warps the CTAs have less to add up per tile, of more they have less to walk
+// (1 x 16384 x 4096 bf16: 13.1 us with 4 CTAs of 4, 14.1 with 2 of 8; 1 x 4096 x 4096: 7.4 and 6.9).  Otherwise one tile a CTA, or a
+// cluster, with as many warps as there are blocks.
+constexpr size_t kSmemBytes = 200 * 1024;   // of an SM, for the staged rows and the slots
+struct Plan { int share, warps, chunk, grid; };
+static Plan plan_of(const hx_w4_matrix &m, int most, size_t staged) {
+    const int sms = sm_count(), blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + 15) / 16);
     Plan p;
-    p.tiles = (int)(((int64_t)m.rows + outs - 1) / outs);
-    p.share = std::max(1, std::min({sms / p.tiles, (blocks + most - 1) / most, 8}));
+    p.share = std::max(1, std::min({sms / tiles, (blocks + most - 1) / most, 8}));
     const int part = (blocks + p.share - 1) / p.share;   // blocks of a CTA
-    if (p.tiles > sms) {   // a stream of tiles: chunks of four, two CTAs of half the warps on an SM
+    if (tiles > sms) {
+        int ctas = tiles >= 3 * sms ? 4 : 2;
+        while (ctas > 1 && ctas * (staged + 24 * 1024) > kSmemBytes) ctas /= 2;
         p.chunk = part >= 4 ? 4 : part >= 2 ? 2 : 1;
-        most = std::max(most / 2, 1);
-        p.warps = std::min(most, (part + p.chunk - 1) / p.chunk);
-        p.grid = std::min(p.tiles, 2 * most / p.warps * sms);
-    } else {               // one tile a CTA: as many warps as there are blocks
+        p.warps = std::max(1, std::min(most / ctas, (part + p.chunk - 1) / p.chunk));
+        p.grid = std::min(tiles, std::max(ctas, most / p.warps) * sms);
+    } else {
         p.chunk = part <= most ? 1 : part <= 2 * most ? 2 : 4;
         p.warps = std::min(most, (part + p.chunk - 1) / p.chunk);
-        p.grid = p.tiles * p.share;
+        p.grid = tiles * p.share;
     }
     return p;
 }
 
-template <typename TA, int NT, int RT, int GROUP, int CH, bool VEC>
+template <typename TA, int NT, int GROUP, int CH, int ROWS>
 static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
-                           int epilogue, const Plan &p, cudaStream_t st) {
+                           int epilogue, const Plan &p, size_t smem, bool vec, cudaStream_t st) {
     const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
     HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
-    auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, VEC>;
-    const size_t smem = (size_t)2 * p.warps * RT * NT * 128 * sizeof(float);
+    auto kernel = gemm_w4_kernel<TA, NT, GROUP, CH, ROWS>;
     if (smem > 48 * 1024) HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, (unsigned)down);
@@ -331,36 +360,46 @@ static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, co
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.share > 1 ? 1 : 0;
-    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue));
+    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue, vec));
     return check_launch("gemm_w4_kernel");
 }
-template <typename TA, int NT, int RT>
+template <typename TA, int NT>
 static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                              int epilogue, cudaStream_t st) {
     const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
-    const Plan p = plan_of(m, 16 * RT, max_warps(NT));
-#define HX_W4_AS(G, CH, VEC) return launch_as<TA, NT, RT, G, CH, VEC>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, st)
-#define HX_W4_GROUP(G)                              \
-    do {                                            \
-        if (!vec) HX_W4_AS(G, 2, false);            \
-        if (p.chunk == 1) HX_W4_AS(G, 1, true);     \
-        if (p.chunk == 2) HX_W4_AS(G, 2, true);     \
-        HX_W4_AS(G, 4, true);                       \
+    size_t staged = (size_t)std::min(M, 8 * NT) * staged_pitch<TA>(m.cols);
+    const bool stage = staged + (size_t)max_warps(NT) * (NT * 1024 + 4096) <= kSmemBytes;
+    if (!stage) staged = 0;
+    const Plan p = plan_of(m, max_warps(NT), staged);
+    const size_t smem = (size_t)p.warps * (NT * 1024 + p.chunk * 1024) + staged;   // sums twice, slots
+#define HX_W4_AS(G, CH, ROWS) return launch_as<TA, NT, G, CH, ROWS>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, vec, st)
+#define HX_W4_CHUNK(G, CH)                   \
+    do {                                     \
+        if (stage) HX_W4_AS(G, CH, kStaged); \
+        if (vec) HX_W4_AS(G, CH, kDirect);   \
+        HX_W4_AS(G, CH, kDirectAny);         \
+    } while (0)
+#define HX_W4_GROUP(G)                        \
+    do {                                      \
+        if (p.chunk == 1) HX_W4_CHUNK(G, 1);  \
+        if (p.chunk == 2) HX_W4_CHUNK(G, 2);  \
+        HX_W4_CHUNK(G, 4);                    \
     } while (0)
     if (m.group == 32) HX_W4_GROUP(32);
     if (m.group == 64) HX_W4_GROUP(64);
     HX_W4_GROUP(128);
 #undef HX_W4_GROUP
+#undef HX_W4_CHUNK
 #undef HX_W4_AS
 }
 
 template <typename TA>
 static hx_status gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                       cudaStream_t st) {
-    if (M <= 8) return launch_gemm<TA, 1, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 16) return launch_gemm<TA, 2, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 32) return launch_gemm<TA, 4, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    return launch_gemm<TA, 8, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 8) return launch_gemm<TA, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 16) return launch_gemm<TA, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 32) return launch_gemm<TA, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_gemm<TA, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
 }
 
 }  // namespace w4
