@@ -64,11 +64,13 @@ inline bool aligned8(const void *p, int64_t ld, int dtype) {   // rows whose eve
     return ((uintptr_t)p & 15) == 0 && (ld * (int64_t)dtype_size(dtype)) % 16 == 0;
 }
 
-// C = A W^T (+ bias) (+ activation) on checked arguments; one translation unit per type of A (w4_gemm_bf16.cu, w4_gemm_f32.cu).
+// C = A W^T (+ bias) (+ activation) on checked arguments, in translation units of their own (w4_gemm_*.cu).
 hx_status gemm_bf16(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                     cudaStream_t st);
 hx_status gemm_f32(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                    cudaStream_t st);
+hx_status gemm_f32_rows(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
+                        cudaStream_t st);
 
 }  // namespace w4
 }  // namespace hx

@@ -20,7 +20,7 @@ namespace w4 {
 // Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut into three
 // bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
 //
-// A CTA works through tiles of 16 outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
+// A CTA works through tiles of 16 RT outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
 // block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  Codes come by cp.async
 // into the lane's own slots and A waits in shared memory (STAGED), so that no load in the loop but the next scales is waited for by
 // scoreboard: loads that miss and loads that hit would share one.  The four lanes of a row need the same scales, so lane c loads
@@ -110,9 +110,9 @@ __device__ __forceinline__ void finish(float v, int n, int row, const float *bia
     else static_cast<float *>(C)[row * ldc + n] = v;
 }
 
-// Where a warp's partial sum of output n of the tile and row `row` of A lies: [NT][lane][i].
-__device__ __forceinline__ int place(int n, int row) {
-    return ((row >> 3) * 32 + (n & 7) * 4 + ((row & 7) >> 1)) * 4 + (n >> 3) * 2 + (row & 1);
+// Where a warp's partial sum of output n of the tile and row `row` of A lies: [RT][NT][lane][i].
+template <int NT> __device__ __forceinline__ int place(int n, int row) {
+    return (((n >> 4) * NT + (row >> 3)) * 32 + (n & 7) * 4 + ((row & 7) >> 1)) * 4 + ((n >> 3) & 1) * 2 + (row & 1);
 }
 
 // Bytes from one staged row of A to the next: rows g and g + 1 fall on different banks.
@@ -122,12 +122,12 @@ template <typename TA> __host__ __device__ constexpr size_t staged_pitch(int col
 
 enum Rows { kStaged, kDirect, kDirectAny };   // A from shared memory; from global memory in 16-byte loads; at any alignment
 
-// NT tiles of 8 rows of A, CH blocks of a chunk.
-template <typename TA, int NT, int GROUP, int CH, int ROWS>
+// NT tiles of 8 rows of A, RT of 16 outputs, CH blocks of a chunk.
+template <typename TA, int NT, int RT, int GROUP, int CH, int ROWS>
 __global__ void __launch_bounds__(32 * max_warps(NT), 1)
 gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
                int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
-    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = NT * 128;
+    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = RT * NT * 128, kOuts = 16 * RT;
     extern __shared__ __align__(16) float partial[];   // [2][warps][kSums], then the codes' slots, then A
     const auto cluster = cooperative_groups::this_cluster();
     const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();   // CTAs of a tile
@@ -135,15 +135,15 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int m0 = blockIdx.y * 8 * NT, here = min(M - m0, 8 * NT);                 // rows of A
     const int64_t row_bytes = (int64_t)blocks * kBlockBytes;
-    const int groups = m.cols / GROUP, tiles = (m.rows + 15) / 16, stride = gridDim.x / share;
+    const int groups = m.cols / GROUP, tiles = (m.rows + kOuts - 1) / kOuts, stride = gridDim.x / share;
     const int first = (rank * warps + warp) * CH, apart = share * warps * CH;   // first block of this warp's chunks
     const int chunks = (blocks + apart - 1) / apart;                            // of a tile, the last one not for all warps
     const bool scale_bf16 = m.scale_dtype == HX_BF16;
     const int scale_shift = scale_bf16 ? 16 : 0;
-    uint4 *slots = reinterpret_cast<uint4 *>(partial + 2 * warps * kSums) + warp * CH * 64 + lane;
+    uint4 *slots = reinterpret_cast<uint4 *>(partial + 2 * warps * kSums) + warp * CH * RT * 64 + lane;
 
     if constexpr (ROWS == kStaged) {
-        unsigned char *staged = reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * 1024;
+        unsigned char *staged = reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * RT * 1024;
         const size_t pitch = staged_pitch<TA>(m.cols);
         constexpr int per = 16 / (int)sizeof(TA);
         const int pieces = m.cols / per;
@@ -165,45 +165,51 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
     for (int t = 0; t < NT; ++t) {
         const int row = min(t * 8 + g, here - 1);
         if constexpr (ROWS == kStaged)
-            rows[t] = reinterpret_cast<const TA *>(reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * 1024 +
+            rows[t] = reinterpret_cast<const TA *>(reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * RT * 1024 +
                                                    row * staged_pitch<TA>(m.cols)) + 8 * c;
         else rows[t] = A + (int64_t)(m0 + row) * lda + 8 * c;
     }
 
     // the chunk that is asked for: its tile, its number there, where its rows of codes and scales are
     int ahead_tile = blockIdx.x / share, ahead = 0;
-    const uint8_t *codes[2];
-    int64_t at[2];
+    const uint8_t *codes[RT][2];
+    int64_t at[RT][2];
     auto rows_of = [&](int tile) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int n = min(tile * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
-            codes[half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
-            at[half] = (int64_t)n * groups + (first + c) * kGroups;
-        }
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int n = min(tile * kOuts + r * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
+                codes[r][half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
+                at[r][half] = (int64_t)n * groups + (first + c) * kGroups;
+            }
     };
     auto fetch_codes = [&](int u) {
         if (ahead_tile < tiles && first + ahead * apart + u < blocks)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) cp_async16(slots + (u * 2 + half) * 32, codes[half] + u * kBlockBytes);
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) cp_async16(slots + ((u * RT + r) * 2 + half) * 32, codes[r][half] + u * kBlockBytes);
         cp_commit();
     };
     // Scales and zero points under way stay as they are loaded: any arithmetic on them would wait for them.
-    uint32_t scale[2][2][kGroups], zero[2][2][kGroups];   // of block c of this chunk and of the next
-    auto fetch_scales = [&](uint32_t (&s)[2][kGroups], uint32_t (&z)[2][kGroups]) {
+    uint32_t scale[2][RT][2][kGroups], zero[2][RT][2][kGroups];   // of block c of this chunk and of the next
+    auto fetch_scales = [&](uint32_t (&s)[RT][2][kGroups], uint32_t (&z)[RT][2][kGroups]) {
         const int block = first + ahead * apart + c;
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                s[half][q] = 0;
-                z[half][q] = 8;
-                if (ahead_tile < tiles && c < CH && block * kGroups + q < groups) {
-                    if (scale_bf16) s[half][q] = static_cast<const uint16_t *>(m.scale)[at[half] + q];
-                    else s[half][q] = static_cast<const uint32_t *>(m.scale)[at[half] + q];
-                    if (m.zero) z[half][q] = m.zero[at[half] + q];
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    s[r][half][q] = 0;
+                    z[r][half][q] = 8;
+                    if (ahead_tile < tiles && c < CH && block * kGroups + q < groups) {
+                        if (scale_bf16) s[r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
+                        else s[r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
+                        if (m.zero) z[r][half][q] = m.zero[at[r][half] + q];
+                    }
                 }
-            }
     };
     auto advance = [&]() {
         if (++ahead == chunks) {
@@ -212,10 +218,12 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
             rows_of(ahead_tile);
         } else {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                codes[half] += (int64_t)apart * kBlockBytes;
-                at[half] += (int64_t)apart * kGroups;
-            }
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    codes[r][half] += (int64_t)apart * kBlockBytes;
+                    at[r][half] += (int64_t)apart * kGroups;
+                }
         }
     };
     rows_of(ahead_tile);
@@ -228,7 +236,7 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
         __syncthreads();
     }
 
-    float total[NT][4] = {};
+    float total[RT][NT][4] = {};
     int buffer = 0;
     for (int tile = blockIdx.x / share; tile < tiles; tile += stride) {
         for (int chunk = 0; chunk < chunks; ++chunk) {
@@ -238,79 +246,95 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
                 const int block = first + chunk * apart + u;
                 cp_wait<CH - 1>();   // the lane's own slots: nobody else to wait for
                 if (block < blocks) {
-                    const uint4 w[2] = {slots[(u * 2) * 32], slots[(u * 2 + 1) * 32]};
+                    uint4 w[RT][2];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) w[r][half] = slots[((u * RT + r) * 2 + half) * 32];
 #pragma unroll
                     for (int q = 0; q < kGroups; ++q) {
                         if (GROUP < kBlockCols && block * kGroups + q >= groups) break;   // the filled-up end of a row
-                        float sum[NT][4], by[2];
-                        uint32_t offset[2];   // -(zero point) / 64, twice
+                        float sum[RT][NT][4], by[RT][2];
+                        uint32_t offset[RT][2];   // -(zero point) / 64, twice
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            by[half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][half][q], u, 4) << scale_shift);
-                            offset[half] = 0xbe00be00u;
-                            if (m.zero) offset[half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
-                        }
+                        for (int r = 0; r < RT; ++r)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                by[r][half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][r][half][q], u, 4) << scale_shift);
+                                offset[r][half] = 0xbe00be00u;
+                                if (m.zero) offset[r][half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][r][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
+                            }
 #pragma unroll
                         for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
-                            uint32_t a[2][4];
+                            uint32_t a[RT][2][4];
 #pragma unroll
-                            for (int half = 0; half < 2; ++half)
-                                eight_weights(j == 0 ? w[half].x : j == 1 ? w[half].y : j == 2 ? w[half].z : w[half].w, offset[half], a[half]);
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int half = 0; half < 2; ++half)
+                                    eight_weights(j == 0 ? w[r][half].x : j == 1 ? w[r][half].y : j == 2 ? w[r][half].z : w[r][half].w, offset[r][half], a[r][half]);
 #pragma unroll
                             for (int t = 0; t < NT; ++t) {
                                 Operand<TA> b;
                                 b.template load<ROWS != kDirectAny>(rows[t] + block * kBlockCols + j * 32);
 #pragma unroll
-                                for (int part = 0; part < kParts; ++part) {
-                                    if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.r[part][0], b.r[part][1]);
-                                    else mma_bf16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.r[part][0], b.r[part][1]);
-                                    mma_bf16(sum[t], a[0][2], a[1][2], a[0][3], a[1][3], b.r[part][2], b.r[part][3]);
-                                }
+                                for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                                    for (int r = 0; r < RT; ++r) {
+                                        if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
+                                        else mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
+                                        mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
+                                    }
                             }
                         }
                         // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
+                        for (int r = 0; r < RT; ++r)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) total[t][i] = fmaf(by[i >> 1], sum[t][i], total[t][i]);
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(by[r][i >> 1], sum[r][t][i], total[r][t][i]);
                     }
                 }
                 fetch_codes(u);
             }
             advance();
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int q = 0; q < kGroups; ++q) scale[0][half][q] = scale[1][half][q], zero[0][half][q] = zero[1][half][q];
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q) scale[0][r][half][q] = scale[1][r][half][q], zero[0][r][half][q] = zero[1][r][half][q];
         }
         // the tile's sums: every warp's into this tile's buffer, then added in the order of the warps
         float *mine = partial + (buffer * warps + warp) * kSums + lane * 4;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            *reinterpret_cast<float4 *>(mine + t * 128) = make_float4(total[t][0], total[t][1], total[t][2], total[t][3]);
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
-        }
+            for (int t = 0; t < NT; ++t) {
+                *reinterpret_cast<float4 *>(mine + (r * NT + t) * 128) = make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
+            }
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * here; i += threads) {   // output i mod 16 of the tile, row i / 16 of A
-            const int n = i & 15, row = i >> 4;
-            if (tile * 16 + n >= m.rows) continue;
-            float *p = partial + buffer * warps * kSums + place(n, row);
+        for (int i = threadIdx.x; i < kOuts * here; i += threads) {
+            const int n = i % kOuts, row = i / kOuts;
+            if (tile * kOuts + n >= m.rows) continue;
+            float *p = partial + buffer * warps * kSums + place<NT>(n, row);
             float v = 0.f;
             for (int q = 0; q < warps; ++q) v += p[q * kSums];
             if (share > 1) *p = v;   // for the cluster's first CTA
-            else finish(kSumScale * v, tile * 16 + n, m0 + row, bias, C, ldc, c_dtype, epilogue);
+            else finish(kSumScale * v, tile * kOuts + n, m0 + row, bias, C, ldc, c_dtype, epilogue);
         }
         buffer ^= 1;
     }
     if (share > 1) {   // one tile a cluster: its sums are in buffer 0
         cluster.sync();
         if (rank == 0)
-            for (int i = threadIdx.x; i < 16 * here; i += threads) {
-                const int n = i & 15, row = i >> 4, out = blockIdx.x / share * 16 + n;
+            for (int i = threadIdx.x; i < kOuts * here; i += threads) {
+                const int n = i % kOuts, row = i / kOuts, out = blockIdx.x / share * kOuts + n;
                 if (out >= m.rows) continue;
                 float v = 0.f;
-                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + place(n, row), q);
+                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + place<NT>(n, row), q);
                 finish(kSumScale * v, out, m0 + row, bias, C, ldc, c_dtype, epilogue);
             }
         cluster.sync();   // the others' shared memory stays until it has been read
@@ -323,8 +347,8 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
 // cluster, with as many warps as there are blocks.
 constexpr size_t kSmemBytes = 200 * 1024;   // of an SM, for the staged rows and the slots
 struct Plan { int share, warps, chunk, grid; };
-static Plan plan_of(const hx_w4_matrix &m, int most, size_t staged) {
-    const int sms = sm_count(), blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + 15) / 16);
+static Plan plan_of(const hx_w4_matrix &m, int outs, int most, size_t staged) {
+    const int sms = sm_count(), blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + outs - 1) / outs);
     Plan p;
     p.share = std::max(1, std::min({sms / tiles, (blocks + most - 1) / most, 8}));
     const int part = (blocks + p.share - 1) / p.share;   // blocks of a CTA
@@ -342,12 +366,12 @@ static Plan plan_of(const hx_w4_matrix &m, int most, size_t staged) {
     return p;
 }
 
-template <typename TA, int NT, int GROUP, int CH, int ROWS>
+template <typename TA, int NT, int RT, int GROUP, int CH, int ROWS>
 static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                            int epilogue, const Plan &p, size_t smem, bool vec, cudaStream_t st) {
     const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
     HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
-    auto kernel = gemm_w4_kernel<TA, NT, GROUP, CH, ROWS>;
+    auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, ROWS>;
     if (smem > 48 * 1024) HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, (unsigned)down);
@@ -363,44 +387,40 @@ static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, co
     HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue, vec));
     return check_launch("gemm_w4_kernel");
 }
-template <typename TA, int NT>
+template <typename TA, int NT, int RT>
 static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                              int epilogue, cudaStream_t st) {
     const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
     size_t staged = (size_t)std::min(M, 8 * NT) * staged_pitch<TA>(m.cols);
-    const bool stage = staged + (size_t)max_warps(NT) * (NT * 1024 + 4096) <= kSmemBytes;
+    const bool stage = staged + (size_t)max_warps(NT) * RT * (NT * 1024 + (RT > 1 ? 2048 : 4096)) <= kSmemBytes;
     if (!stage) staged = 0;
-    const Plan p = plan_of(m, max_warps(NT), staged);
-    const size_t smem = (size_t)p.warps * (NT * 1024 + p.chunk * 1024) + staged;   // sums twice, slots
-#define HX_W4_AS(G, CH, ROWS) return launch_as<TA, NT, G, CH, ROWS>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, vec, st)
-#define HX_W4_CHUNK(G, CH)                   \
-    do {                                     \
-        if (stage) HX_W4_AS(G, CH, kStaged); \
-        if (vec) HX_W4_AS(G, CH, kDirect);   \
-        HX_W4_AS(G, CH, kDirectAny);         \
-    } while (0)
-#define HX_W4_GROUP(G)                        \
-    do {                                      \
-        if (p.chunk == 1) HX_W4_CHUNK(G, 1);  \
-        if (p.chunk == 2) HX_W4_CHUNK(G, 2);  \
-        HX_W4_CHUNK(G, 4);                    \
+    Plan p = plan_of(m, 16 * RT, max_warps(NT), staged);
+    if (RT > 1 || !stage) p.chunk = 2;   // instances there are; the walk covers any number of blocks
+    else if (NT > 1 && p.chunk == 1) p.chunk = 2;
+    const size_t smem = (size_t)p.warps * RT * (NT * 1024 + p.chunk * 1024) + staged;   // sums twice, slots
+#define HX_W4_AS(G, CH, ROWS) return launch_as<TA, NT, RT, G, CH, ROWS>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, vec, st)
+#define HX_W4_GROUP(G)                                                \
+    do {                                                              \
+        if (!stage && vec) HX_W4_AS(G, 2, kDirect);                   \
+        if (!stage) HX_W4_AS(G, 2, kDirectAny);                       \
+        if constexpr (RT == 1) {                                      \
+            if constexpr (NT == 1) {                                  \
+                if (p.chunk == 1) HX_W4_AS(G, 1, kStaged);            \
+            }                                                         \
+            if (p.chunk == 4) HX_W4_AS(G, 4, kStaged);                \
+        }                                                             \
+        HX_W4_AS(G, 2, kStaged);                                      \
     } while (0)
     if (m.group == 32) HX_W4_GROUP(32);
     if (m.group == 64) HX_W4_GROUP(64);
     HX_W4_GROUP(128);
 #undef HX_W4_GROUP
-#undef HX_W4_CHUNK
 #undef HX_W4_AS
 }
 
-template <typename TA>
-static hx_status gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
-                      cudaStream_t st) {
-    if (M <= 8) return launch_gemm<TA, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 16) return launch_gemm<TA, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 32) return launch_gemm<TA, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    return launch_gemm<TA, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-}
+// Whether tiles of `outs` outputs still fill the SMs.
+static bool fills(const hx_w4_matrix &m, int outs) { return (int64_t)m.rows * 3 >= (int64_t)outs * sm_count() * 2; }
+#define HX_W4_ROWS(TA, NT, RT) return launch_gemm<TA, NT, RT>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st)
 
 }  // namespace w4
 }  // namespace hx
