@@ -599,11 +599,12 @@ static size_t map_bytes(int batch, int d_inner, const Plan &plan) {
     return (size_t)(plan.segs - 1) * batch * ((d_inner + 1) & ~1) * sizeof(float2);
 }
 
-template <typename K, typename Args>
-static hx_status launch(K kernel, size_t ring, bool chained, int64_t warps, const Args &args, const Plan &plan, const char *name, cudaStream_t st) {
+template <auto KERNEL, typename Args>
+static hx_status launch(size_t ring, bool chained, int64_t warps, const Args &args, const Plan &plan, const char *name, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
     const int64_t ctas = (warps + kWarps - 1) / kWarps;
     HX_REQUIRE(ctas <= 0x7fffffff, HX_ERR_INVALID_DIMENSION, "%s: batch * d_inner is too large for one launch", name);
-    HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kWarps * ring)));
+    if (kWarps * ring > 48 * 1024) HX_CUDA(allow_smem((const void *)KERNEL, kWarps * ring, done));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(32 * kWarps);
@@ -614,25 +615,25 @@ static hx_status launch(K kernel, size_t ring, bool chained, int64_t warps, cons
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = chained ? 1 : 0;
-    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args, static_cast<float2 *>(args.workspace), plan.seg_len, plan.segs));
+    HX_CUDA(cudaLaunchKernelEx(&cfg, KERNEL, args, static_cast<float2 *>(args.workspace), plan.seg_len, plan.segs));
     return check_launch(name);
 }
 template <typename T, int GATE, int PIECE> static hx_status launch_fwd(const hx_gated_scan_args &a, const Plan &plan, cudaStream_t st) {
     const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
     const size_t ring = sizeof(T[kStages][2][kRun][kC]);
     if (plan.segs > 1) {
-        const hx_status s = launch(gated_scan_kernel<T, GATE, PIECE, true>, ring, false, chains * (plan.segs - 1), a, plan, "gated_scan_kernel", st);
+        const hx_status s = launch<gated_scan_kernel<T, GATE, PIECE, true>>(ring, false, chains * (plan.segs - 1), a, plan, "gated_scan_kernel", st);
         if (s != HX_OK) return s;
     }
-    return launch(gated_scan_kernel<T, GATE, PIECE, false>, ring, plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_kernel", st);
+    return launch<gated_scan_kernel<T, GATE, PIECE, false>>(ring, plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_kernel", st);
 }
 template <typename T, int GATE, int PIECE> static hx_status launch_bwd(const hx_gated_scan_bwd_args &a, const Plan &plan, cudaStream_t st) {
     const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
     if (plan.segs > 1) {
-        const hx_status s = launch(gated_scan_bwd_kernel<T, GATE, PIECE, true>, sizeof(T[kStages][2][kRun][kC]), false, chains * (plan.segs - 1), a, plan, "gated_scan_bwd_kernel", st);
+        const hx_status s = launch<gated_scan_bwd_kernel<T, GATE, PIECE, true>>(sizeof(T[kStages][2][kRun][kC]), false, chains * (plan.segs - 1), a, plan, "gated_scan_bwd_kernel", st);
         if (s != HX_OK) return s;
     }
-    return launch(gated_scan_bwd_kernel<T, GATE, PIECE, false>, sizeof(T[kBlockStages][3][kBlock][kC]), plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_bwd_kernel", st);
+    return launch<gated_scan_bwd_kernel<T, GATE, PIECE, false>>(sizeof(T[kBlockStages][3][kBlock][kC]), plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_bwd_kernel", st);
 }
 // The plan a call may use: one segment where it brings no workspace.
 template <typename Args> static hx_status choose_plan(const char *who, const Args &a, Plan *plan) {

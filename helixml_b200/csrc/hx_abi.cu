@@ -32,6 +32,17 @@ int sm_count() {
     return cached[dev];
 }
 
+cudaError_t allow_smem(const void *kernel, size_t bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
+    if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 // ---- block cache of the module layer's tensors: whole cudaMalloc blocks, one free list per device keyed by size
 namespace {
 struct Pool {

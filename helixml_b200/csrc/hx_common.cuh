@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -41,6 +42,9 @@ inline size_t dtype_size(int dt) { return dt == HX_F32 ? 4 : dt == HX_BF16 ? 2 :
 
 // Number of SMs of the current device, cached per device.
 int sm_count();
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device; `done` (one per kernel and size, zero at first) remembers
+// the devices on which that has been asked for.
+cudaError_t allow_smem(const void *kernel, size_t bytes, std::atomic<uint64_t> &done);
 
 // Device memory for the tensors the module layer makes and drops on every call (results, workspaces, uploaded inputs).
 // cudaMalloc and cudaFree cost 0.1 to several ms each and cudaFree waits for the whole device; a freed block is kept

@@ -15,13 +15,24 @@ __device__ __forceinline__ float round_quotient(float w, float s, float inv) {
     return n;
 }
 
+// Row and column of item i of a matrix with `across` items a row; nearly always 32 bits do.
+__device__ __forceinline__ void split(int64_t i, int across, int64_t &row, int &col) {
+    if (i >> 32 == 0) {
+        row = (uint32_t)i / (uint32_t)across;
+        col = (int)((uint32_t)i - (uint32_t)row * (uint32_t)across);
+    } else {
+        row = i / across;
+        col = (int)(i - row * across);
+    }
+}
+
 // One thread per word of 8 columns, 16 threads per block of 128; a group's 4, 8 or 16 threads meet in shuffles.
 template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int blocks, bool vec) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;   // word of the matrix, in the order of rows and columns
-    const int64_t n = i / (blocks * 16);
-    const int w = (int)(i % (blocks * 16));
+    int64_t n;   // row, and the word of the row
+    int w;
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, blocks * 16, n, w);
     const bool live = n < m.rows && w * 8 < m.cols;
     float v[8] = {};
     if (live) load8(W + n * ldw + w * 8, vec, v);
@@ -68,9 +79,9 @@ quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int 
 
 __global__ void __launch_bounds__(256)
 pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, int blocks) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t n = i / (blocks * 16);
-    const int w = (int)(i % (blocks * 16));
+    int64_t n;
+    int w;
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, blocks * 16, n, w);
     if (n >= m.rows) return;
     uint32_t word = kFill;
     if (w * 8 < m.cols) {
@@ -85,10 +96,9 @@ pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, i
 template <typename T>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int blocks, bool vec) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int words = m.cols / 8;
-    const int64_t n = i / words;
-    const int w = (int)(i % words);
+    int64_t n;
+    int w;
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, m.cols / 8, n, w);
     if (n >= m.rows) return;
     const uint32_t word = reinterpret_cast<const uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)];
     const int64_t at = n * (m.cols / m.group) + w / (m.group / 8);

@@ -372,7 +372,8 @@ static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, co
     const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
     HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
     auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, ROWS>;
-    if (smem > 48 * 1024) HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done{0};
+    if (smem > 48 * 1024) HX_CUDA(allow_smem((const void *)kernel, kSmemBytes + 16 * 1024, done));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, (unsigned)down);
     cfg.blockDim = dim3(32 * p.warps);

@@ -192,12 +192,18 @@ def _cuda(name, t) -> int:
 
 
 def _like(name, t, shape, dtype, dev):
+    if t.shape == shape and t.dtype == dtype and t.get_device() == dev:
+        return
     if t.get_device() != dev:
         raise L.HxError(3, f"{name} is on {t.device}, expected cuda:{dev}")
     if t.dtype != dtype:
         raise L.HxError(4, f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.shape != shape:
-        raise L.HxError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    raise L.HxError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _same(t):
+    """An uninitialised dense tensor like t (torch.empty takes twice as long)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _dense(name, t, shape, dtype, dev):
@@ -241,7 +247,7 @@ def _gated_scan_workspace_bytes(dev, batch, seq_len, d_inner, dtype) -> int:
 def _gated_scan_workspace(dev, batch, seq_len, d_inner, dtype):
     """The memory a call needs whose sequence is cut into segments."""
     n = _gated_scan_workspace_bytes(dev, batch, seq_len, d_inner, dtype)
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=dev) if n else None
 
 
 def _state_rows(seq_len):
@@ -265,14 +271,14 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     gb, gr = _view3(g)
     Bsz, Lq, Dm = shape
     if out is None:
-        h = torch.empty(shape, dtype=x.dtype, device=dev)
+        h = _same(x)
     else:
         h = out
         _like("out", h, shape, x.dtype, dev)
     hb, hr = _view3(h)
     h0 = _dense("h0", h0, (Bsz, Dm), torch.float32, dev)
     lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
-    last = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev) if return_state else None
+    last = torch.empty_strided((Bsz, Dm), (Dm, 1), dtype=torch.float32, device=dev) if return_state else None
     if states is not None:
         _dense_out("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
     ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
@@ -295,7 +301,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     db, dr = _view3(dh)
     Bsz, Lq, Dm = shape
     if out is None:
-        dx, dg = torch.empty(shape, dtype=x.dtype, device=dev), torch.empty(shape, dtype=x.dtype, device=dev)
+        dx, dg = _same(x), _same(x)
     else:
         dx, dg = out
         _like("dx", dx, shape, x.dtype, dev)
@@ -305,7 +311,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     states = _dense("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
     dh_last = _dense("dh_last", dh_last, (Bsz, Dm), torch.float32, dev)
     lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
-    dh0 = torch.empty((Bsz, Dm), dtype=torch.float32, device=dev)
+    dh0 = torch.empty_strided((Bsz, Dm), (Dm, 1), dtype=torch.float32, device=dev)
     ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
     a = L.GatedScanBwdArgs(Bsz, Lq, Dm, dt, _gate(gate), 0, x.data_ptr(), g.data_ptr(), dh.data_ptr(), dx.data_ptr(), dg.data_ptr(), xb,
                            xr, gb, gr, db, dr, dxb, dxr, dgb, dgr, _at(states), _at(dh_last), _at(dh0), _at(lengths), _at(ws),
@@ -328,7 +334,7 @@ def gated_scan_step(x, g, h, gate="sigmoid", h_out=None, out=None):
     else:
         _dense_out("h_out", h_out, shape, torch.float32, dev)
     if out is None:
-        y = torch.empty(shape, dtype=x.dtype, device=dev)
+        y = _same(x)
     else:
         y = out
         _like("out", y, shape, x.dtype, dev)
@@ -518,7 +524,7 @@ def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=
         raise L.HxError(3, f"a is on {a.device}, W on {m.codes.device}")
     bias = _dense("bias", bias, (m.rows,), torch.float32, dev)
     if out is None:
-        c = torch.empty((M, m.rows), dtype=out_dtype or a.dtype, device=dev)
+        c = torch.empty_strided((M, m.rows), (m.rows, 1), dtype=out_dtype or a.dtype, device=dev)
         ldc = m.rows
     else:
         c = out
