@@ -5,16 +5,6 @@
 namespace hx {
 namespace w4 {
 
-// round(w / s) to even as exact arithmetic decides it.  The fp32 quotient w * inv is off by less than 2^-20 for the |w / s| < 17
-// that matter (larger ones are clamped), so only a fraction within 2^-16 of 1/2 can be decided wrongly; there the division is
-// done in double, whose quotient of two fp32 numbers cannot round across a half: the distance of w / s from a half that it does
-// not meet is at least 2^-25 relative.
-__device__ __forceinline__ float round_quotient(float w, float s, float inv) {
-    const float q = w * inv, n = rintf(q);
-    if (fabsf(q - n) > 0.5f - 1.52587890625e-5f || !(fabsf(q) < 1e6f)) return (float)rint((double)w / (double)s);
-    return n;
-}
-
 // Row and column of item i of a matrix with `across` items a row; nearly always 32 bits do.
 __device__ __forceinline__ void split(int64_t i, int across, int64_t &row, int &col) {
     if (i >> 32 == 0) {
@@ -26,55 +16,116 @@ __device__ __forceinline__ void split(int64_t i, int across, int64_t &row, int &
     }
 }
 
-// One thread per word of 8 columns, 16 threads per block of 128; a group's 4, 8 or 16 threads meet in shuffles.
-template <typename T>
+constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer, ties to even, and leaves that in the low bits
+constexpr float kNear = 0.5f - 1.52587890625e-5f;   // 1/2 - 2^-16
+
+// w / s rounded as exact arithmetic decides it, given fp32's q = w * (1 / s) and n, that rounded.  q is off by less than 2^-20 for
+// |w / s| < 17 (larger ones are clamped), so only a q within 2^-16 of a half can have gone to the wrong side, and there the sign of
+// w - half * s, which a fused multiply-add gives exactly, tells.
+__device__ __forceinline__ float settle(float w, float s, float q, float n) {
+    const float e = q - n;
+    if (!(fabsf(e) > kNear)) return n;
+    const float step = e > 0.f ? 1.f : -1.f, d = step * fmaf(-(n + 0.5f * step), s, w);
+    const bool odd = (int)n & 1;
+    return d > 0.f || (d == 0.f && odd) ? n + step : n;
+}
+
+constexpr int kEach = 2;   // words of a thread
+
+// A thread takes 16 columns, two words, 8 threads a block of 128; a group's 2, 4 or 8 threads meet in shuffles.  What bounds it is
+// instructions, 25 a weight.
+template <typename T, bool ZERO>
 __global__ void __launch_bounds__(256)
-quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int blocks, bool vec) {
-    int64_t n;   // row, and the word of the row
-    int w;
-    split((int64_t)blockIdx.x * 256 + threadIdx.x, blocks * 16, n, w);
-    const bool live = n < m.rows && w * 8 < m.cols;
-    float v[8] = {};
-    if (live) load8(W + n * ldw + w * 8, vec, v);
-    float lo = 0.f, hi = 0.f;
-    bool bad = false;
+quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int blocks, int shift, bool vec) {   // group = 2^shift
+    constexpr int per = 8 * kEach;
+    int64_t n;   // row, and the thread's part of the row
+    int part;
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, blocks * (kBlockCols / per), n, part);
+    const bool live = n < m.rows && part * per < m.cols;
+    float v[kEach][8] = {};
+    if (live) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        bad |= !(fabsf(v[j]) <= 3.402823466e38f);
-        lo = fminf(lo, v[j]);
-        hi = fmaxf(hi, v[j]);
+        for (int i = 0; i < kEach; ++i) load8(W + n * ldw + part * per + i * 8, vec, v[i]);
     }
-    for (int o = 1; o < m.group / 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    float lo = 0.f, hi = 0.f, bad = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            bad = fmaf(v[i][j], 0.f, bad);   // NaN from the first infinity or NaN on
+            if constexpr (ZERO) lo = fminf(lo, v[i][j]), hi = fmaxf(hi, v[i][j]);
+            else hi = fmaxf(hi, fabsf(v[i][j]));
+        }
+    if (bad != bad) hi = __int_as_float(0x7f800000);   // travels with the maximum
+    for (int o = 1; o << 4 < m.group; o <<= 1) {   // 16 columns a thread
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+        if constexpr (ZERO) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
     if (n >= m.rows) return;
-    uint32_t word = kFill;
-    if (live) {
-        float s = m.zero ? (float)(((double)hi - (double)lo) / 15.0) : (float)((double)fmaxf(hi, -lo) / 7.0);
-        if (m.scale_dtype == HX_BF16) s = __bfloat162float(__float2bfloat16_rn(s));
-        if (bad) s = __int_as_float(0x7fc00000);
-        float zero = 8.f;
-        if (s > 0.f) {   // neither zero nor NaN
-            const float inv = 1.0f / s;
-            if (m.zero) zero = fminf(fmaxf(round_quotient(-lo, s, inv), 0.f), 15.f);
-            const float low = m.zero ? 0.f : 1.f;
-            word = 0;
+    uint32_t word[kEach];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float q = fminf(fmaxf(round_quotient(v[j], s, inv) + zero, low), 15.f);
-                word |= (uint32_t)q << (4 * nibble_of(j));
+    for (int i = 0; i < kEach; ++i) word[i] = kFill;
+    if (live) {
+        float s, zero = 8.f;
+        if constexpr (ZERO) {
+            const double d = (double)hi - (double)lo;
+            s = (float)d / 15.f;
+            if ((double)(float)d != d) s = (float)(d / 15.0);
+        } else {
+            s = hi / 7.f;
+        }
+        if (m.scale_dtype == HX_BF16) s = __bfloat162float(__float2bfloat16_rn(s));
+        if (hi > 3.402823466e38f) s = __int_as_float(0x7fc00000);
+        if (s > 0.f) {   // neither zero nor NaN
+            float t = s;   // the divisor, out of the range where its reciprocal overflows
+            if (s < 0x1p-100f) {
+                t *= 0x1p100f;
+                lo *= 0x1p100f;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] *= 0x1p100f;
+            }
+            const float inv = 1.f / t;
+            if constexpr (ZERO) {
+                const float q = fminf(-lo * inv, 16.f);
+                zero = fminf(fmaxf(settle(-lo, t, q, (q + kRound) - kRound), 0.f), 15.f);
+            }
+            const float low = (ZERO ? 0.f : 1.f) - zero, high = 15.f - zero;
+            const uint32_t add = (uint32_t)zero;   // 15 + 15 at most: no carry out of what is kept
+            float worst = 0.f;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                word[i] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float q = fminf(fmaxf(v[i][j] * inv, low), high), u = q + kRound;
+                    worst = fmaxf(worst, fabsf(q - (u - kRound)));
+                    word[i] |= ((__float_as_uint(u) + add) & 15u) << (4 * nibble_of(j));
+                }
+            }
+            if (worst > kNear) {
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    word[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float q = fminf(fmaxf(v[i][j] * inv, low), high);
+                        word[i] |= (uint32_t)(settle(v[i][j], t, q, (q + kRound) - kRound) + zero) << (4 * nibble_of(j));
+                    }
+                }
             }
         }
-        if (w % (m.group / 8) == 0) {
-            const int64_t at = n * (m.cols / m.group) + w / (m.group / 8);
+        if ((part * per & (m.group - 1)) == 0) {
+            const int64_t at = n * (m.cols >> shift) + (part * per >> shift);
             if (m.scale_dtype == HX_BF16) static_cast<__nv_bfloat16 *>(m.scale)[at] = __float2bfloat16_rn(s);
             else static_cast<float *>(m.scale)[at] = s;
-            if (m.zero) m.zero[at] = (uint8_t)zero;
+            if constexpr (ZERO) m.zero[at] = (uint8_t)zero;
         }
     }
-    reinterpret_cast<uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)] = word;
+    uint32_t *row = reinterpret_cast<uint32_t *>(m.codes) + (n * blocks + part / (16 / kEach)) * 16;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) row[word_at(part % (16 / kEach) * kEach + i)] = word[i];
 }
 
 __global__ void __launch_bounds__(256)
@@ -93,20 +144,21 @@ pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, i
     reinterpret_cast<uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)] = word;
 }
 
+// A thread per word: its 8 values are 32 or 16 consecutive bytes.
 template <typename T>
 __global__ void __launch_bounds__(256)
-dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int blocks, bool vec) {
+dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int blocks, int shift, bool vec) {
     int64_t n;
     int w;
-    split((int64_t)blockIdx.x * 256 + threadIdx.x, m.cols / 8, n, w);
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, m.cols >> 3, n, w);
     if (n >= m.rows) return;
-    const uint32_t word = reinterpret_cast<const uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)];
-    const int64_t at = n * (m.cols / m.group) + w / (m.group / 8);
+    const uint32_t word = reinterpret_cast<const uint32_t *>(m.codes)[(n * blocks + (w >> 4)) * 16 + word_at(w & 15)];
+    const int64_t at = n * (m.cols >> shift) + (w * 8 >> shift);
     const float s = load_scale(m.scale, m.scale_dtype, at);
-    const int zero = m.zero ? m.zero[at] : 8;
+    const float base = 8388608.f + (float)(m.zero ? m.zero[at] : 8);   // 2^23: a code in its low bits adds itself
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = s * (float)((int)((word >> (4 * nibble_of(j))) & 15) - zero);
+    for (int j = 0; j < 8; ++j) v[j] = s * (__uint_as_float(((word >> (4 * nibble_of(j))) & 15u) | 0x4b000000u) - base);
     store8(W + n * ldw + w * 8, vec, v);
 }
 
@@ -150,11 +202,20 @@ hx_status hx_w4_quantize(const void *W, int64_t ldw, int32_t w_dtype, const hx_w
     HX_REQUIRE(ldw >= 0, HX_ERR_INVALID_INPUT, "hx_w4_quantize: negative stride");
     const int blocks = blocks_of(m->cols);
     unsigned grid;
-    const hx_status g = grid_of("hx_w4_quantize", (int64_t)m->rows * blocks * 16, &grid);
+    const hx_status g = grid_of("hx_w4_quantize", (int64_t)m->rows * blocks * (16 / kEach), &grid);
     if (g != HX_OK) return g;
     const bool vec = aligned8(W, ldw, w_dtype);
-    if (w_dtype == HX_BF16) quantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(static_cast<const __nv_bfloat16 *>(W), ldw, *m, blocks, vec);
-    else quantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(static_cast<const float *>(W), ldw, *m, blocks, vec);
+    const int shift = m->group == 32 ? 5 : m->group == 64 ? 6 : 7;
+    auto st = (cudaStream_t)stream;
+    if (w_dtype == HX_BF16) {
+        auto w = static_cast<const __nv_bfloat16 *>(W);
+        if (m->zero) quantize_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(w, ldw, *m, blocks, shift, vec);
+        else quantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(w, ldw, *m, blocks, shift, vec);
+    } else {
+        auto w = static_cast<const float *>(W);
+        if (m->zero) quantize_kernel<float, true><<<grid, 256, 0, st>>>(w, ldw, *m, blocks, shift, vec);
+        else quantize_kernel<float, false><<<grid, 256, 0, st>>>(w, ldw, *m, blocks, shift, vec);
+    }
     return check_launch("quantize_kernel");
 }
 
@@ -183,9 +244,10 @@ hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t 
     const hx_status g = grid_of("hx_w4_dequantize", (int64_t)m->rows * (m->cols / 8), &grid);
     if (g != HX_OK) return g;
     const bool vec = aligned8(W, ldw, w_dtype);
+    const int shift = m->group == 32 ? 5 : m->group == 64 ? 6 : 7;
     const int blocks = blocks_of(m->cols);
-    if (w_dtype == HX_BF16) dequantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(*m, static_cast<__nv_bfloat16 *>(W), ldw, blocks, vec);
-    else dequantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(*m, static_cast<float *>(W), ldw, blocks, vec);
+    if (w_dtype == HX_BF16) dequantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(*m, static_cast<__nv_bfloat16 *>(W), ldw, blocks, shift, vec);
+    else dequantize_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(*m, static_cast<float *>(W), ldw, blocks, shift, vec);
     return check_launch("dequantize_kernel");
 }
 
