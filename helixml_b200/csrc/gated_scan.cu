@@ -199,6 +199,35 @@ __device__ __forceinline__ float4 *map_at(float2 *maps, int seg, int b, int c, i
     return reinterpret_cast<float4 *>(maps + ((int64_t)seg * batch + b) * ((d_inner + 1) & ~1) + c);
 }
 
+// Folds `count` maps onto h, the k-th at `first + k * step`, kFold of them in one round trip to L2 and the next kFold under way.
+// Returns how many are folded: fewer where a map's A or a folded state of one of the warp's channels is not finite.
+constexpr int kFold = 8;
+__device__ __forceinline__ int fold(const float4 *first, int64_t step, int count, bool real, float2 &h) {
+    float4 m[2][kFold];
+    auto load = [&](float4 (&b)[kFold], int k0) {
+#pragma unroll
+        for (int k = 0; k < kFold; ++k) b[k] = k0 + k < count && real ? __ldcg(first + (k0 + k) * step) : make_float4(1.f, 0.f, 1.f, 0.f);
+    };
+    load(m[0], 0);
+    for (int k0 = 0; k0 < count; k0 += 2 * kFold)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int at = k0 + half * kFold;
+            if (at >= count) break;
+            load(m[half ^ 1], at + kFold);
+            float2 next = h;
+            bool odd = false;
+#pragma unroll
+            for (int k = 0; k < kFold; ++k) {
+                next = make_float2(fmaf(m[half][k].x, next.x, m[half][k].y), fmaf(m[half][k].z, next.y, m[half][k].w));
+                odd |= !finite(next) || !finite(make_float2(m[half][k].x, m[half][k].z));
+            }
+            if (__any_sync(0xffffffffu, odd)) return at;
+            h = next;
+        }
+    return count;
+}
+
 // ---------------------------------------------------------------- forward
 // MAP: writes the maps of segments 0 .. segs - 2.  Otherwise: outputs of all segments.
 template <typename T, int GATE, int PIECE, bool MAP>
@@ -250,24 +279,9 @@ gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int seg
         if (p.h0) h = load_some(p.h0 + (int64_t)q.b * p.d_inner + q.c, q.n);
         if (segs > 1) {
             chain_wait();
-            bool odd = false;
-            int j = 0;
-            for (; j < q.seg && !odd; j += 4) {
-                float4 m[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    m[k] = j + k < q.seg && q.n ? *map_at(maps, j + k, q.b, q.c, p.batch, p.d_inner) : make_float4(1.f, 0.f, 1.f, 0.f);
-                float2 next = h;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    next = make_float2(fmaf(m[k].x, next.x, m[k].y), fmaf(m[k].z, next.y, m[k].w));
-                    odd |= !finite(next) || !finite(make_float2(m[k].x, m[k].z));
-                }
-                odd = __any_sync(0xffffffffu, odd);
-                if (odd) break;   // h is the state before segment j
-                h = next;
-            }
-            if (odd)
+            const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
+            const int j = fold(map_at(maps, 0, q.b, q.c, p.batch, p.d_inner), step, q.seg, q.n > 0, h);
+            if (j < q.seg)   // h is the state before segment j: walk on from there
                 for (int64_t t = (int64_t)j * seg_len; t < q.t0; ++t) {
                     float2 a, b, rest;
                     gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), load_some(x + t * p.x_row_stride + 2 * q.lane, q.n), a, b, rest);
@@ -437,24 +451,11 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len,
         float2 state = state_of(0);
         if (segs > 1) {
             chain_wait();
-            bool odd = false;
-            int j = segs - 1;
-            for (; j > q.seg && !odd; j -= 4) {
-                float4 m[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    m[k] = j - k > q.seg && q.n ? *map_at(maps, j - k - 1, q.b, q.c, p.batch, p.d_inner) : make_float4(1.f, 0.f, 1.f, 0.f);
-                float2 next = e;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    next = make_float2(fmaf(m[k].x, next.x, m[k].y), fmaf(m[k].z, next.y, m[k].w));
-                    odd |= !finite(next) || !finite(make_float2(m[k].x, m[k].z));
-                }
-                odd = __any_sync(0xffffffffu, odd);
-                if (odd) break;   // e is the one behind segment j
-                e = next;
-            }
-            if (odd)
+            const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
+            const int count = segs - 1 - q.seg;
+            const int folded = fold(map_at(maps, segs - 2, q.b, q.c, p.batch, p.d_inner), -step, count, q.n > 0, e);
+            const int j = segs - 1 - folded;
+            if (folded < count)   // e is the one behind segment j
                 for (int64_t t = min((int64_t)(j + 1) * seg_len, (int64_t)q.len) - 1; t >= q.t1; --t) {
                     float2 a, b, rest;
                     const float2 d = load_some(dh + t * p.dh_row_stride + 2 * q.lane, q.n);
@@ -582,14 +583,15 @@ static int piece_of(size_t element, std::initializer_list<const void *> bases, s
 // How the sequence is cut.  One segment where a step's channels are at least kStepBytes: a warp takes about 0.04 us a step however
 // little else runs, so from there on a single pass is done before two passes (five tensors instead of three, seven instead of five)
 // have moved their bytes.  16 x 2048 x 1536 fp32 sigmoid: 111 us whole, 144 in two; 4 x 4096 x 1024 bf16: 182 whole, 40 in 27.
-// Otherwise as many segments as give an SM kWarpBytes / element size warps (1 x 16384 x 1536 bf16: 60 us with 64 segments, 67 with
-// 32 or 128; 1 x 32768 x 1536 fp32: 169, 166, 175 us with 16, 32, 64).
-constexpr int64_t kStepBytes = 45000, kWarpBytes = 24;
+// Otherwise as many segments as give an SM kWarpBytes / element size warps (1 x 16384 x 1536 bf16: 61, 49, 49 us with 32, 48, 96;
+// 1 x 32768 x 1536 fp32: 157, 153, 160 with 16, 24, 64), but no more than kMostSegments, whose maps every warp folds
+// (1 x 16384 x 256 bf16: 25 us with 96, 34 with 342).
+constexpr int64_t kStepBytes = 45000, kWarpBytes = 24, kMostSegments = 128;
 struct Plan { int segs, seg_len; };
 static Plan plan_of(int batch, int seq_len, int d_inner, int io_dtype) {
     const int64_t chains = (int64_t)batch * ((d_inner + kC - 1) / kC), e = (int64_t)dtype_size(io_dtype);
     int64_t segs = 1;
-    if ((int64_t)batch * d_inner * e < kStepBytes) segs = std::max<int64_t>(kWarpBytes / e * sm_count() / chains, 1);
+    if ((int64_t)batch * d_inner * e < kStepBytes) segs = std::min(std::max<int64_t>(kWarpBytes / e * sm_count() / chains, 1), kMostSegments);
     int64_t seg_len = (seq_len + segs - 1) / segs;
     seg_len = std::max<int64_t>((seg_len + kBlock - 1) / kBlock * kBlock, 2 * kBlock);
     segs = std::max<int64_t>((seq_len + seg_len - 1) / seg_len, 1);
