@@ -116,6 +116,8 @@ __device__ __forceinline__ float2 load2(const __nv_bfloat16 *p) {
 }
 __device__ __forceinline__ void store2(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
 __device__ __forceinline__ void store2(__nv_bfloat16 *p, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y); }
+// what another launch of the call may have written: from L2
+__device__ __forceinline__ float2 load_carry(const float *p, int n) { return make_float2(n > 0 ? __ldcg(p) : 0.f, n > 1 ? __ldcg(p + 1) : 0.f); }
 // the first n of them, at any alignment
 template <typename T> __device__ __forceinline__ float2 load_some(const T *p, int n) {
     return make_float2(n > 0 ? ld_f32(p) : 0.f, n > 1 ? ld_f32(p + 1) : 0.f);
@@ -168,14 +170,23 @@ template <int GATE, bool FAST> __device__ __forceinline__ void gate_step(float2 
     }
 }
 
+// The steps a launch covers, and the state (backwards: e) it starts from and leaves behind.
+struct Span {
+    int begin, end;
+    const float *in;   // [batch, d_inner] or NULL: zero
+    float *out;        // or NULL
+    bool more;         // another launch of the same call follows
+};
+
 // What one warp works on.
 struct Part {
     int b, d0, seg, lane, c, n, cols;   // batch row, first channel of the tile, segment; the lane's channels c.. and how many exist
-    int len;                            // of the batch row
-    int t0, t1;                         // the segment's steps, inside len
+    int len, end;                       // of the batch row, and of what the launch covers of it
+    int t0, t1;                         // the segment's steps, before `end`
     bool live;
 };
-__device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, const int32_t *lengths, int seg_len, int segs) {
+__device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, const int32_t *lengths, const Span &span, int seg_len, int segs,
+                                        int first_seg) {
     Part q;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int tiles = (d_inner + kC - 1) / kC;
@@ -184,14 +195,15 @@ __device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, con
     const int64_t row = q.live ? w / tiles : 0;
     q.d0 = q.live ? (int)(w % tiles) * kC : 0;
     q.b = (int)(row % batch);
-    q.seg = (int)(row / batch);
+    q.seg = (int)(row / batch) + first_seg;
     q.lane = threadIdx.x & 31;
     q.c = q.d0 + 2 * q.lane;
     q.cols = d_inner - q.d0;
     q.n = min(max(d_inner - q.c, 0), 2);
     q.len = lengths ? min(max(lengths[q.b], 0), seq_len) : seq_len;
-    q.t0 = (int)min((int64_t)q.seg * seg_len, (int64_t)q.len);
-    q.t1 = (int)min((int64_t)(q.seg + 1) * seg_len, (int64_t)q.len);
+    q.end = min(q.len, span.end);
+    q.t0 = (int)min(span.begin + (int64_t)q.seg * seg_len, (int64_t)q.end);
+    q.t1 = (int)min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)q.end);
     return q;
 }
 // maps: [segment][batch][d_inner rounded up to 2] pairs (A, B) of a channel
@@ -232,14 +244,14 @@ __device__ __forceinline__ int fold(const float4 *first, int64_t step, int count
 // MAP: writes the maps of segments 0 .. segs - 2.  Otherwise: outputs of all segments.
 template <typename T, int GATE, int PIECE, bool MAP>
 __global__ void __launch_bounds__(32 * kWarps, kOccupancy)
-gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int segs) {
+gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int seg_len, int segs) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int STAGES = kStages;
     extern __shared__ __align__(16) unsigned char smem[];
     using Ring = T[STAGES][2][kRun][kC];
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
-    if constexpr (MAP) chain_trigger();
-    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, seg_len, MAP ? segs - 1 : segs);
+    if (MAP || span.more) chain_trigger();
+    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, 0);
     if (!q.live) return;
     const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
     const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
@@ -276,13 +288,13 @@ gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int seg
     float *states = !MAP && p.states ? p.states + q.b * blocks * p.d_inner + q.c : nullptr;
     const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2, even = p.d_inner % 2 == 0;
     if constexpr (!MAP) {
-        if (p.h0) h = load_some(p.h0 + (int64_t)q.b * p.d_inner + q.c, q.n);
+        if (segs > 1) chain_wait();
+        if (span.in) h = load_carry(span.in + (int64_t)q.b * p.d_inner + q.c, q.n);
         if (segs > 1) {
-            chain_wait();
             const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
             const int j = fold(map_at(maps, 0, q.b, q.c, p.batch, p.d_inner), step, q.seg, q.n > 0, h);
             if (j < q.seg)   // h is the state before segment j: walk on from there
-                for (int64_t t = (int64_t)j * seg_len; t < q.t0; ++t) {
+                for (int64_t t = span.begin + (int64_t)j * seg_len; t < q.t0; ++t) {
                     float2 a, b, rest;
                     gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), load_some(x + t * p.x_row_stride + 2 * q.lane, q.n), a, b, rest);
                     h = fma2(a, h, b);
@@ -347,11 +359,12 @@ gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int seg
         }
     }
     if constexpr (MAP) {
+        chain_wait();   // the launch before this one has read the maps of its span
         if (q.n) *map_at(maps, q.seg, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, h.x, A.y, h.y);
     } else {
-        const int64_t end = q.seg == segs - 1 ? p.seq_len : min((int64_t)(q.seg + 1) * seg_len, (int64_t)p.seq_len);
-        for (int64_t t = max((int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) store_some(out + t * p.h_row_stride, make_float2(0.f, 0.f), q.n);
-        if (p.h_last && q.seg == segs - 1) store_some(p.h_last + (int64_t)q.b * p.d_inner + q.c, h, q.n);
+        const int64_t end = q.seg == segs - 1 ? span.end : min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)span.end);
+        for (int64_t t = max(span.begin + (int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) store_some(out + t * p.h_row_stride, make_float2(0.f, 0.f), q.n);
+        if (span.out && q.seg == segs - 1) store_some(span.out + (int64_t)q.b * p.d_inner + q.c, h, q.n);
     }
 }
 
@@ -360,20 +373,15 @@ gated_scan_kernel(const hx_gated_scan_args p, float2 *maps, int seg_len, int seg
 // walking from the end.
 template <typename T, int GATE, int PIECE, bool MAP>
 __global__ void __launch_bounds__(32 * kWarps, MAP ? kOccupancy : kBlockOccupancy)
-gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len, int segs) {
+gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *maps, int seg_len, int segs) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int STAGES = MAP ? kStages : kBlockStages, ROWS = MAP ? kRun : kBlock, TENSORS = MAP ? 2 : 3;
     extern __shared__ __align__(16) unsigned char smem[];
     using Ring = T[STAGES][TENSORS][ROWS][kC];   // g, dh, x
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
-    if constexpr (MAP) chain_trigger();
-    Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, seg_len, MAP ? segs - 1 : segs);
+    if (MAP || span.more) chain_trigger();
+    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, MAP ? 1 : 0);
     if (!q.live) return;
-    if constexpr (MAP) {
-        ++q.seg;
-        q.t0 = (int)min((int64_t)q.seg * seg_len, (int64_t)q.len);
-        q.t1 = (int)min((int64_t)(q.seg + 1) * seg_len, (int64_t)q.len);
-    }
     const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
     const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
     const T *dh = static_cast<const T *>(p.dh) + q.b * p.dh_batch_stride + q.d0;
@@ -438,9 +446,9 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len,
                 }
             }
         }
+        chain_wait();   // the launch before this one has read the maps of its span
         if (q.n) *map_at(maps, q.seg - 1, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, E.x, A.y, E.y);
     } else {
-        float2 e = p.dh_last ? load_some(p.dh_last + (int64_t)q.b * p.d_inner + q.c, q.n) : make_float2(0.f, 0.f);
         const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
         const bool even = p.d_inner % 2 == 0;
         auto state_of = [&](int r) {   // the state before the r-th block of the walk
@@ -449,14 +457,15 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len,
             return even && q.n == 2 ? load2(st) : load_some(st, q.n);
         };
         float2 state = state_of(0);
+        if (segs > 1) chain_wait();
+        float2 e = span.in ? load_carry(span.in + (int64_t)q.b * p.d_inner + q.c, q.n) : make_float2(0.f, 0.f);
         if (segs > 1) {
-            chain_wait();
             const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
             const int count = segs - 1 - q.seg;
             const int folded = fold(map_at(maps, segs - 2, q.b, q.c, p.batch, p.d_inner), -step, count, q.n > 0, e);
             const int j = segs - 1 - folded;
             if (folded < count)   // e is the one behind segment j
-                for (int64_t t = min((int64_t)(j + 1) * seg_len, (int64_t)q.len) - 1; t >= q.t1; --t) {
+                for (int64_t t = min(span.begin + (int64_t)(j + 1) * seg_len, (int64_t)q.end) - 1; t >= q.t1; --t) {
                     float2 a, b, rest;
                     const float2 d = load_some(dh + t * p.dh_row_stride + 2 * q.lane, q.n);
                     gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), d, a, b, rest);
@@ -518,12 +527,12 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, float2 *maps, int seg_len,
             slot += TENSORS * ROWS * kC;
             if (slot == slot_end) slot = &ring[0][0][0][2 * q.lane];
         }
-        const int64_t end = q.seg == segs - 1 ? p.seq_len : min((int64_t)(q.seg + 1) * seg_len, (int64_t)p.seq_len);
-        for (int64_t t = max((int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) {
+        const int64_t end = q.seg == segs - 1 ? span.end : min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)span.end);
+        for (int64_t t = max(span.begin + (int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) {
             store_some(dx + t * p.dx_row_stride, make_float2(0.f, 0.f), q.n);
             store_some(dg + t * p.dg_row_stride, make_float2(0.f, 0.f), q.n);
         }
-        if (p.dh0 && q.seg == 0) store_some(p.dh0 + (int64_t)q.b * p.d_inner + q.c, e, q.n);
+        if (span.out && q.seg == 0) store_some(span.out + (int64_t)q.b * p.d_inner + q.c, e, q.n);
     }
 }
 
@@ -587,22 +596,36 @@ static int piece_of(size_t element, std::initializer_list<const void *> bases, s
 // 1 x 32768 x 1536 fp32: 157, 153, 160 with 16, 24, 64), but no more than kMostSegments, whose maps every warp folds
 // (1 x 16384 x 256 bf16: 25 us with 96, 34 with 342).
 constexpr int64_t kStepBytes = 45000, kWarpBytes = 24, kMostSegments = 128;
-struct Plan { int segs, seg_len; };
-static Plan plan_of(int batch, int seq_len, int d_inner, int io_dtype) {
-    const int64_t chains = (int64_t)batch * ((d_inner + kC - 1) / kC), e = (int64_t)dtype_size(io_dtype);
-    int64_t segs = 1;
-    if ((int64_t)batch * d_inner * e < kStepBytes) segs = std::min(std::max<int64_t>(kWarpBytes / e * sm_count() / chains, 1), kMostSegments);
-    int64_t seg_len = (seq_len + segs - 1) / segs;
+// Cut sequences whose two tensors of the first launch are more than L2 holds go span by span, so that the second launch of a span
+// finds in L2 what the first has read; the first launch of the next span runs as the second of this one ends.  Forward, 1 x 32768 x
+// 1536 fp32: 161 us whole, 143 in spans of 112 MiB, 133 of 56, 140 of 28.  Backward the second launch has a third tensor to read and
+// two to write, and shorter spans gain less: 1 x 16384 x 4096 bf16 167 us whole, 154 of 112, 147 of 56; fp32 as above 223, 222, 232.
+constexpr int64_t kSpanBytes = (int64_t)56 << 20, kSpanBytesBwd = (int64_t)112 << 20;
+struct Plan { int segs, seg_len, span; };
+static Plan whole(int seq_len) { return {1, 0x7fffffff / kBlock * kBlock, seq_len}; }
+static Plan plan_of(int batch, int seq_len, int d_inner, int io_dtype, int64_t span_bytes) {
+    const int64_t chains = (int64_t)batch * ((d_inner + kC - 1) / kC), e = (int64_t)dtype_size(io_dtype), step = (int64_t)batch * d_inner * e;
+    int64_t segs = 1, span = seq_len;
+    if (step < kStepBytes) {
+        segs = std::min(std::max<int64_t>(kWarpBytes / e * sm_count() / chains, 1), kMostSegments);
+        const int64_t spans = (2 * step * seq_len + span_bytes / 2) / span_bytes;
+        if (spans > 1 && segs > 1) span = ((seq_len + spans - 1) / spans + kBlock - 1) / kBlock * kBlock;
+    }
+    int64_t seg_len = (span + segs - 1) / segs;
     seg_len = std::max<int64_t>((seg_len + kBlock - 1) / kBlock * kBlock, 2 * kBlock);
-    segs = std::max<int64_t>((seq_len + seg_len - 1) / seg_len, 1);
-    return {(int)segs, (int)std::min<int64_t>(seg_len, 0x7fffffff / kBlock * kBlock)};
+    segs = std::max<int64_t>((span + seg_len - 1) / seg_len, 1);
+    if (segs == 1) return whole(seq_len);
+    return {(int)segs, (int)seg_len, (int)span};
 }
-static size_t map_bytes(int batch, int d_inner, const Plan &plan) {
-    return (size_t)(plan.segs - 1) * batch * ((d_inner + 1) & ~1) * sizeof(float2);
+static size_t row_floats(int batch, int d_inner) { return (size_t)batch * ((d_inner + 1) & ~1); }   // of one map's A or B, a multiple of 2
+// the maps, and the states between spans, two that take turns
+static size_t plan_bytes(int batch, int seq_len, int d_inner, const Plan &plan) {
+    if (plan.segs == 1) return 0;
+    return ((size_t)(plan.segs - 1) * 2 + (plan.span < seq_len ? 2 : 0)) * row_floats(batch, d_inner) * sizeof(float);
 }
 
 template <auto KERNEL, typename Args>
-static hx_status launch(size_t ring, bool chained, int64_t warps, const Args &args, const Plan &plan, const char *name, cudaStream_t st) {
+static hx_status launch(size_t ring, bool chained, int64_t warps, const Args &args, const Span &span, const Plan &plan, const char *name, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     const int64_t ctas = (warps + kWarps - 1) / kWarps;
     HX_REQUIRE(ctas <= 0x7fffffff, HX_ERR_INVALID_DIMENSION, "%s: batch * d_inner is too large for one launch", name);
@@ -617,36 +640,48 @@ static hx_status launch(size_t ring, bool chained, int64_t warps, const Args &ar
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = chained ? 1 : 0;
-    HX_CUDA(cudaLaunchKernelEx(&cfg, KERNEL, args, static_cast<float2 *>(args.workspace), plan.seg_len, plan.segs));
+    HX_CUDA(cudaLaunchKernelEx(&cfg, KERNEL, args, span, static_cast<float2 *>(args.workspace), plan.seg_len, plan.segs));
     return check_launch(name);
 }
-template <typename T, int GATE, int PIECE> static hx_status launch_fwd(const hx_gated_scan_args &a, const Plan &plan, cudaStream_t st) {
+// One launch, or two for every span in the order of the walk, each programmatically behind the one before it: MAP(span) starts while
+// OUT(span - 1) ends and waits for it before it writes, OUT(span) waits for MAP(span).
+template <auto MAP, auto OUT, typename Args>
+static hx_status launch_all(size_t map_ring, size_t ring, bool backwards, const float *in, float *out, const Args &a, const Plan &plan,
+                            const char *name, cudaStream_t st) {
     const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
-    const size_t ring = sizeof(T[kStages][2][kRun][kC]);
-    if (plan.segs > 1) {
-        const hx_status s = launch<gated_scan_kernel<T, GATE, PIECE, true>>(ring, false, chains * (plan.segs - 1), a, plan, "gated_scan_kernel", st);
+    if (plan.segs == 1) return launch<OUT>(ring, false, chains, a, Span{0, a.seq_len, in, out, false}, plan, name, st);
+    float *between = static_cast<float *>(a.workspace) + (size_t)(plan.segs - 1) * 2 * row_floats(a.batch, a.d_inner);
+    const int spans = (int)(((int64_t)a.seq_len + plan.span - 1) / plan.span);
+    for (int i = 0; i < spans; ++i) {
+        const int64_t begin = (int64_t)(backwards ? spans - 1 - i : i) * plan.span;
+        Span span{(int)begin, (int)std::min<int64_t>(begin + plan.span, a.seq_len), in, out, i + 1 < spans};
+        if (i > 0) span.in = between + ((i - 1) & 1) * row_floats(a.batch, a.d_inner);
+        if (span.more) span.out = between + (i & 1) * row_floats(a.batch, a.d_inner);
+        hx_status s = launch<MAP>(map_ring, i > 0, chains * (plan.segs - 1), a, span, plan, name, st);
+        if (s == HX_OK) s = launch<OUT>(ring, true, chains * plan.segs, a, span, plan, name, st);
         if (s != HX_OK) return s;
     }
-    return launch<gated_scan_kernel<T, GATE, PIECE, false>>(ring, plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_kernel", st);
+    return HX_OK;
+}
+template <typename T, int GATE, int PIECE> static hx_status launch_fwd(const hx_gated_scan_args &a, const Plan &plan, cudaStream_t st) {
+    constexpr size_t ring = sizeof(T[kStages][2][kRun][kC]);
+    return launch_all<gated_scan_kernel<T, GATE, PIECE, true>, gated_scan_kernel<T, GATE, PIECE, false>>(ring, ring, false, a.h0, a.h_last, a, plan,
+                                                                                                         "gated_scan_kernel", st);
 }
 template <typename T, int GATE, int PIECE> static hx_status launch_bwd(const hx_gated_scan_bwd_args &a, const Plan &plan, cudaStream_t st) {
-    const int64_t chains = (int64_t)a.batch * ((a.d_inner + kC - 1) / kC);
-    if (plan.segs > 1) {
-        const hx_status s = launch<gated_scan_bwd_kernel<T, GATE, PIECE, true>>(sizeof(T[kStages][2][kRun][kC]), false, chains * (plan.segs - 1), a, plan, "gated_scan_bwd_kernel", st);
-        if (s != HX_OK) return s;
-    }
-    return launch<gated_scan_bwd_kernel<T, GATE, PIECE, false>>(sizeof(T[kBlockStages][3][kBlock][kC]), plan.segs > 1, chains * plan.segs, a, plan, "gated_scan_bwd_kernel", st);
+    return launch_all<gated_scan_bwd_kernel<T, GATE, PIECE, true>, gated_scan_bwd_kernel<T, GATE, PIECE, false>>(
+        sizeof(T[kStages][2][kRun][kC]), sizeof(T[kBlockStages][3][kBlock][kC]), true, a.dh_last, a.dh0, a, plan, "gated_scan_bwd_kernel", st);
 }
+
 // The plan a call may use: one segment where it brings no workspace.
-template <typename Args> static hx_status choose_plan(const char *who, const Args &a, Plan *plan) {
-    *plan = plan_of(a.batch, a.seq_len, a.d_inner, a.io_dtype);
+template <typename Args> static hx_status choose_plan(const char *who, const Args &a, int64_t span_bytes, Plan *plan) {
+    *plan = plan_of(a.batch, a.seq_len, a.d_inner, a.io_dtype, span_bytes);
     if (plan->segs == 1) return HX_OK;
     if (a.workspace == nullptr) {
-        plan->segs = 1;
-        plan->seg_len = 0x7fffffff / kBlock * kBlock;
+        *plan = whole(a.seq_len);
         return HX_OK;
     }
-    const size_t need = map_bytes(a.batch, a.d_inner, *plan);
+    const size_t need = plan_bytes(a.batch, a.seq_len, a.d_inner, *plan);
     HX_REQUIRE(a.workspace_bytes >= need, HX_ERR_INVALID_INPUT, "%s: a workspace of %zu bytes, %zu are needed", who, a.workspace_bytes, need);
     HX_REQUIRE(((uintptr_t)a.workspace & 15) == 0, HX_ERR_INVALID_INPUT, "%s: the workspace must be 16-byte aligned", who);
     return HX_OK;
@@ -694,7 +729,7 @@ hx_status hx_gated_scan_fwd(const hx_gated_scan_args *a, void *stream) {
     const int piece = piece_of(dtype_size(a->io_dtype), {a->x, a->g, a->h},
                                {a->x_batch_stride, a->x_row_stride, a->g_batch_stride, a->g_row_stride, a->h_batch_stride, a->h_row_stride});
     Plan plan;
-    const hx_status ps = choose_plan("hx_gated_scan_fwd", *a, &plan);
+    const hx_status ps = choose_plan("hx_gated_scan_fwd", *a, kSpanBytes, &plan);
     if (ps != HX_OK) return ps;
     HX_GATED_LAUNCH(launch_fwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
 }
@@ -703,7 +738,10 @@ hx_status hx_gated_scan_workspace_bytes(int32_t batch, int32_t seq_len, int32_t 
     HX_REQUIRE(bytes != nullptr, HX_ERR_INVALID_INPUT, "hx_gated_scan_workspace_bytes: bytes is NULL");
     const hx_status s = check_common("hx_gated_scan_workspace_bytes", batch, seq_len, d_inner, HX_GATE_DECAY, io_dtype);
     if (s != HX_OK) return s;
-    *bytes = (int64_t)batch * d_inner == 0 ? 0 : map_bytes(batch, d_inner, plan_of(batch, seq_len, d_inner, io_dtype));
+    *bytes = 0;
+    if ((int64_t)batch * d_inner > 0)
+        for (int64_t span_bytes : {kSpanBytes, kSpanBytesBwd})
+            *bytes = std::max(*bytes, plan_bytes(batch, seq_len, d_inner, plan_of(batch, seq_len, d_inner, io_dtype, span_bytes)));
     return HX_OK;
 }
 
@@ -726,7 +764,7 @@ hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *a, void *stream) {
                                {a->x_batch_stride, a->x_row_stride, a->g_batch_stride, a->g_row_stride, a->dh_batch_stride,
                                 a->dh_row_stride, a->dx_batch_stride, a->dx_row_stride, a->dg_batch_stride, a->dg_row_stride});
     Plan plan;
-    const hx_status ps = choose_plan("hx_gated_scan_bwd", *a, &plan);
+    const hx_status ps = choose_plan("hx_gated_scan_bwd", *a, kSpanBytesBwd, &plan);
     if (ps != HX_OK) return ps;
     HX_GATED_LAUNCH(launch_bwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
 }

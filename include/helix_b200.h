@@ -335,8 +335,8 @@ typedef struct hx_gated_scan_args {
     size_t workspace_bytes;
 } hx_gated_scan_args;
 HX_API hx_status hx_gated_scan_fwd(const hx_gated_scan_args *args, void *stream);
-/* Bytes of `workspace` for the forward and the backward pass of these sizes on the current device: 8 bytes per channel, batch row
- * and segment the sequence is cut into (0: it is not). */
+/* Bytes of `workspace` that serve the forward and the backward pass of these sizes on the current device: 8 bytes per channel, batch
+ * row and segment the sequence is cut into, and the states between the spans of a very long one (0: it is not cut). */
 HX_API hx_status hx_gated_scan_workspace_bytes(int32_t batch, int32_t seq_len, int32_t d_inner, int32_t io_dtype, size_t *bytes);
 
 /* Its gradients.  With dh = dL/dh and dh_last = dL/dh_last, from the end of each sequence:

@@ -146,6 +146,31 @@ def test_long_memory_over_many_tiles(dtype, gate):
     check(x, g, h0, dh, dh_last, gate)
 
 
+@pytest.mark.parametrize("dtype,gate,shape,lengths", [("f32", "decay", (1, 22500, 1030), None),
+                                                      ("bf16", "sigmoid", (3, 16000, 1000), [16000, 37, 11001])])
+def test_inputs_larger_than_the_cache(dtype, gate, shape, lengths):
+    """Long sequences of few channels are worked off span by span; a row may end in any of them."""
+    x, g, h0, dh, dh_last = inputs(6, *shape, dtype, gate, shift=6.0)
+    check(x, g, h0, dh, dh_last, gate, lengths=lengths)
+
+
+def test_infinity_across_spans():
+    """A state that has become infinite in the first span is what the last one starts from, and a gradient the other way."""
+    Lq, D = 24000, 1024
+    a = torch.full((1, Lq, D), 0.5, device="cuda")
+    x, dh = torch.zeros(1, Lq, D, device="cuda"), torch.zeros(1, Lq, D, device="cuda")
+    x[0, 3, 7], dh[0, Lq - 5, 9] = float("inf"), float("-inf")
+    a[0, :, 11], x[0, 12000:, 11] = 2.0, 1.0          # a product that overflows over a state of zero
+    states = ops.gated_scan_states(1, Lq, D)
+    h, last = ops.gated_scan(x, a, gate="decay", states=states, return_state=True)
+    assert torch.isposinf(h[0, 3:, 7]).all() and (h[0, :3, 7] == 0).all() and torch.isposinf(last[0, 7])
+    assert (h[0, :12000, 11] == 0).all() and h[0, 12003, 11].item() == 15.0 and torch.isposinf(last[0, 11])
+    others = [c for c in range(D) if c not in (7, 11)]
+    assert (h[0][:, others] == 0).all()
+    dx, dg, dh0 = ops.gated_scan_bwd(dh, x, a, states, gate="decay")
+    assert torch.isneginf(dx[0, :Lq - 4, 9]).all() and (dx[0, Lq - 4:, 9] == 0).all() and torch.isneginf(dh0[0, 9])
+
+
 @pytest.mark.parametrize("gate", ["decay", "sigmoid"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_padded_batches(dtype, gate):
