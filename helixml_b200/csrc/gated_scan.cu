@@ -39,9 +39,9 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // One tensor's way into a warp's ring: pieces of ROWS rows of kC channels, from row `t` of src on.  `cols` channels exist, those
-// behind them are zeros.  PIECE: what every address is a multiple of, in bytes; two-byte pieces go through registers.
+// behind them are zeros.  PIECE: what every address is a multiple of, in bytes.
 template <int ROWS, int PIECE, typename T> struct Feed {
-    static constexpr int per = PIECE >= 4 ? PIECE / (int)sizeof(T) : 1, across = kC / per;   // elements of a piece, pieces of a row
+    static constexpr int per = PIECE / (int)sizeof(T), across = kC / per;   // elements of a piece, pieces of a row
     static constexpr int wide = across < 32 ? across : 32, high = 32 / wide;    // one instruction of the warp: high rows x wide pieces
     static constexpr int turns = across / wide;
     const T *from;        // this lane's first piece of the next fetch
@@ -62,49 +62,68 @@ template <int ROWS, int PIECE, typename T> struct Feed {
     __device__ __forceinline__ void whole(uint32_t slot) {
         const T *f = from;
         from += advance;
-        if constexpr (PIECE >= 4) {
 #pragma unroll
-            for (int r = 0; r < ROWS; r += high) {
+        for (int r = 0; r < ROWS; r += high) {
 #pragma unroll
-                for (int q = 0; q < turns; ++q)
-                    cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, bytes[q]);
-                f += high * row_stride;
-            }
-        } else {
-            copy(slot, f, ROWS);
+            for (int q = 0; q < turns; ++q)
+                cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, bytes[q]);
+            f += high * row_stride;
         }
     }
     // `rows` of them do
     __device__ __forceinline__ void part(uint32_t slot, int rows) {
         const T *f = from;
         from += advance;
-        if constexpr (PIECE >= 4) {
-            const int r0 = (threadIdx.x & 31) / wide;
+        const int r0 = (threadIdx.x & 31) / wide;
 #pragma unroll
-            for (int r = 0; r < ROWS; r += high) {
+        for (int r = 0; r < ROWS; r += high) {
 #pragma unroll
-                for (int q = 0; q < turns; ++q) {
-                    const int n = r0 + r < rows ? bytes[q] : 0;   // nothing is read where n is 0
-                    cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, n);
-                }
-                f += high * row_stride;
+            for (int q = 0; q < turns; ++q) {
+                const int n = r0 + r < rows ? bytes[q] : 0;   // nothing is read where n is 0
+                cp_async<PIECE>(slot + offset + (r * kC + q * wide * per) * (int)sizeof(T), f + q * wide * per, n);
             }
-        } else {
-            copy(slot, f, rows);
+            f += high * row_stride;
         }
     }
-    // two-byte elements at any address: the lane's columns are lane and lane + 32
-    __device__ __forceinline__ void copy(uint32_t slot, const T *f, int rows) {
+    __device__ __forceinline__ int shift(int) const { return 0; }
+};
+
+// Elements from one row of a slot to the next.
+constexpr int pitch_of(int piece) { return piece >= 4 ? kC : kC + 2; }
+
+// Two-byte elements at any address: the aligned words that hold a row, 32 or 33 of them, of which an odd row uses the first from its
+// upper half on.  (The lower half of that word is the element before the row or, before a tensor's first, whatever shares its four
+// bytes: it is fetched and not used.)
+template <int ROWS, typename T> struct Feed<ROWS, 2, T> {
+    const T *from;
+    int64_t row_stride, advance;
+    int cols, first, odd;   // halves before row 0's first element in its word, and whether rows take turns
+    __device__ __forceinline__ Feed(const T *src, int64_t t, int64_t rs, int steps, int cols_, int) {
+        row_stride = rs;
+        advance = steps * rs;
+        cols = min(cols_, kC);
+        from = src + t * rs;
+        first = (int)((uintptr_t)from >> 1) & 1;
+        odd = (int)rs & 1;   // steps is even, so the first row of every fetch lies like the first
+    }
+    __device__ __forceinline__ int shift(int row) const { return first ^ (row & odd); }
+    __device__ __forceinline__ void whole(uint32_t slot) { part(slot, ROWS); }
+    __device__ __forceinline__ int bytes(int word, int before) const { return min(max((cols - (2 * word - before)) * 2, 0), 4); }
+    // word `word` of a row; nothing is read where n is 0
+    __device__ __forceinline__ void copy(uint32_t dst, const T *row, int word, int n) const {
+        cp_async<4>(dst + 4 * word, reinterpret_cast<const char *>((uintptr_t)row & ~(uintptr_t)3) + 4 * word, n);
+    }
+    __device__ __forceinline__ void part(uint32_t slot, int rows) {
         const int lane = threadIdx.x & 31;
-        f -= lane % wide * per;   // across = 64 elements: wide = 32, high = 1
+        const int n[2] = {bytes(lane, first), bytes(lane, first ^ odd)};   // of even rows, of odd ones
+        const T *f = from;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-            for (int k = 0; k < kC / 32; ++k) {
-                const int col = lane + 32 * k;
-                const T v = r < rows && col < cols ? f[r * row_stride + col] : T(0.f);
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(slot + (r * kC + col) * 2), "h"(*reinterpret_cast<const uint16_t *>(&v)) : "memory");
-            }
+        for (int r = 0; r < ROWS; ++r) {
+            copy(slot + r * pitch_of(2) * 2, f, lane, r < rows ? n[r & 1] : 0);
+            f += row_stride;
+        }
+        if (lane < ROWS) copy(slot + lane * pitch_of(2) * 2, from + lane * row_stride, 32, lane < rows ? bytes(32, shift(lane)) : 0);
+        from += advance;
     }
 };
 
@@ -113,6 +132,16 @@ __device__ __forceinline__ float2 load2(const float *p) { return *reinterpret_ca
 __device__ __forceinline__ float2 load2(const __nv_bfloat16 *p) {
     const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+// the same of a row of a slot, which begins `shift` elements into its first word
+template <int PIECE, typename T> __device__ __forceinline__ float2 slot2(const T *p, int shift) {
+    if constexpr (PIECE >= 4) {
+        return load2(p);
+    } else {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(p);
+        const uint32_t u = __funnelshift_r(w[0], w[1], 16 * shift);
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
 }
 __device__ __forceinline__ void store2(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
 __device__ __forceinline__ void store2(__nv_bfloat16 *p, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y); }
@@ -248,7 +277,8 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int STAGES = kStages;
     extern __shared__ __align__(16) unsigned char smem[];
-    using Ring = T[STAGES][2][kRun][kC];
+    constexpr int P = pitch_of(PIECE);
+    using Ring = T[STAGES][2][kRun][P];
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
     if (MAP || span.more) chain_trigger();
     const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, 0);
@@ -301,7 +331,7 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
                 }
         }
     }
-    const T *slot_g = &ring[0][0][0][2 * q.lane], *const slot_end = slot_g + STAGES * 2 * kRun * kC;
+    const T *slot_g = &ring[0][0][0][2 * q.lane], *const slot_end = slot_g + STAGES * 2 * kRun * P;
     T *o = out + q.t0 * p.h_row_stride;
     float *st = states ? states + (int64_t)(q.t0 / kBlock) * p.d_inner : nullptr;
     bool keep = states != nullptr;   // every other run starts at a state to be kept
@@ -312,9 +342,9 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
 #pragma unroll
         for (int s = 0; s < kRun; ++s) {
             float2 rest;
-            gate_step<GATE, FAST>(load2(slot_g + s * kC), load2(slot_g + (kRun + s) * kC), a[s], v[s], rest);
+            gate_step<GATE, FAST>(slot2<PIECE>(slot_g + s * P, feed_g.shift(s)), slot2<PIECE>(slot_g + (kRun + s) * P, feed_x.shift(s)), a[s], v[s], rest);
         }
-        slot_g += 2 * kRun * kC;
+        slot_g += 2 * kRun * P;
         if (slot_g == slot_end) slot_g = &ring[0][0][0][2 * q.lane];
         issue(r + STAGES - 1);
         const int rows = ragged && r == (MAP ? 0 : runs - 1) ? ragged : kRun;
@@ -377,7 +407,8 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int STAGES = MAP ? kStages : kBlockStages, ROWS = MAP ? kRun : kBlock, TENSORS = MAP ? 2 : 3;
     extern __shared__ __align__(16) unsigned char smem[];
-    using Ring = T[STAGES][TENSORS][ROWS][kC];   // g, dh, x
+    constexpr int P = pitch_of(PIECE);
+    using Ring = T[STAGES][TENSORS][ROWS][P];   // g, dh, x
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
     if (MAP || span.more) chain_trigger();
     const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, MAP ? 1 : 0);
@@ -414,7 +445,7 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
     };
 #pragma unroll
     for (int r = 0; r < STAGES - 1; ++r) issue(r);
-    const T *slot = &ring[0][0][0][2 * q.lane], *const slot_end = slot + STAGES * TENSORS * ROWS * kC;
+    const T *slot = &ring[0][0][0][2 * q.lane], *const slot_end = slot + STAGES * TENSORS * ROWS * P;
 
     if constexpr (MAP) {
         float2 E = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);
@@ -425,10 +456,10 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
 #pragma unroll
             for (int s = 0; s < kRun; ++s) {
                 float2 rest, b;
-                v[s] = load2(slot + (ROWS + s) * kC);
-                gate_step<GATE, FAST>(load2(slot + s * kC), v[s], a[s], b, rest);
+                v[s] = slot2<PIECE>(slot + (ROWS + s) * P, feed_d.shift(s));
+                gate_step<GATE, FAST>(slot2<PIECE>(slot + s * P, feed_g.shift(s)), v[s], a[s], b, rest);
             }
-            slot += TENSORS * ROWS * kC;
+            slot += TENSORS * ROWS * P;
             if (slot == slot_end) slot = &ring[0][0][0][2 * q.lane];
             issue(r + STAGES - 1);
             if (ragged && r == runs - 1) {
@@ -485,19 +516,19 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
 #pragma unroll
             for (int s = 0; s < kBlock; ++s) {   // rows behind the end are zeros here: what they give is not used
                 float2 b;
-                gate_step<GATE, FAST>(load2(slot + s * kC), load2(slot + (2 * kBlock + s) * kC), a[s], b, rest[s]);
+                gate_step<GATE, FAST>(slot2<PIECE>(slot + s * P, feed_g.shift(s)), slot2<PIECE>(slot + (2 * kBlock + s) * P, feed_x.shift(s)), a[s], b, rest[s]);
                 before[s] = state;
                 state = fma2(a[s], state, b);
             }
             state = next_state;
             issue(r + STAGES - 1);
             auto gradients = [&](int s, float2 &dxv, float2 &dgv) {
-                const float2 d = add2(load2(slot + (kBlock + s) * kC), e);   // delta
+                const float2 d = add2(slot2<PIECE>(slot + (kBlock + s) * P, feed_d.shift(s)), e);   // delta
                 e = mul2(a[s], d);
                 if constexpr (GATE == HX_GATE_SIGMOID) {
                     dxv = mul2(d, rest[s]);
                     // delta (h - x) a (1 - a), with e = a delta
-                    dgv = mul2(mul2(e, rest[s]), fma2(load2(slot + (2 * kBlock + s) * kC), make_float2(-1.f, -1.f), before[s]));
+                    dgv = mul2(mul2(e, rest[s]), fma2(slot2<PIECE>(slot + (2 * kBlock + s) * P, feed_x.shift(s)), make_float2(-1.f, -1.f), before[s]));
                 } else {
                     dxv = d;
                     dgv = mul2(d, before[s]);
@@ -524,7 +555,7 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
                         og -= p.dg_row_stride;
                     }
             }
-            slot += TENSORS * ROWS * kC;
+            slot += TENSORS * ROWS * P;
             if (slot == slot_end) slot = &ring[0][0][0][2 * q.lane];
         }
         const int64_t end = q.seg == segs - 1 ? span.end : min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)span.end);
@@ -664,13 +695,13 @@ static hx_status launch_all(size_t map_ring, size_t ring, bool backwards, const 
     return HX_OK;
 }
 template <typename T, int GATE, int PIECE> static hx_status launch_fwd(const hx_gated_scan_args &a, const Plan &plan, cudaStream_t st) {
-    constexpr size_t ring = sizeof(T[kStages][2][kRun][kC]);
+    constexpr size_t ring = sizeof(T[kStages][2][kRun][pitch_of(PIECE)]);
     return launch_all<gated_scan_kernel<T, GATE, PIECE, true>, gated_scan_kernel<T, GATE, PIECE, false>>(ring, ring, false, a.h0, a.h_last, a, plan,
                                                                                                          "gated_scan_kernel", st);
 }
 template <typename T, int GATE, int PIECE> static hx_status launch_bwd(const hx_gated_scan_bwd_args &a, const Plan &plan, cudaStream_t st) {
     return launch_all<gated_scan_bwd_kernel<T, GATE, PIECE, true>, gated_scan_bwd_kernel<T, GATE, PIECE, false>>(
-        sizeof(T[kStages][2][kRun][kC]), sizeof(T[kBlockStages][3][kBlock][kC]), true, a.dh_last, a.dh0, a, plan, "gated_scan_bwd_kernel", st);
+        sizeof(T[kStages][2][kRun][pitch_of(PIECE)]), sizeof(T[kBlockStages][3][kBlock][pitch_of(PIECE)]), true, a.dh_last, a.dh0, a, plan, "gated_scan_bwd_kernel", st);
 }
 
 // The plan a call may use: one segment where it brings no workspace.
