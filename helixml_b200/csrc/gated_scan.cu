@@ -215,12 +215,12 @@ struct Part {
     bool live;
 };
 __device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, const int32_t *lengths, const Span &span, int seg_len, int segs,
-                                        int first_seg) {
+                                        int first_seg, int count) {   // segments first_seg .. first_seg + count - 1 of segs
     Part q;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int tiles = (d_inner + kC - 1) / kC;
     const int64_t w = (int64_t)blockIdx.x * kWarps + warp;
-    q.live = w < (int64_t)tiles * batch * segs;
+    q.live = w < (int64_t)tiles * batch * count;
     const int64_t row = q.live ? w / tiles : 0;
     q.d0 = q.live ? (int)(w % tiles) * kC : 0;
     q.b = (int)(row % batch);
@@ -232,7 +232,7 @@ __device__ __forceinline__ Part part_of(int batch, int seq_len, int d_inner, con
     q.len = lengths ? min(max(lengths[q.b], 0), seq_len) : seq_len;
     q.end = min(q.len, span.end);
     q.t0 = (int)min(span.begin + (int64_t)q.seg * seg_len, (int64_t)q.end);
-    q.t1 = (int)min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)q.end);
+    q.t1 = q.seg == segs - 1 ? q.end : (int)min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)q.end);
     return q;
 }
 // maps: [segment][batch][d_inner rounded up to 2] pairs (A, B) of a channel
@@ -281,18 +281,17 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
     using Ring = T[STAGES][2][kRun][P];
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
     if (MAP || span.more) chain_trigger();
-    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, 0);
+    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, segs, 0, MAP ? segs - 1 : segs);
     if (!q.live) return;
     const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
     const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
-    const int runs = (q.t1 - q.t0 + kRun - 1) / kRun;
+    const int ragged = (q.t1 - q.t0) % kRun, runs = (q.t1 - q.t0) / kRun + (ragged > 0);   // rows of the last run, 0: all
     // MAP walks from the last run to the first
     const int64_t first = q.t0 + (int64_t)(MAP ? runs - 1 : 0) * kRun;
     Feed<kRun, PIECE, T> feed_g(g, first, p.g_row_stride, MAP ? -kRun : kRun, q.cols, q.lane);
     Feed<kRun, PIECE, T> feed_x(x, first, p.x_row_stride, MAP ? -kRun : kRun, q.cols, q.lane);
     constexpr uint32_t slot_bytes = sizeof(ring[0]), ring_bytes = sizeof(ring);
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(&ring[0][0][0][0]);
-    const int ragged = (q.t1 - q.t0) % kRun;   // rows of the last run, 0: all
     uint32_t to = 0;                           // slot that is filled next
     auto issue = [&](int r) {                  // the r-th run of the walk
         if (r < runs) {
@@ -316,7 +315,8 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
     T *out = static_cast<T *>(p.h) + q.b * p.h_batch_stride + q.c;
     const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
     float *states = !MAP && p.states ? p.states + q.b * blocks * p.d_inner + q.c : nullptr;
-    const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2, even = p.d_inner % 2 == 0;
+    const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2;
+    const bool even = p.d_inner % 2 == 0 && (uintptr_t)p.states % 8 == 0;   // two states at a time
     if constexpr (!MAP) {
         if (segs > 1) chain_wait();
         if (span.in) h = load_carry(span.in + (int64_t)q.b * p.d_inner + q.c, q.n);
@@ -324,10 +324,21 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
             const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
             const int j = fold(map_at(maps, 0, q.b, q.c, p.batch, p.d_inner), step, q.seg, q.n > 0, h);
             if (j < q.seg)   // h is the state before segment j: walk on from there
-                for (int64_t t = span.begin + (int64_t)j * seg_len; t < q.t0; ++t) {
-                    float2 a, b, rest;
-                    gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), load_some(x + t * p.x_row_stride + 2 * q.lane, q.n), a, b, rest);
-                    h = fma2(a, h, b);
+                for (int64_t t = span.begin + (int64_t)j * seg_len; t < q.t0; t += kRun) {
+                    float2 gv[kRun], xv[kRun];
+#pragma unroll
+                    for (int s = 0; s < kRun; ++s) {
+                        const int n = t + s < q.t0 ? q.n : 0;
+                        gv[s] = load_some(g + (t + s) * p.g_row_stride + 2 * q.lane, n);
+                        xv[s] = load_some(x + (t + s) * p.x_row_stride + 2 * q.lane, n);
+                    }
+#pragma unroll
+                    for (int s = 0; s < kRun; ++s)
+                        if (t + s < q.t0) {
+                            float2 a, b, rest;
+                            gate_step<GATE, FAST>(gv[s], xv[s], a, b, rest);
+                            h = fma2(a, h, b);
+                        }
                 }
         }
     }
@@ -411,12 +422,12 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
     using Ring = T[STAGES][TENSORS][ROWS][P];   // g, dh, x
     Ring &ring = reinterpret_cast<Ring *>(smem)[threadIdx.x >> 5];
     if (MAP || span.more) chain_trigger();
-    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, MAP ? segs - 1 : segs, MAP ? 1 : 0);
+    const Part q = part_of(p.batch, p.seq_len, p.d_inner, p.lengths, span, seg_len, segs, MAP ? 1 : 0, MAP ? segs - 1 : segs);
     if (!q.live) return;
     const T *x = static_cast<const T *>(p.x) + q.b * p.x_batch_stride + q.d0;
     const T *g = static_cast<const T *>(p.g) + q.b * p.g_batch_stride + q.d0;
     const T *dh = static_cast<const T *>(p.dh) + q.b * p.dh_batch_stride + q.d0;
-    const int runs = (q.t1 - q.t0 + ROWS - 1) / ROWS;
+    const int ragged = (q.t1 - q.t0) % ROWS, runs = (q.t1 - q.t0) / ROWS + (ragged > 0);
     const int64_t first = q.t0 + (int64_t)(MAP ? 0 : runs - 1) * ROWS;
     constexpr int way = MAP ? ROWS : -ROWS;
     Feed<ROWS, PIECE, T> feed_g(g, first, p.g_row_stride, way, q.cols, q.lane);
@@ -424,7 +435,6 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
     Feed<ROWS, PIECE, T> feed_x(x, first, p.x_row_stride, way, q.cols, q.lane);
     constexpr uint32_t part_bytes = sizeof(ring[0][0]), slot_bytes = sizeof(ring[0]), ring_bytes = sizeof(ring);
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(&ring[0][0][0][0]);
-    const int ragged = (q.t1 - q.t0) % ROWS;
     uint32_t to = 0;
     auto issue = [&](int r) {
         if (r < runs) {
@@ -481,7 +491,7 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
         if (q.n) *map_at(maps, q.seg - 1, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, E.x, A.y, E.y);
     } else {
         const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
-        const bool even = p.d_inner % 2 == 0;
+        const bool even = p.d_inner % 2 == 0 && (uintptr_t)p.states % 8 == 0;   // two states at a time
         auto state_of = [&](int r) {   // the state before the r-th block of the walk
             if (r >= runs) return make_float2(0.f, 0.f);
             const float *st = p.states + (q.b * blocks + q.t0 / kBlock + (runs - 1 - r)) * p.d_inner + q.c;
@@ -496,11 +506,21 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
             const int folded = fold(map_at(maps, segs - 2, q.b, q.c, p.batch, p.d_inner), -step, count, q.n > 0, e);
             const int j = segs - 1 - folded;
             if (folded < count)   // e is the one behind segment j
-                for (int64_t t = min(span.begin + (int64_t)(j + 1) * seg_len, (int64_t)q.end) - 1; t >= q.t1; --t) {
-                    float2 a, b, rest;
-                    const float2 d = load_some(dh + t * p.dh_row_stride + 2 * q.lane, q.n);
-                    gate_step<GATE, FAST>(load_some(g + t * p.g_row_stride + 2 * q.lane, q.n), d, a, b, rest);
-                    e = mul2(a, add2(e, d));
+                for (int64_t t = min(span.begin + (int64_t)(j + 1) * seg_len, (int64_t)q.end) - 1; t >= q.t1; t -= kRun) {
+                    float2 gv[kRun], dv[kRun];
+#pragma unroll
+                    for (int s = 0; s < kRun; ++s) {
+                        const int n = t - s >= q.t1 ? q.n : 0;
+                        gv[s] = load_some(g + (t - s) * p.g_row_stride + 2 * q.lane, n);
+                        dv[s] = load_some(dh + (t - s) * p.dh_row_stride + 2 * q.lane, n);
+                    }
+#pragma unroll
+                    for (int s = 0; s < kRun; ++s)
+                        if (t - s >= q.t1) {
+                            float2 a, b, rest;
+                            gate_step<GATE, FAST>(gv[s], dv[s], a, b, rest);
+                            e = mul2(a, add2(e, dv[s]));
+                        }
                 }
         }
         const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2;

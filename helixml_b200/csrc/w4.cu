@@ -164,7 +164,7 @@ dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int bloc
 
 static hx_status check_matrix(const char *who, const hx_w4_matrix *m) {
     HX_REQUIRE(m != nullptr, HX_ERR_INVALID_INPUT, "%s: the matrix is NULL", who);
-    HX_REQUIRE(m->rows >= 0 && m->cols >= 0, HX_ERR_INVALID_DIMENSION, "%s: a matrix of %d x %d", who, m->rows, m->cols);
+    HX_REQUIRE(m->rows >= 0 && m->rows <= 0x7fffff00 && m->cols >= 0, HX_ERR_INVALID_DIMENSION, "%s: a matrix of %d x %d", who, m->rows, m->cols);
     HX_REQUIRE(m->group == 32 || m->group == 64 || m->group == 128, HX_ERR_INVALID_DIMENSION, "%s: group %d is not 32, 64 or 128", who,
                m->group);
     HX_REQUIRE(m->cols % m->group == 0, HX_ERR_SHAPE_MISMATCH, "%s: %d columns are not a multiple of the group %d", who, m->cols, m->group);

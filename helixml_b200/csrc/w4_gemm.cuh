@@ -369,13 +369,10 @@ static Plan plan_of(const hx_w4_matrix &m, int outs, int most, size_t staged) {
 template <typename TA, int NT, int RT, int GROUP, int CH, int ROWS>
 static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                            int epilogue, const Plan &p, size_t smem, bool vec, cudaStream_t st) {
-    const int64_t down = ((int64_t)M + 8 * NT - 1) / (8 * NT);
-    HX_REQUIRE(down <= 65535, HX_ERR_INVALID_DIMENSION, "hx_gemm_w4: %d rows", M);
     auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, ROWS>;
     static std::atomic<uint64_t> done{0};
     if (smem > 48 * 1024) HX_CUDA(allow_smem((const void *)kernel, kSmemBytes + 16 * 1024, done));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.grid, (unsigned)down);
     cfg.blockDim = dim3(32 * p.warps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -385,7 +382,14 @@ static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, co
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.share > 1 ? 1 : 0;
-    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue, vec));
+    constexpr int most = 65535 * 8 * NT;   // rows of a launch
+    for (int64_t m0 = 0; m0 < M; m0 += most) {
+        const int rows = (int)std::min<int64_t>(M - m0, most);
+        cfg.gridDim = dim3((unsigned)p.grid, (unsigned)((rows + 8 * NT - 1) / (8 * NT)));
+        HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A) + m0 * lda, lda, m, bias,
+                                   static_cast<void *>(static_cast<char *>(C) + m0 * ldc * (int64_t)dtype_size(c_dtype)), ldc, c_dtype, rows,
+                                   blocks_of(m.cols), epilogue, vec));
+    }
     return check_launch("gemm_w4_kernel");
 }
 template <typename TA, int NT, int RT>

@@ -243,6 +243,24 @@ def test_views(dtype, offset, pad):
     assert (gv[:, :, 2 * D:] == 7).all() and (grads[:offset] == 7).all()
 
 
+@pytest.mark.parametrize("D", [64, 37])
+def test_fp32_operands_off_eight_bytes(D):
+    """Contiguous states, h0 and dh_last that begin one element into a buffer."""
+    x, g, h0, dh, dh_last = inputs(19, 2, 100, D, "bf16", "sigmoid")
+    off = lambda t: torch.cat([torch.zeros(1, device="cuda"), t.flatten()])[1:].view(t.shape)
+    st = ops.gated_scan_states(2, 100, D)
+    flat = torch.full((st.numel() + 2,), 7.0, device="cuda")
+    shifted = flat[1:-1].view(st.shape)
+    want = ops.gated_scan(x, g, h0=h0, states=st)
+    assert torch.equal(ops.gated_scan(x, g, h0=off(h0), states=shifted), want)
+    assert torch.equal(shifted, st) and flat[0] == 7 and flat[-1] == 7
+    for a, b in zip(ops.gated_scan_bwd(dh, x, g, shifted, dh_last=off(dh_last)), ops.gated_scan_bwd(dh, x, g, st, dh_last=dh_last)):
+        assert torch.equal(a, b)
+    h, other = off(h0), off(torch.zeros_like(h0))
+    y = ops.gated_scan_step(x[:, 0], g[:, 0], h, h_out=other)
+    assert torch.equal(y, ops.gated_scan_step(x[:, 0], g[:, 0], h0)) and torch.equal(other, h0)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_time_major_and_broadcast_views(dtype):
     x, g, h0, dh, dh_last = inputs(10, 4, 100, 36, dtype, "decay")

@@ -113,7 +113,7 @@ def test_w4_argument_errors():
     }
     for name, f in calls.items():
         assert f(None) == 10, name
-        assert f(w4(rows=-1)) == 2 and f(w4(cols=-64)) == 2 and f(w4(group=48)) == 2, name
+        assert f(w4(rows=2 ** 31 - 1)) == 2 and f(w4(rows=-1)) == 2 and f(w4(cols=-64)) == 2 and f(w4(group=48)) == 2, name
         assert f(w4(cols=96)) == 1 and f(w4(scale_dtype=L.HX_U8)) == 4, name
         assert f(w4(codes=None)) == 10 and f(w4(scale=None)) == 10 and f(w4(codes=264)) == 10, name
         assert f(w4(), W=None) == 10, name

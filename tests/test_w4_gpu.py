@@ -225,6 +225,20 @@ def test_product_on_views(adt, offset, pad):
     assert torch.equal(ops.gemm_w4(one.expand(5, K), m), ops.gemm_w4(one.expand(5, K).contiguous(), m))   # one row five times
 
 
+def test_product_of_more_rows_than_a_grid_holds():
+    codes, scale, _ = make(14, 5, 32, 32, torch.float32, False)
+    m = ops.w4_pack(codes.cuda(), scale.cuda())
+    M = 65535 * 64 + 70
+    a = torch.zeros(M, 32, device="cuda", dtype=torch.bfloat16)
+    for r in (0, 63, 65535 * 64 - 1, 65535 * 64, M - 1):
+        a[r] = torch.randn(32, generator=torch.Generator().manual_seed(r)).bfloat16()
+    c = ops.gemm_w4(a, m, out_dtype=torch.float32)
+    w = values(codes, scale, None, 32)
+    rows = torch.tensor([0, 63, 64, 65535 * 64 - 1, 65535 * 64, M - 2, M - 1])
+    check_product(c[rows.cuda()], a[rows.cuda()], w, None)
+    assert (c != 0).any(1).sum().item() == 5
+
+
 def test_product_keeps_fp32_operands():
     """fp32 rows whose bf16 part cancels: what is left is in the bits below."""
     K = 256
