@@ -69,8 +69,6 @@ hx_status gemm_bf16(const void *A, int64_t lda, const hx_w4_matrix &m, const flo
                     cudaStream_t st);
 hx_status gemm_f32(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                    cudaStream_t st);
-hx_status gemm_f32_rows(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
-                        cudaStream_t st);
 
 }  // namespace w4
 }  // namespace hx

@@ -423,9 +423,236 @@ static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, 
 #undef HX_W4_AS
 }
 
-// Whether tiles of `outs` outputs still fill the SMs.
-static bool fills(const hx_w4_matrix &m, int outs) { return (int64_t)m.rows * 3 >= (int64_t)outs * sm_count() * 2; }
-#define HX_W4_ROWS(TA, NT, RT) return launch_gemm<TA, NT, RT>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st)
+// ---------------------------------------------------------------- more than eight rows
+// The same products where a piece of A is read for more than one tile of rows: here it costs as much as the codes, so a CTA's warps take
+// different outputs, 16 each, walk the columns together and share the block of A they are at, staged in shared memory (fp32 rows
+// already cut into their three parts, once a CTA).  One barrier a block; codes, A and scales of the next blocks are under way.  What
+// bounds it is the warp-level tensor pipe and the instructions that feed it.  Where tiles of 128 outputs are few, a cluster of CTAs
+// shares the columns; each adds up a part of the outputs out of the others' shared memory, in the order of the ranks.
+constexpr int kRowWarps = 8, kRowOuts = 16 * kRowWarps;
+constexpr int kRowPitch = kBlockCols * 2 + 64;   // bytes from one staged row to the next: rows g and g + 1 fall on different banks
+template <typename TA> constexpr int row_stages() { return sizeof(TA) == 2 ? 3 : 2; }   // of A
+
+template <typename TA, int NT, int GROUP>
+__global__ void __launch_bounds__(32 * kRowWarps, NT * (int)sizeof(TA) <= 16 ? 2 : 1)
+gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
+                    int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
+    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kRows = 8 * NT, kSlots = 3, kStages = row_stages<TA>();
+    constexpr int kStage = kParts * kRows * kRowPitch, kThreads = 32 * kRowWarps;
+    extern __shared__ __align__(16) unsigned char shared[];   // [kStages][kParts][kRows][kRowPitch], then the codes' slots
+    const auto cluster = cooperative_groups::this_cluster();
+    const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int m0 = blockIdx.y * kRows, here = min(M - m0, kRows), tile0 = blockIdx.x / share * kRowOuts;
+    const int k0 = (int)((int64_t)blocks * rank / share), k1 = (int)((int64_t)blocks * (rank + 1) / share);   // this CTA's blocks
+    const int groups = m.cols / GROUP;
+    const int scale_shift = m.scale_dtype == HX_BF16 ? 16 : 0;
+    uint4 *slots = reinterpret_cast<uint4 *>(shared + kStages * kStage) + warp * kSlots * 64 + lane;
+
+    const uint8_t *codes[2];
+    int64_t at[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int n = min(tile0 + warp * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
+        codes[half] = m.codes + ((int64_t)n * blocks + k0) * kBlockBytes + c * 16;
+        at[half] = (int64_t)n * groups + (int64_t)(k0 + c) * kGroups;
+    }
+    auto fetch_codes = [&](int k) {
+        if (k < k1)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) cp_async16(slots + ((k - k0) % kSlots * 2 + half) * 32, codes[half] + (int64_t)(k - k0) * kBlockBytes);
+    };
+    // scales and zero points of four blocks at a time, lane c those of block c
+    uint32_t scale[2][2][kGroups], zero[2][2][kGroups];
+    auto fetch_scales = [&](int k, uint32_t (&s)[2][kGroups], uint32_t (&z)[2][kGroups]) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) {
+                const int64_t i = at[half] + (int64_t)(k - k0) * kGroups + q;
+                s[half][q] = 0;
+                z[half][q] = 8;
+                if (k + c < k1 && (k + c) * kGroups + q < groups) {
+                    if (scale_shift) s[half][q] = static_cast<const uint16_t *>(m.scale)[i];
+                    else s[half][q] = static_cast<const uint32_t *>(m.scale)[i];
+                    if (m.zero) z[half][q] = m.zero[i];
+                }
+            }
+    };
+    // A: bf16 goes straight into its stage; fp32 waits in registers for a block's time and is cut on its way
+    constexpr int per = 16 / (int)sizeof(TA), across = kBlockCols / per, kPieces = kRows * across / kThreads;
+    float4 held[sizeof(TA) == 4 ? kPieces : 1];
+    auto fetch_rows = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int piece = threadIdx.x + i * kThreads, row = piece / across, col = piece % across * per;
+            const bool in = k < k1 && row < here && k * kBlockCols + col < m.cols;   // cols is a multiple of 32
+            const TA *from = A + (int64_t)(m0 + row) * lda + (int64_t)k * kBlockCols + col;
+            if constexpr (sizeof(TA) == 2) {
+                TA *to = reinterpret_cast<TA *>(shared + (k - k0) % kStages * kStage + row * kRowPitch) + col;
+                if (in && vec) cp_async16(to, from);
+                else if (in)
+#pragma unroll
+                    for (int e = 0; e < per; ++e) to[e] = from[e];
+            } else {
+                if (in && vec) held[i] = *reinterpret_cast<const float4 *>(from);
+                else if (in) held[i] = make_float4(from[0], from[1], from[2], from[3]);
+            }
+        }
+    };
+    auto cut_rows = [&](int k) {   // what is held goes into block k's stage
+        if constexpr (sizeof(TA) == 4) {
+            if (k < k1)
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int piece = threadIdx.x + i * kThreads, row = piece / across, col = piece % across * per;
+                    float v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+                    unsigned char *to = shared + (k - k0) % kStages * kStage + row * kRowPitch + col * 2;
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
+                        uint32_t u[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(Operand<float>::take(v[e]));
+                        *reinterpret_cast<uint2 *>(to + part * kRows * kRowPitch) = make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
+                    }
+                }
+        }
+    };
+
+    fetch_scales(k0, scale[0], zero[0]);
+#pragma unroll
+    for (int k = 0; k < kSlots - 1; ++k) {
+        fetch_codes(k0 + k);
+        if constexpr (sizeof(TA) == 2) fetch_rows(k0 + k);
+        cp_commit();
+    }
+    if constexpr (sizeof(TA) == 4) {
+        fetch_rows(k0);
+        cut_rows(k0);
+        fetch_rows(k0 + 1);
+    }
+    float total[NT][4] = {};
+    const unsigned char *mine = shared + g * kRowPitch + c * 16;
+    for (int k = k0; k < k1; ++k) {
+        const int u = (k - k0) & 3;
+        if (u == 0) fetch_scales(k + 4, scale[1], zero[1]);
+        cp_wait<kSlots - 2>();
+        __syncthreads();   // block k is staged; block k - 1 is done with
+        fetch_codes(k + kSlots - 1);
+        if constexpr (sizeof(TA) == 2) fetch_rows(k + kSlots - 1);
+        cp_commit();
+        cut_rows(k + 1);
+        if constexpr (sizeof(TA) == 4) fetch_rows(k + 2);
+        const uint4 w[2] = {slots[((k - k0) % kSlots * 2) * 32], slots[((k - k0) % kSlots * 2 + 1) * 32]};
+        const unsigned char *stage = mine + (k - k0) % kStages * kStage;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            if (GROUP < kBlockCols && k * kGroups + q >= groups) break;   // the filled-up end of a row
+            float sum[NT][4], by[2];
+            uint32_t offset[2];   // -(zero point) / 64, twice
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                by[half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][half][q], u, 4) << scale_shift);
+                offset[half] = 0xbe00be00u;
+                if (m.zero) offset[half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
+            }
+#pragma unroll
+            for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
+                uint32_t a[2][4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    eight_weights(j == 0 ? w[half].x : j == 1 ? w[half].y : j == 2 ? w[half].z : w[half].w, offset[half], a[half]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        const uint4 b = *reinterpret_cast<const uint4 *>(stage + (part * kRows + t * 8) * kRowPitch + j * 64);
+                        if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                        else mma_bf16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                        mma_bf16(sum[t], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) total[t][i] = fmaf(by[i >> 1], sum[t][i], total[t][i]);
+        }
+        if (u == 3) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) scale[0][half][q] = scale[1][half][q], zero[0][half][q] = zero[1][half][q];
+        }
+    }
+    // totals 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
+    if (share == 1) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = tile0 + warp * 16 + (i >> 1) * 8 + g, row = t * 8 + 2 * c + (i & 1);
+                if (n < m.rows && row < here) finish(kSumScale * total[t][i], n, m0 + row, bias, C, ldc, c_dtype, epilogue);
+            }
+        return;
+    }
+    float *sums = reinterpret_cast<float *>(shared);   // [kRows][kRowOuts]
+    cp_wait<0>();
+    __syncthreads();   // the stages have been read
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[(t * 8 + 2 * c + (i & 1)) * kRowOuts + warp * 16 + (i >> 1) * 8 + g] = total[t][i];
+    cluster.sync();
+    for (int i = rank * kThreads + threadIdx.x; i < here * kRowOuts; i += share * kThreads) {
+        const int n = tile0 + i % kRowOuts, row = i / kRowOuts;
+        if (n >= m.rows) continue;
+        float v = 0.f;
+        for (int r = 0; r < share; ++r) v += *cluster.map_shared_rank(sums + i, r);
+        finish(kSumScale * v, n, m0 + row, bias, C, ldc, c_dtype, epilogue);
+    }
+    cluster.sync();   // the others' shared memory stays until it has been read
+}
+
+template <typename TA, int NT, int GROUP>
+static hx_status launch_rows_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                                int epilogue, cudaStream_t st) {
+    constexpr int kRows = 8 * NT, per_sm = NT * (int)sizeof(TA) <= 16 ? 2 : 1;
+    constexpr size_t staged = (size_t)row_stages<TA>() * Operand<TA>::kParts * kRows * kRowPitch, smem = staged + kRowWarps * 3 * 1024;
+    static_assert(staged + kRowWarps * 3 * 1024 >= (size_t)kRows * kRowOuts * sizeof(float), "the sums of a cluster's CTA fit");
+    auto kernel = gemm_w4_rows_kernel<TA, NT, GROUP>;
+    static std::atomic<uint64_t> done{0};
+    HX_CUDA(allow_smem((const void *)kernel, smem, done));
+    const int blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + kRowOuts - 1) / kRowOuts);
+    const int64_t down = ((int64_t)M + kRows - 1) / kRows;
+    const int share = (int)std::max<int64_t>(1, std::min<int64_t>({per_sm * sm_count() / (tiles * down), blocks / 2, 8}));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(32 * kRowWarps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)share;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = share > 1 ? 1 : 0;
+    const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
+    constexpr int most = 65535 * kRows;   // rows of a launch
+    for (int64_t m0 = 0; m0 < M; m0 += most) {
+        const int rows = (int)std::min<int64_t>(M - m0, most);
+        cfg.gridDim = dim3((unsigned)(tiles * share), (unsigned)((rows + kRows - 1) / kRows));
+        HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A) + m0 * lda, lda, m, bias,
+                                   static_cast<void *>(static_cast<char *>(C) + m0 * ldc * (int64_t)dtype_size(c_dtype)), ldc, c_dtype, rows, blocks,
+                                   epilogue, vec));
+    }
+    return check_launch("gemm_w4_rows_kernel");
+}
+template <typename TA, int NT>
+static hx_status launch_rows(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                             int epilogue, cudaStream_t st) {
+    if (m.group == 32) return launch_rows_as<TA, NT, 32>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (m.group == 64) return launch_rows_as<TA, NT, 64>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_rows_as<TA, NT, 128>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+}
 
 }  // namespace w4
 }  // namespace hx

@@ -1,5 +1,4 @@
-// hx_gemm_w4 with up to 16 fp32 rows of A.  Cutting a piece of A into its parts costs three times what a block of codes
-// does, so it is done once for three tiles of outputs where those still fill the SMs.
+// hx_gemm_w4 with fp32 rows of A.
 #include "w4_gemm.cuh"
 
 namespace hx {
@@ -7,10 +6,11 @@ namespace w4 {
 
 hx_status gemm_f32(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                    cudaStream_t st) {
-    if (M <= 8) HX_W4_ROWS(float, 1, 1);
-    if (M > 16) return gemm_f32_rows(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (fills(m, 48)) HX_W4_ROWS(float, 2, 3);
-    HX_W4_ROWS(float, 2, 1);
+    if (M <= 8) return launch_gemm<float, 1, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 16) return launch_rows<float, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 24) return launch_rows<float, 3>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    if (M <= 32) return launch_rows<float, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_rows<float, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
 }
 
 }  // namespace w4
