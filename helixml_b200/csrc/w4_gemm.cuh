@@ -449,18 +449,21 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
     const int scale_shift = m.scale_dtype == HX_BF16 ? 16 : 0;
     uint4 *slots = reinterpret_cast<uint4 *>(shared + kStages * kStage) + warp * kSlots * 64 + lane;
 
-    const uint8_t *codes[2];
-    int64_t at[2];
+    const uint8_t *codes[2];   // of the next block that is asked for
+    int64_t at[2];             // of the next four blocks' scales
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int n = min(tile0 + warp * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
         codes[half] = m.codes + ((int64_t)n * blocks + k0) * kBlockBytes + c * 16;
         at[half] = (int64_t)n * groups + (int64_t)(k0 + c) * kGroups;
     }
-    auto fetch_codes = [&](int k) {
+    auto fetch_codes = [&](int k, int slot) {
         if (k < k1)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) cp_async16(slots + ((k - k0) % kSlots * 2 + half) * 32, codes[half] + (int64_t)(k - k0) * kBlockBytes);
+            for (int half = 0; half < 2; ++half) {
+                cp_async16(slots + (slot * 2 + half) * 32, codes[half]);
+                codes[half] += kBlockBytes;
+            }
     };
     // scales and zero points of four blocks at a time, lane c those of block c
     uint32_t scale[2][2][kGroups], zero[2][2][kGroups];
@@ -469,7 +472,7 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
         for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
-                const int64_t i = at[half] + (int64_t)(k - k0) * kGroups + q;
+                const int64_t i = at[half] + q;
                 s[half][q] = 0;
                 z[half][q] = 8;
                 if (k + c < k1 && (k + c) * kGroups + q < groups) {
@@ -478,73 +481,85 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
                     if (m.zero) z[half][q] = m.zero[i];
                 }
             }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) at[half] += 4 * kGroups;
     };
     // A: bf16 goes straight into its stage; fp32 waits in registers for a block's time and is cut on its way
-    constexpr int per = 16 / (int)sizeof(TA), across = kBlockCols / per, kPieces = kRows * across / kThreads;
+    constexpr int per = 16 / (int)sizeof(TA), across = kBlockCols / per, kPieces = kRows * across / kThreads, down = kThreads / across;
+    const int row0 = threadIdx.x / across, col = threadIdx.x % across * per;   // a thread's pieces: this column of rows row0, row0 + down, ...
+    const TA *from = A + (int64_t)(m0 + row0) * lda + (int64_t)k0 * kBlockCols + col;
+    unsigned char *const to = shared + row0 * kRowPitch + col * 2;
     float4 held[sizeof(TA) == 4 ? kPieces : 1];
-    auto fetch_rows = [&](int k) {
+    auto fetch_rows = [&](int k, int stage) {
+        const int rows = k < k1 && k * kBlockCols + col < m.cols ? here - row0 : 0;   // cols is a multiple of 32
+        if (vec) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int piece = threadIdx.x + i * kThreads, row = piece / across, col = piece % across * per;
-            const bool in = k < k1 && row < here && k * kBlockCols + col < m.cols;   // cols is a multiple of 32
-            const TA *from = A + (int64_t)(m0 + row) * lda + (int64_t)k * kBlockCols + col;
-            if constexpr (sizeof(TA) == 2) {
-                TA *to = reinterpret_cast<TA *>(shared + (k - k0) % kStages * kStage + row * kRowPitch) + col;
-                if (in && vec) cp_async16(to, from);
-                else if (in)
+            for (int i = 0; i < kPieces; ++i)
+                if (i * down < rows) {
+                    if constexpr (sizeof(TA) == 2) cp_async16(to + stage * kStage + i * down * kRowPitch, from + i * down * lda);
+                    else held[i] = *reinterpret_cast<const float4 *>(from + i * down * lda);
+                }
+        } else {
 #pragma unroll
-                    for (int e = 0; e < per; ++e) to[e] = from[e];
-            } else {
-                if (in && vec) held[i] = *reinterpret_cast<const float4 *>(from);
-                else if (in) held[i] = make_float4(from[0], from[1], from[2], from[3]);
-            }
-        }
-    };
-    auto cut_rows = [&](int k) {   // what is held goes into block k's stage
-        if constexpr (sizeof(TA) == 4) {
-            if (k < k1)
+            for (int i = 0; i < kPieces; ++i)
+                if (i * down < rows) {
+                    const TA *p = from + i * down * lda;
+                    if constexpr (sizeof(TA) == 2) {
+                        TA *t = reinterpret_cast<TA *>(to + stage * kStage + i * down * kRowPitch);
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int piece = threadIdx.x + i * kThreads, row = piece / across, col = piece % across * per;
-                    float v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
-                    unsigned char *to = shared + (k - k0) % kStages * kStage + row * kRowPitch + col * 2;
-#pragma unroll
-                    for (int part = 0; part < 3; ++part) {
-                        uint32_t u[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(Operand<float>::take(v[e]));
-                        *reinterpret_cast<uint2 *>(to + part * kRows * kRowPitch) = make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
+                        for (int e = 0; e < per; ++e) t[e] = p[e];
+                    } else {
+                        held[i] = make_float4(p[0], p[1], p[2], p[3]);
                     }
                 }
+        }
+        from += kBlockCols;
+    };
+    auto cut_rows = [&](int stage) {   // what is held goes into its stage
+        if constexpr (sizeof(TA) == 4) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                float v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(Operand<float>::take(v[e]));
+                    *reinterpret_cast<uint2 *>(to + stage * kStage + (part * kRows + i * down) * kRowPitch) =
+                        make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
+                }
+            }
         }
     };
 
     fetch_scales(k0, scale[0], zero[0]);
 #pragma unroll
     for (int k = 0; k < kSlots - 1; ++k) {
-        fetch_codes(k0 + k);
-        if constexpr (sizeof(TA) == 2) fetch_rows(k0 + k);
+        fetch_codes(k0 + k, k);
+        if constexpr (sizeof(TA) == 2) fetch_rows(k0 + k, k);
         cp_commit();
     }
     if constexpr (sizeof(TA) == 4) {
-        fetch_rows(k0);
-        cut_rows(k0);
-        fetch_rows(k0 + 1);
+        fetch_rows(k0, 0);
+        cut_rows(0);
+        fetch_rows(k0 + 1, 0);
     }
     float total[NT][4] = {};
-    const unsigned char *mine = shared + g * kRowPitch + c * 16;
+    int slot = 0, u = 0;   // of the codes (bf16: and of A), and the block's place among four
     for (int k = k0; k < k1; ++k) {
-        const int u = (k - k0) & 3;
         if (u == 0) fetch_scales(k + 4, scale[1], zero[1]);
         cp_wait<kSlots - 2>();
         __syncthreads();   // block k is staged; block k - 1 is done with
-        fetch_codes(k + kSlots - 1);
-        if constexpr (sizeof(TA) == 2) fetch_rows(k + kSlots - 1);
+        const int next = slot == 0 ? kSlots - 1 : slot - 1;   // what block k - 1 had
+        fetch_codes(k + kSlots - 1, next);
+        if constexpr (sizeof(TA) == 2) fetch_rows(k + kSlots - 1, next);
         cp_commit();
-        cut_rows(k + 1);
-        if constexpr (sizeof(TA) == 4) fetch_rows(k + 2);
-        const uint4 w[2] = {slots[((k - k0) % kSlots * 2) * 32], slots[((k - k0) % kSlots * 2 + 1) * 32]};
-        const unsigned char *stage = mine + (k - k0) % kStages * kStage;
+        if constexpr (sizeof(TA) == 4) {
+            cut_rows((k + 1 - k0) & 1);
+            fetch_rows(k + 2, 0);
+        }
+        const uint4 w[2] = {slots[(slot * 2) * 32], slots[(slot * 2 + 1) * 32]};
+        const unsigned char *stage = shared + (sizeof(TA) == 2 ? slot : (k - k0) & 1) * kStage + g * kRowPitch + c * 16;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
             if (GROUP < kBlockCols && k * kGroups + q >= groups) break;   // the filled-up end of a row
@@ -577,7 +592,9 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) total[t][i] = fmaf(by[i >> 1], sum[t][i], total[t][i]);
         }
-        if (u == 3) {
+        slot = slot == kSlots - 1 ? 0 : slot + 1;
+        u = (u + 1) & 3;
+        if (u == 0) {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -624,16 +641,33 @@ static hx_status launch_rows_as(const void *A, int64_t lda, const hx_w4_matrix &
     HX_CUDA(allow_smem((const void *)kernel, smem, done));
     const int blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + kRowOuts - 1) / kRowOuts);
     const int64_t down = ((int64_t)M + kRows - 1) / kRows;
-    const int share = (int)std::max<int64_t>(1, std::min<int64_t>({per_sm * sm_count() / (tiles * down), blocks / 2, 8}));
+    int share = (int)std::max<int64_t>(1, std::min<int64_t>({per_sm * sm_count() / (tiles * down), blocks / 2, 8}));
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(32 * kRowWarps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)share;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
+    // Clusters that are not all resident at once take twice the time: how many fit is asked for once a kernel, size and device.
+    static std::atomic<int> resident[64][9];
+    int dev = 0;
+    HX_CUDA(cudaGetDevice(&dev));
+    for (; share > 1; --share) {
+        std::atomic<int> *known = dev < 64 ? &resident[dev][share] : nullptr;
+        int fit = known ? known->load(std::memory_order_relaxed) : 0;
+        if (fit == 0) {
+            attr.val.clusterDim.x = (unsigned)share;
+            cfg.numAttrs = 1;
+            cfg.gridDim = dim3((unsigned)share);
+            HX_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+            fit = std::max(fit, 1);
+            if (known) known->store(fit, std::memory_order_relaxed);
+        }
+        if (tiles * down <= fit) break;
+    }
+    attr.val.clusterDim.x = (unsigned)share;
     cfg.numAttrs = share > 1 ? 1 : 0;
     const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
     constexpr int most = 65535 * kRows;   // rows of a launch
