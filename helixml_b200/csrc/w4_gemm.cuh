@@ -19,14 +19,6 @@ namespace w4 {
 // the group size, one 16-byte load brings a lane's share of 128 columns, and the matching piece of A is 8 consecutive elements.
 // Products are exact in fp32, sums fp32; a group's sum is scaled in fp32 and added to the total.  fp32 rows of A are cut into three
 // bf16 parts of 8 bits that add up to them exactly, each with its own MMA.
-//
-// A CTA works through tiles of 16 RT outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
-// block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  Codes come by cp.async
-// into the lane's own slots and A waits in shared memory (STAGED), so that no load in the loop but the next scales is waited for by
-// scoreboard: loads that miss and loads that hit would share one.  The four lanes of a row need the same scales, so lane c loads
-// those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are added in the order of the warps.
-// Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of
-// their shared memory.
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -62,45 +54,14 @@ __device__ __forceinline__ void eight_weights(uint32_t word, uint32_t minus_zero
 }
 constexpr float kSumScale = 64.f;   // what the sums have to be multiplied by in the end
 
-constexpr int max_warps(int NT) { return NT == 1 ? 16 : 8; }   // of a CTA, by its registers
-
-// Eight consecutive elements of a row of A as MMA operands: one part (bf16) or three that add up to them (fp32).
-template <typename TA> struct Operand;
-template <> struct Operand<__nv_bfloat16> {
-    static constexpr int kParts = 1;
-    uint32_t r[1][4];
-    template <bool VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
-        if constexpr (VEC) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p);
-            r[0][0] = v.x, r[0][1] = v.y, r[0][2] = v.z, r[0][3] = v.w;
-        } else {
-            const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[0][i] = (uint32_t)u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
-        }
-    }
-};
-template <> struct Operand<float> {
-    static constexpr int kParts = 3;
-    uint32_t r[3][4];
-    // v = high 8 bits + rest; the rest is exact, and zero for an infinity
-    static __device__ __forceinline__ float take(float &v) {
-        const float high = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-        v = v == high ? 0.f : v - high;
-        return high;
-    }
-    template <bool VEC> __device__ __forceinline__ void load(const float *p) {
-        float v[8];
-        load8(p, VEC, v);
-#pragma unroll
-        for (int part = 0; part < 3; ++part)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a = __float_as_uint(take(v[2 * i])), b = __float_as_uint(take(v[2 * i + 1]));
-                r[part][i] = __byte_perm(a, b, 0x7632);
-            }
-    }
-};
+// fp32 rows of A go into the MMA as three bf16 parts that add up to them.  v = high 8 bits + rest; the rest is exact, and zero for an
+// infinity.
+template <typename TA> constexpr int kPartsOf = sizeof(TA) == 2 ? 1 : 3;
+__device__ __forceinline__ float take_part(float &v) {
+    const float high = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    v = v == high ? 0.f : v - high;
+    return high;
+}
 
 __device__ __forceinline__ void finish(float v, int n, int row, const float *bias, void *C, int64_t ldc, int c_dtype, int epilogue) {
     if (bias) v += bias[n];
@@ -110,106 +71,93 @@ __device__ __forceinline__ void finish(float v, int n, int row, const float *bia
     else static_cast<float *>(C)[row * ldc + n] = v;
 }
 
-// Where a warp's partial sum of output n of the tile and row `row` of A lies: [RT][NT][lane][i].
-template <int NT> __device__ __forceinline__ int place(int n, int row) {
-    return (((n >> 4) * NT + (row >> 3)) * 32 + (n & 7) * 4 + ((row & 7) >> 1)) * 4 + ((n >> 3) & 1) * 2 + (row & 1);
-}
+// ---------------------------------------------------------------- up to eight bf16 rows
+// A CTA works through tiles of 16 outputs.  A warp takes CH consecutive blocks of 128 columns at a time (a chunk); as soon as a
+// block's codes have been used, the same block of the next chunk, of the next tile if need be, is asked for.  Codes come by cp.async
+// into the lane's own slots and A waits in shared memory, so that no load in the loop but the next scales is waited for by
+// scoreboard: loads that miss and loads that hit would share one.  The four lanes of a row need the same scales, so lane c loads
+// those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are added in the order of the warps.
+// Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of
+// their shared memory.  16384 x 4096, groups of 128: one row 13.3 us (40 % of HBM's rate; the loads alone take 8.7, the rest is
+// instructions), eight rows 16.7.
+constexpr int kMostWarps = 16;   // of a CTA, by its registers
+
+// Where a warp's partial sum of output n of the tile and row `row` of A lies: [lane][i].
+__device__ __forceinline__ int place(int n, int row) { return ((n & 7) * 4 + (row >> 1)) * 4 + (n >> 3) * 2 + (row & 1); }
 
 // Bytes from one staged row of A to the next: rows g and g + 1 fall on different banks.
-template <typename TA> __host__ __device__ constexpr size_t staged_pitch(int cols) {
-    return ((size_t)cols * sizeof(TA) + 127) / 128 * 128 + (sizeof(TA) == 2 ? 64 : 16);
-}
+__host__ __device__ constexpr size_t staged_pitch(int cols) { return ((size_t)cols * 2 + 127) / 128 * 128 + 64; }
 
-enum Rows { kStaged, kDirect, kDirectAny };   // A from shared memory; from global memory in 16-byte loads; at any alignment
-
-// NT tiles of 8 rows of A, RT of 16 outputs, CH blocks of a chunk.
-template <typename TA, int NT, int RT, int GROUP, int CH, int ROWS>
-__global__ void __launch_bounds__(32 * max_warps(NT), 1)
-gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
-               int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
-    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kSums = RT * NT * 128, kOuts = 16 * RT;
+template <int GROUP, int CH>
+__global__ void __launch_bounds__(32 * kMostWarps, 1)
+gemm_w4_kernel(const __nv_bfloat16 *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias,
+               void *__restrict__ C, int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
+    constexpr int kGroups = kBlockCols / GROUP, kSums = 128, kOuts = 16;
     extern __shared__ __align__(16) float partial[];   // [2][warps][kSums], then the codes' slots, then A
     const auto cluster = cooperative_groups::this_cluster();
     const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();   // CTAs of a tile
     const int warps = blockDim.x / 32, threads = blockDim.x;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int m0 = blockIdx.y * 8 * NT, here = min(M - m0, 8 * NT);                 // rows of A
     const int64_t row_bytes = (int64_t)blocks * kBlockBytes;
     const int groups = m.cols / GROUP, tiles = (m.rows + kOuts - 1) / kOuts, stride = gridDim.x / share;
     const int first = (rank * warps + warp) * CH, apart = share * warps * CH;   // first block of this warp's chunks
     const int chunks = (blocks + apart - 1) / apart;                            // of a tile, the last one not for all warps
     const bool scale_bf16 = m.scale_dtype == HX_BF16;
     const int scale_shift = scale_bf16 ? 16 : 0;
-    uint4 *slots = reinterpret_cast<uint4 *>(partial + 2 * warps * kSums) + warp * CH * RT * 64 + lane;
+    uint4 *slots = reinterpret_cast<uint4 *>(partial + 2 * warps * kSums) + warp * CH * 64 + lane;
 
-    if constexpr (ROWS == kStaged) {
-        unsigned char *staged = reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * RT * 1024;
-        const size_t pitch = staged_pitch<TA>(m.cols);
-        constexpr int per = 16 / (int)sizeof(TA);
-        const int pieces = m.cols / per;
-        for (int i = threadIdx.x; i < here * pieces; i += threads) {
-            const int row = i / pieces, k = i % pieces * per;
-            TA *to = reinterpret_cast<TA *>(staged + row * pitch) + k;
-            const TA *from = A + (int64_t)(m0 + row) * lda + k;
-            if (vec) {
-                cp_async16(to, from);
-            } else {
+    unsigned char *staged = reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * 1024;
+    const size_t pitch = staged_pitch(m.cols);
+    const int pieces = m.cols / 8;
+    for (int i = threadIdx.x; i < M * pieces; i += threads) {
+        const int row = i / pieces, k = i % pieces * 8;
+        __nv_bfloat16 *to = reinterpret_cast<__nv_bfloat16 *>(staged + row * pitch) + k;
+        const __nv_bfloat16 *from = A + row * lda + k;
+        if (vec) {
+            cp_async16(to, from);
+        } else {
 #pragma unroll
-                for (int e = 0; e < per; ++e) to[e] = from[e];
-            }
+            for (int e = 0; e < 8; ++e) to[e] = from[e];
         }
-        cp_commit();
     }
-    const TA *rows[NT];   // this lane's rows of A; past the last one the last, whose sums are then not stored
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int row = min(t * 8 + g, here - 1);
-        if constexpr (ROWS == kStaged)
-            rows[t] = reinterpret_cast<const TA *>(reinterpret_cast<unsigned char *>(partial + 2 * warps * kSums) + warps * CH * RT * 1024 +
-                                                   row * staged_pitch<TA>(m.cols)) + 8 * c;
-        else rows[t] = A + (int64_t)(m0 + row) * lda + 8 * c;
-    }
+    cp_commit();
+    // this lane's row of A; past the last one the last, whose sums are then not stored
+    const unsigned char *mine_a = staged + min(g, M - 1) * pitch + c * 16;
 
     // the chunk that is asked for: its tile, its number there, where its rows of codes and scales are
     int ahead_tile = blockIdx.x / share, ahead = 0;
-    const uint8_t *codes[RT][2];
-    int64_t at[RT][2];
+    const uint8_t *codes[2];
+    int64_t at[2];
     auto rows_of = [&](int tile) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int n = min(tile * kOuts + r * 16 + half * 8 + g, m.rows - 1);   // rows past the last read the last
-                codes[r][half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
-                at[r][half] = (int64_t)n * groups + (first + c) * kGroups;
-            }
+        for (int half = 0; half < 2; ++half) {
+            const int n = min(tile * kOuts + half * 8 + g, m.rows - 1);   // rows past the last read the last
+            codes[half] = m.codes + n * row_bytes + first * kBlockBytes + c * 16;
+            at[half] = (int64_t)n * groups + (first + c) * kGroups;
+        }
     };
     auto fetch_codes = [&](int u) {
         if (ahead_tile < tiles && first + ahead * apart + u < blocks)
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) cp_async16(slots + ((u * RT + r) * 2 + half) * 32, codes[r][half] + u * kBlockBytes);
+            for (int half = 0; half < 2; ++half) cp_async16(slots + (u * 2 + half) * 32, codes[half] + u * kBlockBytes);
         cp_commit();
     };
     // Scales and zero points under way stay as they are loaded: any arithmetic on them would wait for them.
-    uint32_t scale[2][RT][2][kGroups], zero[2][RT][2][kGroups];   // of block c of this chunk and of the next
-    auto fetch_scales = [&](uint32_t (&s)[RT][2][kGroups], uint32_t (&z)[RT][2][kGroups]) {
+    uint32_t scale[2][2][kGroups], zero[2][2][kGroups];   // of block c of this chunk and of the next
+    auto fetch_scales = [&](uint32_t (&s)[2][kGroups], uint32_t (&z)[2][kGroups]) {
         const int block = first + ahead * apart + c;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int q = 0; q < kGroups; ++q) {
-                    s[r][half][q] = 0;
-                    z[r][half][q] = 8;
-                    if (ahead_tile < tiles && c < CH && block * kGroups + q < groups) {
-                        if (scale_bf16) s[r][half][q] = static_cast<const uint16_t *>(m.scale)[at[r][half] + q];
-                        else s[r][half][q] = static_cast<const uint32_t *>(m.scale)[at[r][half] + q];
-                        if (m.zero) z[r][half][q] = m.zero[at[r][half] + q];
-                    }
+            for (int q = 0; q < kGroups; ++q) {
+                s[half][q] = 0;
+                z[half][q] = 8;
+                if (ahead_tile < tiles && c < CH && block * kGroups + q < groups) {
+                    if (scale_bf16) s[half][q] = static_cast<const uint16_t *>(m.scale)[at[half] + q];
+                    else s[half][q] = static_cast<const uint32_t *>(m.scale)[at[half] + q];
+                    if (m.zero) z[half][q] = m.zero[at[half] + q];
                 }
+            }
     };
     auto advance = [&]() {
         if (++ahead == chunks) {
@@ -218,12 +166,10 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
             rows_of(ahead_tile);
         } else {
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    codes[r][half] += (int64_t)apart * kBlockBytes;
-                    at[r][half] += (int64_t)apart * kGroups;
-                }
+            for (int half = 0; half < 2; ++half) {
+                codes[half] += (int64_t)apart * kBlockBytes;
+                at[half] += (int64_t)apart * kGroups;
+            }
         }
     };
     rows_of(ahead_tile);
@@ -231,12 +177,10 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
     for (int u = 0; u < CH; ++u) fetch_codes(u);
     fetch_scales(scale[0], zero[0]);
     advance();
-    if constexpr (ROWS == kStaged) {
-        cp_wait<CH>();
-        __syncthreads();
-    }
+    cp_wait<CH>();
+    __syncthreads();   // A is staged
 
-    float total[RT][NT][4] = {};
+    float total[4] = {};
     int buffer = 0;
     for (int tile = blockIdx.x / share; tile < tiles; tile += stride) {
         for (int chunk = 0; chunk < chunks; ++chunk) {
@@ -246,111 +190,112 @@ gemm_w4_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, cons
                 const int block = first + chunk * apart + u;
                 cp_wait<CH - 1>();   // the lane's own slots: nobody else to wait for
                 if (block < blocks) {
-                    uint4 w[RT][2];
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) w[r][half] = slots[((u * RT + r) * 2 + half) * 32];
+                    const uint4 w[2] = {slots[(u * 2) * 32], slots[(u * 2 + 1) * 32]};
 #pragma unroll
                     for (int q = 0; q < kGroups; ++q) {
                         if (GROUP < kBlockCols && block * kGroups + q >= groups) break;   // the filled-up end of a row
-                        float sum[RT][NT][4], by[RT][2];
-                        uint32_t offset[RT][2];   // -(zero point) / 64, twice
+                        float sum[4], by[2];
+                        uint32_t offset[2];   // -(zero point) / 64, twice
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                by[r][half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][r][half][q], u, 4) << scale_shift);
-                                offset[r][half] = 0xbe00be00u;
-                                if (m.zero) offset[r][half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][r][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
-                            }
+                        for (int half = 0; half < 2; ++half) {
+                            by[half] = __uint_as_float(__shfl_sync(0xffffffffu, scale[0][half][q], u, 4) << scale_shift);
+                            offset[half] = 0xbe00be00u;
+                            if (m.zero) offset[half] = fma_pair(__shfl_sync(0xffffffffu, zero[0][half][q], u, 4) * 0x00010001u, 0xff00ff00u, 0x80008000u);
+                        }
 #pragma unroll
                         for (int j = q * (4 / kGroups); j < (q + 1) * (4 / kGroups); ++j) {
-                            uint32_t a[RT][2][4];
+                            uint32_t a[2][4];
 #pragma unroll
-                            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                                for (int half = 0; half < 2; ++half)
-                                    eight_weights(j == 0 ? w[r][half].x : j == 1 ? w[r][half].y : j == 2 ? w[r][half].z : w[r][half].w, offset[r][half], a[r][half]);
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                Operand<TA> b;
-                                b.template load<ROWS != kDirectAny>(rows[t] + block * kBlockCols + j * 32);
-#pragma unroll
-                                for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                                    for (int r = 0; r < RT; ++r) {
-                                        if (j == q * (4 / kGroups) && part == 0) mma_bf16_first(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
-                                        else mma_bf16(sum[r][t], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], b.r[part][0], b.r[part][1]);
-                                        mma_bf16(sum[r][t], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], b.r[part][2], b.r[part][3]);
-                                    }
-                            }
+                            for (int half = 0; half < 2; ++half)
+                                eight_weights(j == 0 ? w[half].x : j == 1 ? w[half].y : j == 2 ? w[half].z : w[half].w, offset[half], a[half]);
+                            const uint4 b = *reinterpret_cast<const uint4 *>(mine_a + (size_t)block * (kBlockCols * 2) + j * 64);
+                            if (j == q * (4 / kGroups)) mma_bf16_first(sum, a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                            else mma_bf16(sum, a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+                            mma_bf16(sum, a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
                         }
                         // sums 0, 1: output g, rows 2 c and 2 c + 1 of A; 2, 3: output g + 8
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(by[r][i >> 1], sum[r][t][i], total[r][t][i]);
+                        for (int i = 0; i < 4; ++i) total[i] = fmaf(by[i >> 1], sum[i], total[i]);
                     }
                 }
                 fetch_codes(u);
             }
             advance();
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q) scale[0][r][half][q] = scale[1][r][half][q], zero[0][r][half][q] = zero[1][r][half][q];
+                for (int q = 0; q < kGroups; ++q) scale[0][half][q] = scale[1][half][q], zero[0][half][q] = zero[1][half][q];
         }
         // the tile's sums: every warp's into this tile's buffer, then added in the order of the warps
-        float *mine = partial + (buffer * warps + warp) * kSums + lane * 4;
+        *reinterpret_cast<float4 *>(partial + (buffer * warps + warp) * kSums + lane * 4) = make_float4(total[0], total[1], total[2], total[3]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                *reinterpret_cast<float4 *>(mine + (r * NT + t) * 128) = make_float4(total[r][t][0], total[r][t][1], total[r][t][2], total[r][t][3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) total[r][t][i] = 0.f;
-            }
+        for (int i = 0; i < 4; ++i) total[i] = 0.f;
         __syncthreads();
-        for (int i = threadIdx.x; i < kOuts * here; i += threads) {
+        for (int i = threadIdx.x; i < kOuts * M; i += threads) {
             const int n = i % kOuts, row = i / kOuts;
             if (tile * kOuts + n >= m.rows) continue;
-            float *p = partial + buffer * warps * kSums + place<NT>(n, row);
+            float *p = partial + buffer * warps * kSums + place(n, row);
             float v = 0.f;
             for (int q = 0; q < warps; ++q) v += p[q * kSums];
             if (share > 1) *p = v;   // for the cluster's first CTA
-            else finish(kSumScale * v, tile * kOuts + n, m0 + row, bias, C, ldc, c_dtype, epilogue);
+            else finish(kSumScale * v, tile * kOuts + n, row, bias, C, ldc, c_dtype, epilogue);
         }
         buffer ^= 1;
     }
     if (share > 1) {   // one tile a cluster: its sums are in buffer 0
         cluster.sync();
         if (rank == 0)
-            for (int i = threadIdx.x; i < kOuts * here; i += threads) {
+            for (int i = threadIdx.x; i < kOuts * M; i += threads) {
                 const int n = i % kOuts, row = i / kOuts, out = blockIdx.x / share * kOuts + n;
                 if (out >= m.rows) continue;
                 float v = 0.f;
-                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + place<NT>(n, row), q);
-                finish(kSumScale * v, out, m0 + row, bias, C, ldc, c_dtype, epilogue);
+                for (int q = 0; q < share; ++q) v += *cluster.map_shared_rank(partial + place(n, row), q);
+                finish(kSumScale * v, out, row, bias, C, ldc, c_dtype, epilogue);
             }
         cluster.sync();   // the others' shared memory stays until it has been read
     }
+}
+
+// How many clusters of `share` CTAs are on the device at once; clusters that have to wait for others to end double the time
+// (24 x 5001 x 8192 fp32: 40 clusters of 7, 51.7 us; of as many CTAs as leave all of them resident, 37.4).  Asked for once a kernel,
+// size and device.
+template <typename Kernel>
+static hx_status clusters_at_once(Kernel kernel, int threads, size_t smem, int share, std::atomic<int> (&known)[64][9], int &fit) {
+    int dev = 0;
+    HX_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (fit = known[dev][share].load(std::memory_order_relaxed) - 1) >= 0) return HX_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)share);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)share;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    HX_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+    if (dev < 64) known[dev][share].store(fit + 1, std::memory_order_relaxed);
+    return HX_OK;
 }
 
 // How a product is laid out on the SMs.  More tiles than SMs: chunks of four blocks, and 16 warps' worth of CTAs on an SM, as many
 // as the staged rows of A leave room for; of fewer warps the CTAs have less to add up per tile, of more they have less to walk
 // (1 x 16384 x 4096 bf16: 13.1 us with 4 CTAs of 4, 14.1 with 2 of 8; 1 x 4096 x 4096: 7.4 and 6.9).  Otherwise one tile a CTA, or a
 // cluster, with as many warps as there are blocks.
-constexpr size_t kSmemBytes = 200 * 1024;   // of an SM, for the staged rows and the slots
+constexpr size_t kSmemBytes = 200 * 1024;   // of an SM, for the staged rows, the sums and the slots
 struct Plan { int share, warps, chunk, grid; };
-static Plan plan_of(const hx_w4_matrix &m, int outs, int most, size_t staged) {
-    const int sms = sm_count(), blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + outs - 1) / outs);
-    Plan p;
+static hx_status plan_of(const hx_w4_matrix &m, size_t staged, Plan &p) {
+    const int sms = sm_count(), blocks = blocks_of(m.cols), tiles = (int)(((int64_t)m.rows + 15) / 16), most = kMostWarps;
     p.share = std::max(1, std::min({sms / tiles, (blocks + most - 1) / most, 8}));
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> known[64][9];
+    for (int fit = 0; p.share > 1; --p.share) {   // with an SM for each CTA
+        HX_CUDA(allow_smem((const void *)gemm_w4_kernel<128, 4>, kSmemBytes, done));
+        const hx_status s = clusters_at_once(gemm_w4_kernel<128, 4>, 32 * most, kSmemBytes, p.share, known, fit);
+        if (s != HX_OK) return s;
+        if (tiles <= fit) break;
+    }
     const int part = (blocks + p.share - 1) / p.share;   // blocks of a CTA
     if (tiles > sms) {
         int ctas = tiles >= 3 * sms ? 4 : 2;
@@ -363,16 +308,17 @@ static Plan plan_of(const hx_w4_matrix &m, int outs, int most, size_t staged) {
         p.warps = std::min(most, (part + p.chunk - 1) / p.chunk);
         p.grid = tiles * p.share;
     }
-    return p;
+    return HX_OK;
 }
 
-template <typename TA, int NT, int RT, int GROUP, int CH, int ROWS>
-static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
-                           int epilogue, const Plan &p, size_t smem, bool vec, cudaStream_t st) {
-    auto kernel = gemm_w4_kernel<TA, NT, RT, GROUP, CH, ROWS>;
+template <int GROUP, int CH>
+static hx_status launch_few_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                               int epilogue, const Plan &p, size_t smem, cudaStream_t st) {
+    auto kernel = gemm_w4_kernel<GROUP, CH>;
     static std::atomic<uint64_t> done{0};
-    if (smem > 48 * 1024) HX_CUDA(allow_smem((const void *)kernel, kSmemBytes + 16 * 1024, done));
+    if (smem > 48 * 1024) HX_CUDA(allow_smem((const void *)kernel, kSmemBytes, done));
     cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
     cfg.blockDim = dim3(32 * p.warps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -382,53 +328,36 @@ static hx_status launch_as(const void *A, int64_t lda, const hx_w4_matrix &m, co
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.share > 1 ? 1 : 0;
-    constexpr int most = 65535 * 8 * NT;   // rows of a launch
-    for (int64_t m0 = 0; m0 < M; m0 += most) {
-        const int rows = (int)std::min<int64_t>(M - m0, most);
-        cfg.gridDim = dim3((unsigned)p.grid, (unsigned)((rows + 8 * NT - 1) / (8 * NT)));
-        HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const TA *>(A) + m0 * lda, lda, m, bias,
-                                   static_cast<void *>(static_cast<char *>(C) + m0 * ldc * (int64_t)dtype_size(c_dtype)), ldc, c_dtype, rows,
-                                   blocks_of(m.cols), epilogue, vec));
-    }
+    HX_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const __nv_bfloat16 *>(A), lda, m, bias, C, ldc, c_dtype, M, blocks_of(m.cols), epilogue,
+                               aligned8(A, lda, HX_BF16)));
     return check_launch("gemm_w4_kernel");
 }
-template <typename TA, int NT, int RT>
-static hx_status launch_gemm(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
-                             int epilogue, cudaStream_t st) {
-    const bool vec = aligned8(A, lda, sizeof(TA) == 4 ? HX_F32 : HX_BF16);
-    size_t staged = (size_t)std::min(M, 8 * NT) * staged_pitch<TA>(m.cols);
-    const bool stage = staged + (size_t)max_warps(NT) * RT * (NT * 1024 + (RT > 1 ? 2048 : 4096)) <= kSmemBytes;
-    if (!stage) staged = 0;
-    Plan p = plan_of(m, 16 * RT, max_warps(NT), staged);
-    if (RT > 1 || !stage) p.chunk = 2;   // instances there are; the walk covers any number of blocks
-    else if (NT > 1 && p.chunk == 1) p.chunk = 2;
-    const size_t smem = (size_t)p.warps * RT * (NT * 1024 + p.chunk * 1024) + staged;   // sums twice, slots
-#define HX_W4_AS(G, CH, ROWS) return launch_as<TA, NT, RT, G, CH, ROWS>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, vec, st)
-#define HX_W4_GROUP(G)                                                \
-    do {                                                              \
-        if (!stage && vec) HX_W4_AS(G, 2, kDirect);                   \
-        if (!stage) HX_W4_AS(G, 2, kDirectAny);                       \
-        if constexpr (RT == 1) {                                      \
-            if constexpr (NT == 1) {                                  \
-                if (p.chunk == 1) HX_W4_AS(G, 1, kStaged);            \
-            }                                                         \
-            if (p.chunk == 4) HX_W4_AS(G, 4, kStaged);                \
-        }                                                             \
-        HX_W4_AS(G, 2, kStaged);                                      \
-    } while (0)
+
+// Whether M rows of A fit into shared memory beside the warps' sums and slots.
+static bool fits_staged(const hx_w4_matrix &m, int M) { return M * staged_pitch(m.cols) + kMostWarps * (1024 + 4096) <= kSmemBytes; }
+
+static hx_status launch_few(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
+                            int epilogue, cudaStream_t st) {
+    const size_t staged = M * staged_pitch(m.cols);
+    Plan p;
+    const hx_status s = plan_of(m, staged, p);
+    if (s != HX_OK) return s;
+    const size_t smem = (size_t)p.warps * (1024 + p.chunk * 1024) + staged;   // sums twice, slots
+#define HX_W4_GROUP(G)                                                                                                           do {                                                                                                                             if (p.chunk == 1) return launch_few_as<G, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, st);                    if (p.chunk == 2) return launch_few_as<G, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, st);                    return launch_few_as<G, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, p, smem, st);                                  } while (0)
     if (m.group == 32) HX_W4_GROUP(32);
     if (m.group == 64) HX_W4_GROUP(64);
     HX_W4_GROUP(128);
 #undef HX_W4_GROUP
-#undef HX_W4_AS
 }
 
-// ---------------------------------------------------------------- more than eight rows
-// The same products where a piece of A is read for more than one tile of rows: here it costs as much as the codes, so a CTA's warps take
-// different outputs, 16 each, walk the columns together and share the block of A they are at, staged in shared memory (fp32 rows
-// already cut into their three parts, once a CTA).  One barrier a block; codes, A and scales of the next blocks are under way.  What
-// bounds it is the warp-level tensor pipe and the instructions that feed it.  Where tiles of 128 outputs are few, a cluster of CTAs
-// shares the columns; each adds up a part of the outputs out of the others' shared memory, in the order of the ranks.
+// ---------------------------------------------------------------- more rows, or fp32 ones
+// The same products where a piece of A costs as much as the codes: more than one tile of 8 rows, or fp32 rows, which have to be cut
+// (1 x 16384 x 4096 fp32: 34.6 us where every warp cuts for itself, 20.5 here).  A CTA's warps take different outputs, 16 each, walk
+// the columns together and share the block of A they are at, staged in shared memory (fp32 rows already cut, once a CTA).  One barrier
+// a block; codes, A and scales of the next blocks are under way.  What bounds it is instructions (1.5 a cycle of the SM) around a
+// warp-level tensor pipe that is 35 to 40 % busy: 16 x 16384 x 4096 bf16 18.2 us, 32 rows 25.9, 64 rows 43.5; 24 x 5001 x 8192 fp32 in
+// groups of 32 with zero points 37.4.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
+// the outputs out of the others' shared memory, in the order of the ranks.
 constexpr int kRowWarps = 8, kRowOuts = 16 * kRowWarps;
 constexpr int kRowPitch = kBlockCols * 2 + 64;   // bytes from one staged row to the next: rows g and g + 1 fall on different banks
 template <typename TA> constexpr int row_stages() { return sizeof(TA) == 2 ? 3 : 2; }   // of A
@@ -437,7 +366,7 @@ template <typename TA, int NT, int GROUP>
 __global__ void __launch_bounds__(32 * kRowWarps, NT * (int)sizeof(TA) <= 16 ? 2 : 1)
 gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
                     int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
-    constexpr int kGroups = kBlockCols / GROUP, kParts = Operand<TA>::kParts, kRows = 8 * NT, kSlots = 3, kStages = row_stages<TA>();
+    constexpr int kGroups = kBlockCols / GROUP, kParts = kPartsOf<TA>, kRows = 8 * NT, kSlots = 3, kStages = row_stages<TA>();
     constexpr int kStage = kParts * kRows * kRowPitch, kThreads = 32 * kRowWarps;
     extern __shared__ __align__(16) unsigned char shared[];   // [kStages][kParts][kRows][kRowPitch], then the codes' slots
     const auto cluster = cooperative_groups::this_cluster();
@@ -524,7 +453,7 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
                 for (int part = 0; part < 3; ++part) {
                     uint32_t u[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(Operand<float>::take(v[e]));
+                    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(take_part(v[e]));
                     *reinterpret_cast<uint2 *>(to + stage * kStage + (part * kRows + i * down) * kRowPitch) =
                         make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
                 }
@@ -634,8 +563,8 @@ template <typename TA, int NT, int GROUP>
 static hx_status launch_rows_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                                 int epilogue, cudaStream_t st) {
     constexpr int kRows = 8 * NT, per_sm = NT * (int)sizeof(TA) <= 16 ? 2 : 1;
-    constexpr size_t staged = (size_t)row_stages<TA>() * Operand<TA>::kParts * kRows * kRowPitch, smem = staged + kRowWarps * 3 * 1024;
-    static_assert(staged + kRowWarps * 3 * 1024 >= (size_t)kRows * kRowOuts * sizeof(float), "the sums of a cluster's CTA fit");
+    constexpr size_t staged = (size_t)row_stages<TA>() * kPartsOf<TA> * kRows * kRowPitch, smem = staged + kRowWarps * 3 * 1024;
+    static_assert(smem >= (size_t)kRows * kRowOuts * sizeof(float), "the sums of a cluster's CTA fit");
     auto kernel = gemm_w4_rows_kernel<TA, NT, GROUP>;
     static std::atomic<uint64_t> done{0};
     HX_CUDA(allow_smem((const void *)kernel, smem, done));
@@ -650,21 +579,10 @@ static hx_status launch_rows_as(const void *A, int64_t lda, const hx_w4_matrix &
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    // Clusters that are not all resident at once take twice the time: how many fit is asked for once a kernel, size and device.
-    static std::atomic<int> resident[64][9];
-    int dev = 0;
-    HX_CUDA(cudaGetDevice(&dev));
-    for (; share > 1; --share) {
-        std::atomic<int> *known = dev < 64 ? &resident[dev][share] : nullptr;
-        int fit = known ? known->load(std::memory_order_relaxed) : 0;
-        if (fit == 0) {
-            attr.val.clusterDim.x = (unsigned)share;
-            cfg.numAttrs = 1;
-            cfg.gridDim = dim3((unsigned)share);
-            HX_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
-            fit = std::max(fit, 1);
-            if (known) known->store(fit, std::memory_order_relaxed);
-        }
+    static std::atomic<int> known[64][9];
+    for (int fit = 0; share > 1; --share) {
+        const hx_status s = clusters_at_once(kernel, 32 * kRowWarps, smem, share, known, fit);
+        if (s != HX_OK) return s;
         if (tiles * down <= fit) break;
     }
     attr.val.clusterDim.x = (unsigned)share;

@@ -193,6 +193,18 @@ def test_product(M, N, K, group, adt, zeros):
     assert L.device_status() == 0
 
 
+@pytest.mark.parametrize("adt", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", [(8, 40, 16384, 128), (2, 768, 12288, 64), (1, 300, 16384, 32), (20, 2600, 1056, 32), (50, 900, 4096, 128)])
+def test_product_shared_by_clusters(M, N, K, group, adt):
+    """Long rows and few outputs: the columns are cut over CTAs, or the rows are too long to be staged whole."""
+    codes, scale, zero = make(M + N + K, N, K, group, DT[adt], True)
+    m = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda())
+    a = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(DT[adt]).cuda()
+    got = ops.gemm_w4(a, m, out_dtype=torch.float32)
+    check_product(got, a, values(codes, scale, zero, group), None)
+    assert torch.equal(got, ops.gemm_w4(a, m, out_dtype=torch.float32))
+
+
 @pytest.mark.parametrize("epilogue", [L.EPI_NONE, L.EPI_SILU, L.EPI_SOFTPLUS])
 @pytest.mark.parametrize("adt,cdt,sdt", [("f32", "f32", "bf16"), ("f32", "bf16", "f32"), ("bf16", "f32", "f32"), ("bf16", "bf16", "bf16")])
 def test_product_types_bias_and_epilogue(adt, cdt, sdt, epilogue):
