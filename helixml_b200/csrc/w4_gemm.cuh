@@ -54,13 +54,14 @@ __device__ __forceinline__ void eight_weights(uint32_t word, uint32_t minus_zero
 }
 constexpr float kSumScale = 64.f;   // what the sums have to be multiplied by in the end
 
-// fp32 rows of A go into the MMA as three bf16 parts that add up to them.  v = high 8 bits + rest; the rest is exact, and zero for an
-// infinity.
+// fp32 rows of A go into the MMA as three bf16 parts that add up to them: the high 8 bits, the next 8, the rest.  The differences are
+// exact; an infinity has no rest, a NaN a NaN.
 template <typename TA> constexpr int kPartsOf = sizeof(TA) == 2 ? 1 : 3;
-__device__ __forceinline__ float take_part(float &v) {
-    const float high = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    v = v == high ? 0.f : v - high;
-    return high;
+__device__ __forceinline__ void cut(float v, uint32_t (&part)[3]) {
+    part[0] = __float_as_uint(v) & 0xffff0000u;
+    const float rest = v == __uint_as_float(part[0]) ? 0.f : v - __uint_as_float(part[0]);
+    part[1] = __float_as_uint(rest) & 0xffff0000u;
+    part[2] = __float_as_uint(rest - __uint_as_float(part[1]));
 }
 
 __device__ __forceinline__ void finish(float v, int n, int row, const float *bias, void *C, int64_t ldc, int c_dtype, int epilogue) {
@@ -358,16 +359,17 @@ static hx_status launch_few(const void *A, int64_t lda, const hx_w4_matrix &m, c
 // warp-level tensor pipe that is 35 to 40 % busy: 16 x 16384 x 4096 bf16 18.2 us, 32 rows 25.9, 64 rows 43.5; 24 x 5001 x 8192 fp32 in
 // groups of 32 with zero points 37.4.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
 // the outputs out of the others' shared memory, in the order of the ranks.
-constexpr int kRowWarps = 8, kRowOuts = 16 * kRowWarps;
+template <typename TA, int NT> constexpr int row_warps() { return 8; }
 constexpr int kRowPitch = kBlockCols * 2 + 64;   // bytes from one staged row to the next: rows g and g + 1 fall on different banks
+template <typename TA, int NT> constexpr int row_ctas() { return NT * (int)sizeof(TA) <= 16 ? 2 : 1; }   // an SM holds
 template <typename TA> constexpr int row_stages() { return sizeof(TA) == 2 ? 3 : 2; }   // of A
 
 template <typename TA, int NT, int GROUP>
-__global__ void __launch_bounds__(32 * kRowWarps, NT * (int)sizeof(TA) <= 16 ? 2 : 1)
+__global__ void __launch_bounds__(32 * row_warps<TA, NT>(), row_ctas<TA, NT>())
 gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m, const float *__restrict__ bias, void *__restrict__ C,
                     int64_t ldc, int c_dtype, int M, int blocks, int epilogue, bool vec) {
     constexpr int kGroups = kBlockCols / GROUP, kParts = kPartsOf<TA>, kRows = 8 * NT, kSlots = 3, kStages = row_stages<TA>();
-    constexpr int kStage = kParts * kRows * kRowPitch, kThreads = 32 * kRowWarps;
+    constexpr int kStage = kParts * kRows * kRowPitch, kThreads = 32 * row_warps<TA, NT>(), kRowOuts = kThreads / 2;
     extern __shared__ __align__(16) unsigned char shared[];   // [kStages][kParts][kRows][kRowPitch], then the codes' slots
     const auto cluster = cooperative_groups::this_cluster();
     const int share = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -414,7 +416,7 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
         for (int half = 0; half < 2; ++half) at[half] += 4 * kGroups;
     };
     // A: bf16 goes straight into its stage; fp32 waits in registers for a block's time and is cut on its way
-    constexpr int per = 16 / (int)sizeof(TA), across = kBlockCols / per, kPieces = kRows * across / kThreads, down = kThreads / across;
+    constexpr int per = 16 / (int)sizeof(TA), across = kBlockCols / per, down = kThreads / across, kPieces = (kRows + down - 1) / down;
     const int row0 = threadIdx.x / across, col = threadIdx.x % across * per;   // a thread's pieces: this column of rows row0, row0 + down, ...
     const TA *from = A + (int64_t)(m0 + row0) * lda + (int64_t)k0 * kBlockCols + col;
     unsigned char *const to = shared + row0 * kRowPitch + col * 2;
@@ -448,15 +450,15 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
         if constexpr (sizeof(TA) == 4) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                float v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+                if (kRows % down != 0 && row0 + i * down >= kRows) break;
+                const float v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+                uint32_t u[4][3];
 #pragma unroll
-                for (int part = 0; part < 3; ++part) {
-                    uint32_t u[4];
+                for (int e = 0; e < 4; ++e) cut(v[e], u[e]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(take_part(v[e]));
+                for (int part = 0; part < 3; ++part)
                     *reinterpret_cast<uint2 *>(to + stage * kStage + (part * kRows + i * down) * kRowPitch) =
-                        make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
-                }
+                        make_uint2(__byte_perm(u[0][part], u[1][part], 0x7632), __byte_perm(u[2][part], u[3][part], 0x7632));
             }
         }
     };
@@ -562,7 +564,7 @@ gemm_w4_rows_kernel(const TA *__restrict__ A, int64_t lda, const hx_w4_matrix m,
 template <typename TA, int NT, int GROUP>
 static hx_status launch_rows_as(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M,
                                 int epilogue, cudaStream_t st) {
-    constexpr int kRows = 8 * NT, per_sm = NT * (int)sizeof(TA) <= 16 ? 2 : 1;
+    constexpr int kRows = 8 * NT, per_sm = row_ctas<TA, NT>(), kRowWarps = row_warps<TA, NT>(), kRowOuts = 16 * kRowWarps;
     constexpr size_t staged = (size_t)row_stages<TA>() * kPartsOf<TA> * kRows * kRowPitch, smem = staged + kRowWarps * 3 * 1024;
     static_assert(smem >= (size_t)kRows * kRowOuts * sizeof(float), "the sums of a cluster's CTA fit");
     auto kernel = gemm_w4_rows_kernel<TA, NT, GROUP>;
