@@ -1,5 +1,8 @@
 // Weights in 4 bits with a scale per group of columns: quantising, laying out given codes, reading back, and the
 // entry points of the product.
+#include <type_traits>
+
+#include "hx_tma.cuh"
 #include "w4.cuh"
 
 namespace hx {
@@ -31,9 +34,20 @@ __device__ __forceinline__ float settle(float w, float s, float q, float n) {
 }
 
 constexpr int kEach = 2;   // words of a thread
+constexpr float kLargest = 3.402823466e38f;
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
-// A thread takes 16 columns, two words, 8 threads a block of 128; a group's 2, 4 or 8 threads meet in shuffles.  What bounds it is
-// instructions, 25 a weight.
+// A thread takes 16 columns, two words; a group's threads meet in shuffles.  What bounds it is instructions, about half of them a
+// thread's own and half a weight's: 8192 x 8192 fp32 59 us (78 % of a copy's rate), 16384 x 4096 bf16 with bf16 scales 50 (52 %).
 template <typename T, bool ZERO>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int blocks, int shift, bool vec) {   // group = 2^shift
@@ -47,17 +61,16 @@ quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int 
 #pragma unroll
         for (int i = 0; i < kEach; ++i) load8(W + n * ldw + part * per + i * 8, vec, v[i]);
     }
-    float lo = 0.f, hi = 0.f, bad = 0.f;
+    float lo = 0.f, hi = 0.f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            bad = fmaf(v[i][j], 0.f, bad);   // NaN from the first infinity or NaN on
-            if constexpr (ZERO) lo = fminf(lo, v[i][j]), hi = fmaxf(hi, v[i][j]);
-            else hi = fmaxf(hi, fabsf(v[i][j]));
+            if constexpr (ZERO) lo = min_nan(lo, v[i][j]), hi = max_nan(hi, v[i][j]);
+            else hi = max_nan(hi, fabsf(v[i][j]));
         }
-    if (bad != bad) hi = __int_as_float(0x7f800000);   // travels with the maximum
-    for (int o = 1; o << 4 < m.group; o <<= 1) {   // 16 columns a thread
+    if (!(hi <= kLargest && lo >= -kLargest)) hi = __int_as_float(0x7f800000);   // an infinity or a NaN travels with the maximum
+    for (int o = 1; o * per < m.group; o <<= 1) {
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         if constexpr (ZERO) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
@@ -75,10 +88,12 @@ quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int 
             s = hi / 7.f;
         }
         if (m.scale_dtype == HX_BF16) s = __bfloat162float(__float2bfloat16_rn(s));
-        if (hi > 3.402823466e38f) s = __int_as_float(0x7fc00000);
+        if (hi > kLargest) s = __int_as_float(0x7fc00000);
         if (s > 0.f) {   // neither zero nor NaN
             float t = s;   // the divisor, out of the range where its reciprocal overflows
-            if (s < 0x1p-100f) {
+            float worst = 0.f;
+            if (s < 0x1p-100f) {   // also where s is so coarse that quotients may lie beyond their range
+                worst = 1.f;
                 t *= 0x1p100f;
                 lo *= 0x1p100f;
 #pragma unroll
@@ -92,18 +107,38 @@ quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int 
                 zero = fminf(fmaxf(settle(-lo, t, q, (q + kRound) - kRound), 0.f), 15.f);
             }
             const float low = (ZERO ? 0.f : 1.f) - zero, high = 15.f - zero;
-            const uint32_t add = (uint32_t)zero;   // 15 + 15 at most: no carry out of what is kept
-            float worst = 0.f;
+            // A word is the sum of its codes times powers of 16, and the integer that kRound leaves in the low bits is one term
+            // of it, without its zero point and with kRound's own bits on top, both of which `rest` makes good.  Symmetric
+            // quotients are within 7 (1 + 2^-8) by themselves.
+            const uint32_t rest = ((uint32_t)zero - __float_as_uint(kRound)) * 0x11111111u;
+            const float2 inv2 = splat2(inv), round2 = splat2(kRound), back2 = splat2(-kRound), minus2 = splat2(-1.f), minus_t2 = splat2(-t);
+            auto words = [&](auto short_operands) {
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                word[i] = 0;
+                for (int i = 0; i < kEach; ++i) {
+                    float u[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float q = fminf(fmaxf(v[i][j] * inv, low), high), u = q + kRound;
-                    worst = fmaxf(worst, fabsf(q - (u - kRound)));
-                    word[i] |= ((__float_as_uint(u) + add) & 15u) << (4 * nibble_of(j));
+                    for (int j = 0; j < 8; j += 2) {
+                        const float2 w = make_float2(v[i][j], v[i][j + 1]);
+                        float2 q = mul2(w, inv2);
+                        if constexpr (short_operands) q = fma2(fma2(q, minus_t2, w), inv2, q);
+                        if constexpr (ZERO) q = make_float2(fminf(fmaxf(q.x, low), high), fminf(fmaxf(q.y, low), high));
+                        const float2 r = add2(q, round2);
+                        if constexpr (!short_operands) {
+                            const float2 off = fma2(add2(r, back2), minus2, q);
+                            worst = fmaxf(worst, fmaxf(fabsf(off.x), fabsf(off.y)));
+                        }
+                        u[j] = r.x, u[j + 1] = r.y;
+                    }
+                    uint32_t sum = 0;
+#pragma unroll
+                    for (int p = 7; p >= 0; --p) sum = (sum << 4) + __float_as_uint(u[column_of(p)]);
+                    word[i] = sum + rest;
                 }
-            }
+            };
+            // Weights and scales of 8 bits: a quotient is a half or at least 2^-9 from one, and one that is a half is common (16384 x
+            // 4096: 66 us where every warp settles some).  The remainder w - q t is exact, and with it q is a half where the quotient is.
+            if (sizeof(T) == 2 && m.scale_dtype == HX_BF16) words(std::true_type{});
+            else words(std::false_type{});
             if (worst > kNear) {
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
@@ -144,22 +179,24 @@ pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, i
     reinterpret_cast<uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)] = word;
 }
 
-// A thread per word: its 8 values are 32 or 16 consecutive bytes.
+// A thread takes 16 columns, two words of one group; they are 64 or 32 bytes of W, written a sector at a time: 8192 x 8192 fp32 51 us
+// (91 % of a copy's rate; 74 in 16-byte stores of a word a thread), 16384 x 4096 bf16 37 (70 %; 49).
 template <typename T>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int blocks, int shift, bool vec) {
     int64_t n;
-    int w;
-    split((int64_t)blockIdx.x * 256 + threadIdx.x, m.cols >> 3, n, w);
+    int part;
+    split((int64_t)blockIdx.x * 256 + threadIdx.x, m.cols >> 4, n, part);
     if (n >= m.rows) return;
-    const uint32_t word = reinterpret_cast<const uint32_t *>(m.codes)[(n * blocks + (w >> 4)) * 16 + word_at(w & 15)];
-    const int64_t at = n * (m.cols >> shift) + (w * 8 >> shift);
+    const uint32_t *words = reinterpret_cast<const uint32_t *>(m.codes) + (n * blocks + (part >> 3)) * 16;
+    const uint32_t word[2] = {words[word_at((part & 7) * 2)], words[word_at((part & 7) * 2 + 1)]};
+    const int64_t at = n * (m.cols >> shift) + (part * 16 >> shift);
     const float s = load_scale(m.scale, m.scale_dtype, at);
     const float base = 8388608.f + (float)(m.zero ? m.zero[at] : 8);   // 2^23: a code in its low bits adds itself
-    float v[8];
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = s * (__uint_as_float(((word >> (4 * nibble_of(j))) & 15u) | 0x4b000000u) - base);
-    store8(W + n * ldw + w * 8, vec, v);
+    for (int j = 0; j < 16; ++j) v[j] = s * (__uint_as_float(((word[j / 8] >> (4 * nibble_of(j % 8))) & 15u) | 0x4b000000u) - base);
+    store16(W + n * ldw + part * 16, vec, v);
 }
 
 static hx_status check_matrix(const char *who, const hx_w4_matrix *m) {
@@ -241,7 +278,7 @@ hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t 
     HX_REQUIRE(W != nullptr, HX_ERR_INVALID_INPUT, "hx_w4_dequantize: W is NULL");
     HX_REQUIRE(m->rows == 1 || ldw >= m->cols, HX_ERR_SHAPE_MISMATCH, "hx_w4_dequantize: rows of W overlap (stride %lld)", (long long)ldw);
     unsigned grid;
-    const hx_status g = grid_of("hx_w4_dequantize", (int64_t)m->rows * (m->cols / 8), &grid);
+    const hx_status g = grid_of("hx_w4_dequantize", (int64_t)m->rows * (m->cols / 16), &grid);
     if (g != HX_OK) return g;
     const bool vec = aligned8(W, ldw, w_dtype);
     const int shift = m->group == 32 ? 5 : m->group == 64 ? 6 : 7;

@@ -13,6 +13,7 @@ constexpr uint32_t kFill = 0x88888888u;  // eight codes of 8: what pads the last
 __device__ __forceinline__ int word_at(int w) { return (w & 3) * 4 + (w >> 2); }
 // column i of 8 is at nibble i / 2 + 4 (i mod 2)
 __device__ __forceinline__ int nibble_of(int i) { return (i >> 1) | ((i & 1) << 2); }
+__device__ __forceinline__ int column_of(int p) { return (p & 3) * 2 + (p >> 2); }
 
 // A thread's eight consecutive elements, as fp32.
 template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]) {
@@ -38,21 +39,40 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = ld_f32(p + i);
 }
-template <typename T> __device__ __forceinline__ void store8(T *p, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// 32 bytes, a whole sector in one instruction where the address allows it
+__device__ __forceinline__ void store32(void *p, const uint32_t (&u)[8]) {
+    if (((uintptr_t)p & 31) == 0) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+                     "r"(u[6]), "r"(u[7])
+                     : "memory");
+    } else {
+        static_cast<uint4 *>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        static_cast<uint4 *>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store16(T *p, bool vec, const float (&v)[16]) {
     if (vec) {
+        uint32_t u[8];
         if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            __nv_bfloat162 r[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(r);
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(v[half * 8 + i]);
+                store32(p + half * 8, u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            store32(p, u);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) st_f32(p + i, v[i]);
+    for (int i = 0; i < 16; ++i) st_f32(p + i, v[i]);
 }
 
 __device__ __forceinline__ float load_scale(const void *scale, int dtype, int64_t i) {

@@ -131,6 +131,31 @@ def test_quantize_on_and_beside_the_halves(zeros, sdt):
     check_quantize(torch.stack(rows).cuda(), 32, zeros, DT[sdt])
 
 
+@pytest.mark.parametrize("sdt", ["f32", "bf16"])
+@pytest.mark.parametrize("wdt", ["f32", "bf16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_short_numbers(zeros, wdt, sdt):
+    """Weights and scales of few bits, whose quotients are often exactly a half, at ordinary and at extreme sizes."""
+    gen = torch.Generator().manual_seed(3)
+    w = torch.randn(640, 1024, generator=gen)
+    w[:320] = (w[:320] * 8).round() / 8
+    w[320:480] = (w[320:480] * 100).round()
+    w = w * torch.tensor([1.0, 2.0 ** -100, 2.0 ** -118, 2.0 ** 100]).repeat(160)[:, None]
+    check_quantize(w.to(DT[wdt]).cuda(), 64, zeros, DT[sdt])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (4, 4), (8, 8), (8, 24), (1, 0), (16, 16)])
+def test_dequantize_at_every_alignment(offset, pad, dtype):
+    codes, scale, zero = make(9, 11, 96, 32, torch.float32, True)
+    m = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda())
+    flat = torch.full((offset + 11 * (96 + pad) + 32,), 7.0, device="cuda", dtype=DT[dtype])
+    out = flat[offset:offset + 11 * (96 + pad)].view(11, 96 + pad)
+    ops.w4_dequantize(m, DT[dtype], out=out[:, :96])
+    assert torch.equal(out[:, :96].cpu(), values(codes, scale, zero, 32).float().to(DT[dtype]))
+    assert (out[:, 96:] == 7).all() and (flat[:offset] == 7).all() and (flat[offset + 11 * (96 + pad):] == 7).all()
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 def test_quantize_of_unusual_groups(zeros):
     """Groups of zeros, of one sign, of one value, of denormals, with the largest numbers; infinities and NaN spoil their group."""
