@@ -37,9 +37,10 @@ def _f32(t):
 
 def _view3(t: torch.Tensor):
     """(batch_stride, row_stride) in elements of a [B, L, D] view whose last stride is 1."""
-    if t.dim() != 3 or t.stride(2) != 1:
-        raise L.HxError(1, f"expected a [B, L, D] tensor with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
-    return t.stride(0), t.stride(1)
+    strides = t.stride()
+    if len(strides) != 3 or strides[2] != 1:
+        raise L.HxError(1, f"expected a [B, L, D] tensor with unit inner stride, got {tuple(t.shape)} / {strides}")
+    return strides[0], strides[1]
 
 
 def check_geometric(A: torch.Tensor) -> bool:
@@ -206,6 +207,11 @@ def _same(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _rows_like(rows, cols, dtype, dev):
+    """An uninitialised dense [rows, cols] tensor, the other way."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=dev)
+
+
 def _dense(name, t, shape, dtype, dev):
     """An operand the library takes without strides: checked, and copied where it is a strided view."""
     if t is None:
@@ -278,7 +284,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     hb, hr = _view3(h)
     h0 = _dense("h0", h0, (Bsz, Dm), torch.float32, dev)
     lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
-    last = torch.empty_strided((Bsz, Dm), (Dm, 1), dtype=torch.float32, device=dev) if return_state else None
+    last = _rows_like(Bsz, Dm, torch.float32, dev) if return_state else None
     if states is not None:
         _dense_out("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
     ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
@@ -311,7 +317,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     states = _dense("states", states, (Bsz, _state_rows(Lq), Dm), torch.float32, dev)
     dh_last = _dense("dh_last", dh_last, (Bsz, Dm), torch.float32, dev)
     lengths = _dense("lengths", lengths, (Bsz,), torch.int32, dev)
-    dh0 = torch.empty_strided((Bsz, Dm), (Dm, 1), dtype=torch.float32, device=dev)
+    dh0 = _rows_like(Bsz, Dm, torch.float32, dev)
     ws = _gated_scan_workspace(dev, Bsz, Lq, Dm, dt)
     a = L.GatedScanBwdArgs(Bsz, Lq, Dm, dt, _gate(gate), 0, x.data_ptr(), g.data_ptr(), dh.data_ptr(), dx.data_ptr(), dg.data_ptr(), xb,
                            xr, gb, gr, db, dr, dxb, dxr, dgb, dgr, _at(states), _at(dh_last), _at(dh0), _at(lengths), _at(ws),
@@ -454,7 +460,7 @@ class W4Matrix:
         self.rows, self.cols, self.group = rows, cols, group
         self.scale = _dense("scale", scale, (rows, cols // group), scale.dtype, dev)
         self.zero = _dense("zero", zero, (rows, cols // group), torch.uint8, dev)
-        self.codes = torch.empty((rows, L.lib().hx_w4_row_bytes(cols)), dtype=torch.uint8, device=dev)
+        self.codes = _rows_like(rows, L.lib().hx_w4_row_bytes(cols), torch.uint8, dev)
 
     def _args(self):
         return L.W4MatrixArgs(self.rows, self.cols, self.group, _FLOATS[self.scale.dtype], self.codes.data_ptr(), self.scale.data_ptr(),
@@ -477,8 +483,8 @@ def w4_quantize(w, group=64, zero_points=False, scale_dtype=torch.float32) -> W4
     N, K = w.shape
     if group not in (32, 64, 128) or K % group:
         raise L.HxError(1, f"{K} columns in groups of {group}: groups are 32, 64 or 128 and divide the columns")
-    scale = torch.empty((N, K // group), dtype=scale_dtype, device=dev)
-    zero = torch.empty((N, K // group), dtype=torch.uint8, device=dev) if zero_points else None
+    scale = _rows_like(N, K // group, scale_dtype, dev)
+    zero = _rows_like(N, K // group, torch.uint8, dev) if zero_points else None
     m = W4Matrix(N, K, group, scale, zero)
     _call(dev, L.lib().hx_w4_quantize, w.data_ptr(), ldw, dt, C.byref(m._args()))
     return m
@@ -505,7 +511,7 @@ def w4_pack(codes, scale, zero=None) -> W4Matrix:
 def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
     """The values a W4Matrix stands for, [N, K] fp32 or bf16 (hx_w4_dequantize)."""
     dev = m.codes.get_device()
-    w = torch.empty((m.rows, m.cols), dtype=dtype, device=dev) if out is None else out
+    w = _rows_like(m.rows, m.cols, dtype, dev) if out is None else out
     dt = _float("out", w)
     _like("out", w, (m.rows, m.cols), dtype, dev)
     _call(dev, L.lib().hx_w4_dequantize, C.byref(m._args()), w.data_ptr(), _rows2("out", w), dt)
@@ -524,7 +530,7 @@ def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=
         raise L.HxError(3, f"a is on {a.device}, W on {m.codes.device}")
     bias = _dense("bias", bias, (m.rows,), torch.float32, dev)
     if out is None:
-        c = torch.empty_strided((M, m.rows), (m.rows, 1), dtype=out_dtype or a.dtype, device=dev)
+        c = _rows_like(M, m.rows, out_dtype or a.dtype, dev)
         ldc = m.rows
     else:
         c = out
