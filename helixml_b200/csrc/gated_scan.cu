@@ -26,9 +26,11 @@ namespace gated {
 constexpr int kC = 64;                    // channels of a warp, two a lane
 constexpr int kRun = 8;                   // steps of a forward fetch
 constexpr int kBlock = HX_GATED_SCAN_STATE_STEPS;   // steps of a backward fetch: from one saved state to the next
-constexpr int kWarps = 4;                 // warps of a CTA, each on its own
+// Warps of a CTA, each on its own.  Small CTAs spread evenly over the SMs: backward 5 x 1003 x 1001 fp32 36.9 us with two, 42.3 with
+// four, 49.5 with one, whose CTAs cost more to start.
+constexpr int kWarps = 2;
 constexpr int kStages = 6, kBlockStages = 3;        // fetches a ring of runs, of blocks holds: all but one are under way
-constexpr int kOccupancy = 4, kBlockOccupancy = 3;  // CTAs an SM is to hold (registers)
+constexpr int kOccupancy = 8, kBlockOccupancy = 6;  // CTAs an SM is to hold (registers)
 static_assert(kBlock == 2 * kRun, "segments are multiples of both");
 
 template <int BYTES> __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
