@@ -652,7 +652,8 @@ constexpr int64_t kStepBytes = 45000, kWarpBytes = 24, kMostSegments = 128;
 // Cut sequences whose two tensors of the first launch are more than L2 holds go span by span, so that the second launch of a span
 // finds in L2 what the first has read; the first launch of the next span runs as the second of this one ends.  Forward, 1 x 32768 x
 // 1536 fp32: 161 us whole, 143 in spans of 112 MiB, 133 of 56, 140 of 28.  Backward the second launch has a third tensor to read and
-// two to write, and shorter spans gain less: 1 x 16384 x 4096 bf16 167 us whole, 154 of 112, 147 of 56; fp32 as above 223, 222, 232.
+// two to write, and shorter spans gain less: 1 x 16384 x 4096 bf16 167 us whole, 154 of 112, 147 of 56; fp32 as above 223, 222, 232.  (All
+// with CTAs of four warps; with two, fp32 131 forward and 212 backward.)
 constexpr int64_t kSpanBytes = (int64_t)56 << 20, kSpanBytesBwd = (int64_t)112 << 20;
 struct Plan { int segs, seg_len, span; };
 static Plan whole(int seq_len) { return {1, 0x7fffffff / kBlock * kBlock, seq_len}; }

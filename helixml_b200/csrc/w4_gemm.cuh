@@ -353,11 +353,11 @@ static hx_status launch_few(const void *A, int64_t lda, const hx_w4_matrix &m, c
 
 // ---------------------------------------------------------------- more rows, or fp32 ones
 // The same products where a piece of A costs as much as the codes: more than one tile of 8 rows, or fp32 rows, which have to be cut
-// (1 x 16384 x 4096 fp32: 34.6 us where every warp cuts for itself, 20.5 here).  A CTA's warps take different outputs, 16 each, walk
+// (1 x 16384 x 4096 fp32: 34.6 us where every warp cuts for itself, 20.0 here).  A CTA's warps take different outputs, 16 each, walk
 // the columns together and share the block of A they are at, staged in shared memory (fp32 rows already cut, once a CTA).  One barrier
 // a block; codes, A and scales of the next blocks are under way.  What bounds it is instructions (1.5 a cycle of the SM) around a
 // warp-level tensor pipe that is 35 to 40 % busy: 16 x 16384 x 4096 bf16 18.2 us, 32 rows 25.9, 64 rows 43.5; 24 x 5001 x 8192 fp32 in
-// groups of 32 with zero points 37.4.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
+// groups of 32 with zero points 36.1.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
 // the outputs out of the others' shared memory, in the order of the ranks.
 template <typename TA, int NT> constexpr int row_warps() { return 8; }
 constexpr int kRowPitch = kBlockCols * 2 + 64;   // bytes from one staged row to the next: rows g and g + 1 fall on different banks

@@ -269,7 +269,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     """Gated linear recurrence (hx_gated_scan_fwd): h_t = g_t h_{t-1} + x_t ("decay"), or a_t h_{t-1} + (1 - a_t) x_t with
     a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
     lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
-    states: a gated_scan_states buffer, filled for gated_scan_bwd.  Returns h, or (h, h_last [B, D] fp32) with return_state."""
+    states: a gated_scan_states buffer, filled for gated_scan_bwd; out shares no memory with x or g.  Returns h, or (h, h_last [B, D] fp32) with return_state."""
     dev, shape = _cuda("x", x), x.shape
     xb, xr = _view3(x)
     dt = _float("x", x)
@@ -520,7 +520,7 @@ def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
 
 def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=None):
     """C = a @ W.T (+ bias) (+ activation) with W in 4 bits (hx_gemm_w4), for the few rows of a decode step.
-    a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's)."""
+    a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's), no memory of a's."""
     dev, lda = _cuda("a", a), _rows2("a", a)
     adt = _float("a", a)
     M, K = a.shape
