@@ -269,7 +269,8 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     """Gated linear recurrence (hx_gated_scan_fwd): h_t = g_t h_{t-1} + x_t ("decay"), or a_t h_{t-1} + (1 - a_t) x_t with
     a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
     lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
-    states: a gated_scan_states buffer, filled for gated_scan_bwd; out shares no memory with x or g.  Returns h, or (h, h_last [B, D] fp32) with return_state."""
+    states: a gated_scan_states buffer, filled for gated_scan_bwd; out shares no memory with x or g.
+    Returns h, or (h, h_last [B, D] fp32) with return_state."""
     dev, shape = _cuda("x", x), x.shape
     xb, xr = _view3(x)
     dt = _float("x", x)

@@ -464,9 +464,10 @@ HX_API hx_status hx_w4_pack(const uint8_t *in, int64_t ldc, const hx_w4_matrix *
 /* The values the matrix stands for: W [rows, cols] fp32 or bf16, row stride ldw. */
 HX_API hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t w_dtype, void *stream);
 /* C[M,N] = A[M,K] . W^T (+ bias[N]) (+ activation: 0 none, 1 SiLU, 2 softplus) with N = m->rows, K = m->cols; A and C fp32 or
- * bf16 with row strides in elements, bias fp32; C overlaps neither A nor the matrix.  Every product and sum is fp32 or wider than its operands: codes are exact,
- * the sum over a group is scaled in fp32.  Made for the few rows of a decode step (any M is right; the weights are
- * turned into operands once per 64 rows, so for hundreds of rows hx_w4_dequantize with hx_gemm_bf16 is the faster way). */
+ * bf16 with row strides in elements, bias fp32; C overlaps neither A nor the matrix.  Every product and sum is fp32 or wider
+ * than its operands: codes are exact, the sum over a group is scaled in fp32.  Made for the few rows of a decode step (any M is
+ * right; the weights are turned into operands once per 64 rows, so from about 200 rows on hx_w4_dequantize with hx_gemm_bf16 is
+ * the faster way: N = K = 4096, 128 rows 24 us against 32, 512 rows 67 against 34). */
 HX_API hx_status hx_gemm_w4(const void *A, int64_t lda, int32_t a_dtype, const hx_w4_matrix *m, const float *bias, void *C,
                      int64_t ldc, int32_t c_dtype, int32_t M, int32_t epilogue, void *stream);
 
