@@ -11,9 +11,11 @@
 // The backward pass is the same recurrence from the end, e_t = a_t (dh_t + e_{t+1}); h_{t-1} is recomputed from the state that the
 // forward pass saved every 16 steps, so h itself, rounded to the io type, is not needed.
 //
-// Folding maps is not the recurrence where numbers leave the format: a product of decays that underflows times an infinite state
-// would be NaN, one that overflows times a state of zero too.  Where a map's A or a folded state is not finite, the warp walks the
-// steps from there to its segment instead.
+// Folding maps is not the recurrence where numbers leave the format.  A state that overflows in the middle of a segment stays infinite
+// when its steps are walked, but a map knows the ends of a segment only, and what overflowed may have decayed by then; a product of
+// decays that underflows has lost what a large state, or growth before it, would have made of it.  So the first launch also bounds how
+// far a state can get within a segment and what its products have lost, marks a map that cannot stand for the walk (A is NaN), and the
+// warp walks the steps from there to its segment where it meets such a map or a state that the map is not made for (Reach, odd).
 #include <algorithm>
 #include <initializer_list>
 
@@ -188,7 +190,7 @@ template <bool FAST> __device__ __forceinline__ void sigmoid2(float2 g, float2 &
     a = add2(r, splat2(-0x1p-126f));
 }
 
-__device__ __forceinline__ bool finite(float2 v) { return fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f; }
+constexpr float kLargest = 3.402823466e38f;
 
 // One step's decay and input from its gate and x; `rest` is 1 - a (sigmoid only).
 template <int GATE, bool FAST> __device__ __forceinline__ void gate_step(float2 g, float2 x, float2 &a, float2 &b, float2 &rest) {
@@ -242,8 +244,84 @@ __device__ __forceinline__ float4 *map_at(float2 *maps, int seg, int b, int c, i
     return reinterpret_cast<float4 *>(maps + ((int64_t)seg * batch + b) * ((d_inner + 1) & ~1) + c);
 }
 
+// A segment's map h -> A h + B of a channel and what it is good for, built from its last run of steps to its first.
+// A run has gone from the state 0 to r and has multiplied by p; `least` and `most` are the smallest and the largest |product| on the way.
+//   overflow   A walk of the run from 0 that overflows leaves r, and then B, infinite or NaN.  What a state entering the run adds to it
+//              is at most lift |h| from before the segment and `reach` from its own runs; where both are below 2^102, half the last
+//              place of the largest number and less, the walk from h overflows where that from 0 does.
+//   underflow  lost_a and lost_b bound the absolute error that products below 2^-126 have left in A and B: half of 2^-149 a rounding,
+//              times the products that follow.
+// A map is marked where lift or reach is too large, or where more is lost than 2^-24 of the value and than what odd() accepts.
+constexpr float kMostLift = 0x1p22f, kMostState = 0x1p80f, kMostReach = 0x1p102f, kNormal = 0x1p-126f;
+template <int GATE> struct Reach {
+    float lift = 1.f, reach = 0.f, lost_a = 0.f, lost_b = 0.f;
+    // before A and B take the run up; ep: the error of p
+    __device__ __forceinline__ void add(float A, float p, float r, float most, float ep) {
+        lost_b = fmaf(lost_a, fabsf(r), lost_b);
+        reach = fmaf(lift, fabsf(r), reach);
+        if constexpr (GATE == HX_GATE_DECAY) lift = fmaxf(fmaxf(most, 1.f), lift * fabsf(p));   // a sigmoid's is 1
+        lost_a = fmaf(lost_a, fabsf(p), fmaf(fabsf(A), ep, A != 0.f && fabsf(A * p) < kNormal ? 0x1p-150f : 0.f));
+    }
+    __device__ __forceinline__ float mark(float A, float B) const {
+        const bool good = lift < kMostLift && reach < kMostReach && (lost_a <= 0x1p-140f || lost_a <= 0x1p-24f * fabsf(A)) &&
+                          (lost_b <= kNormal || lost_b <= 0x1p-24f * fabsf(B));
+        return good ? A : __int_as_float(0x7fc00000);
+    }
+};
+// The run's error of p where products on the way are below 2^-126: nearly never with decays, and then worth a second look.  A sigmoid's
+// decays are at most 1, so that each rounding counts once.
+template <int GATE> __device__ __forceinline__ float lost_in_run(const float (&a)[kRun], float least) {
+    if (!(least < kNormal)) return 0.f;
+    if constexpr (GATE == HX_GATE_SIGMOID) {
+        return 0x1p-147f;
+    } else {
+        float p = 1.f, lost = 0.f;
+        for (int s = 0; s < kRun; ++s) {
+            const float next = p * a[s];
+            lost = fmaf(lost, fabsf(a[s]), p != 0.f && a[s] != 0.f && fabsf(next) < kNormal ? 0x1p-150f : 0.f);
+            p = next;
+        }
+        return lost;
+    }
+}
+// Takes a run up into A and B.  The run itself is walked as the recurrence goes; BACK: e -> a (v + e) from its last step to its first.
+template <int GATE, bool BACK>
+__device__ __forceinline__ void add_run(const float2 (&a)[kRun], const float2 (&v)[kRun], float2 &A, float2 &B, Reach<GATE> (&reach)[2]) {
+    float2 p, r, least, most;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const int s = BACK ? kRun - 1 - i : i;
+        p = i == 0 ? a[s] : mul2(p, a[s]);
+        if constexpr (BACK) r = mul2(a[s], i == 0 ? v[s] : add2(v[s], r));
+        else r = i == 0 ? v[s] : fma2(a[s], r, v[s]);
+        const float2 size = make_float2(fabsf(p.x), fabsf(p.y));
+        if (i == 0) least = most = size;
+        if constexpr (GATE == HX_GATE_DECAY) {
+            least = make_float2(fminf(least.x, size.x), fminf(least.y, size.y));
+            most = make_float2(fmaxf(most.x, size.x), fmaxf(most.y, size.y));
+        } else {
+            least = size;   // the products of a sigmoid only shrink
+        }
+    }
+    float ax[kRun], ay[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) ax[i] = a[BACK ? kRun - 1 - i : i].x, ay[i] = a[BACK ? kRun - 1 - i : i].y;
+    reach[0].add(A.x, p.x, r.x, most.x, lost_in_run<GATE>(ax, least.x));
+    reach[1].add(A.y, p.y, r.y, most.y, lost_in_run<GATE>(ay, least.y));
+    B = fma2(A, r, B);
+    A = mul2(A, p);
+}
+// A map may not be applied to h, where that gave `next`: it is marked; h is beyond what it is good for, or infinite and A zero, which
+// may be an underflow (infinity over any other A, and NaN, are as in the walk); or A has lost what h would have made larger than both
+// 2^-126 and 2^-24 of the result (A is off by up to 2^-140, or by less than 2^-24 of itself).
+__device__ __forceinline__ bool odd(float A, float h, float next) {
+    const float ah = fabsf(h);
+    if (ah <= 0x1p14f) return A != A;
+    return h == h && (A != A || (ah > kMostState && !(ah > kLargest && A != 0.f)) || (fabsf(A) < 0x1p-116f && ah * 0x1p-116f > fabsf(next)));
+}
+
 // Folds `count` maps onto h, the k-th at `first + k * step`, kFold of them in one round trip to L2 and the next kFold under way.
-// Returns how many are folded: fewer where a map's A or a folded state of one of the warp's channels is not finite.
+// Returns how many are folded: fewer where a map may not be applied for one of the warp's channels.
 constexpr int kFold = 8;
 __device__ __forceinline__ int fold(const float4 *first, int64_t step, int count, bool real, float2 &h) {
     float4 m[2][kFold];
@@ -258,15 +336,26 @@ __device__ __forceinline__ int fold(const float4 *first, int64_t step, int count
             const int at = k0 + half * kFold;
             if (at >= count) break;
             load(m[half ^ 1], at + kFold);
-            float2 next = h;
-            bool odd = false;
+            float2 s = h;
+            bool large = false;   // a marked map leaves NaN, so that nothing is odd where no state is large
 #pragma unroll
             for (int k = 0; k < kFold; ++k) {
-                next = make_float2(fmaf(m[half][k].x, next.x, m[half][k].y), fmaf(m[half][k].z, next.y, m[half][k].w));
-                odd |= !finite(next) || !finite(make_float2(m[half][k].x, m[half][k].z));
+                large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
+                s = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
             }
-            if (__any_sync(0xffffffffu, odd)) return at;
-            h = next;
+            large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
+            if (__any_sync(0xffffffffu, large)) {
+                bool any = false;
+                s = h;
+#pragma unroll
+                for (int k = 0; k < kFold; ++k) {
+                    const float2 next = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
+                    any |= odd(m[half][k].x, s.x, next.x) || odd(m[half][k].z, s.y, next.y);
+                    s = next;
+                }
+                if (__any_sync(0xffffffffu, any)) return at;
+            }
+            h = s;
         }
     return count;
 }
@@ -313,7 +402,8 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
 #pragma unroll
     for (int r = 0; r < STAGES - 1; ++r) issue(r);
 
-    float2 h = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);   // MAP: B and A of the steps walked so far
+    float2 h = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);   // MAP: B and A of the runs walked so far
+    Reach<GATE> reach[2];
     T *out = static_cast<T *>(p.h) + q.b * p.h_batch_stride + q.c;
     const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
     float *states = !MAP && p.states ? p.states + q.b * blocks * p.d_inner + q.c : nullptr;
@@ -362,20 +452,12 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
         issue(r + STAGES - 1);
         const int rows = ragged && r == (MAP ? 0 : runs - 1) ? ragged : kRun;
         if constexpr (MAP) {
-            if (rows == kRun) {
+            if (rows < kRun) {   // steps that are not there: identities
 #pragma unroll
-                for (int s = kRun - 1; s >= 0; --s) {
-                    h = fma2(A, v[s], h);
-                    A = mul2(A, a[s]);
-                }
-            } else {
-#pragma unroll
-                for (int s = kRun - 1; s >= 0; --s)
-                    if (s < rows) {
-                        h = fma2(A, v[s], h);
-                        A = mul2(A, a[s]);
-                    }
+                for (int s = 0; s < kRun; ++s)
+                    if (s >= rows) a[s] = make_float2(1.f, 1.f), v[s] = make_float2(0.f, 0.f);
             }
+            add_run<GATE, false>(a, v, A, h, reach);
         } else {
             if (keep) {
                 if (even && q.n == 2) store2(st, h);
@@ -403,7 +485,7 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
     }
     if constexpr (MAP) {
         chain_wait();   // the launch before this one has read the maps of its span
-        if (q.n) *map_at(maps, q.seg, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, h.x, A.y, h.y);
+        if (q.n) *map_at(maps, q.seg, q.b, q.c, p.batch, p.d_inner) = make_float4(reach[0].mark(A.x, h.x), h.x, reach[1].mark(A.y, h.y), h.y);
     } else {
         const int64_t end = q.seg == segs - 1 ? span.end : min(span.begin + (int64_t)(q.seg + 1) * seg_len, (int64_t)span.end);
         for (int64_t t = max(span.begin + (int64_t)q.seg * seg_len, (int64_t)q.len); t < end; ++t) store_some(out + t * p.h_row_stride, make_float2(0.f, 0.f), q.n);
@@ -461,6 +543,7 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
 
     if constexpr (MAP) {
         float2 E = make_float2(0.f, 0.f), A = make_float2(1.f, 1.f);
+        Reach<GATE> reach[2];
         for (int r = 0; r < runs; ++r) {
             cp_wait<STAGES - 2>();
             __syncwarp();
@@ -477,20 +560,12 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
             if (ragged && r == runs - 1) {
 #pragma unroll
                 for (int s = 0; s < kRun; ++s)
-                    if (s < ragged) {
-                        A = mul2(A, a[s]);
-                        E = fma2(A, v[s], E);
-                    }
-            } else {
-#pragma unroll
-                for (int s = 0; s < kRun; ++s) {
-                    A = mul2(A, a[s]);
-                    E = fma2(A, v[s], E);
-                }
+                    if (s >= ragged) a[s] = make_float2(1.f, 1.f), v[s] = make_float2(0.f, 0.f);
             }
+            add_run<GATE, true>(a, v, A, E, reach);
         }
         chain_wait();   // the launch before this one has read the maps of its span
-        if (q.n) *map_at(maps, q.seg - 1, q.b, q.c, p.batch, p.d_inner) = make_float4(A.x, E.x, A.y, E.y);
+        if (q.n) *map_at(maps, q.seg - 1, q.b, q.c, p.batch, p.d_inner) = make_float4(reach[0].mark(A.x, E.x), E.x, reach[1].mark(A.y, E.y), E.y);
     } else {
         const int64_t blocks = ((int64_t)p.seq_len + kBlock - 1) / kBlock;
         const bool even = p.d_inner % 2 == 0 && (uintptr_t)p.states % 8 == 0;   // two states at a time

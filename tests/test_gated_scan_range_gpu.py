@@ -1,0 +1,258 @@
+"""The gated recurrence and its gradients over sequences that are cut into segments, where numbers leave the format or come near its
+ends.  A call without a workspace walks the steps one by one and is what the cut call has to agree with: infinities and NaN exactly,
+other numbers within the bound of either one's rounding.
+
+Tolerances.  u = 2^-24; M_t = |a_t| M_{t-1} + |v_t| and W_t = |a_t| (W_{t-1} + M_{t-1}) as in test_gated_scan_gpu.py, where each way
+of associating the sums is within 16 u W_t + 64 u M_t of the exact value, so two ways are within twice that of one another.  Where a
+segment hands its state on, numbers below 2^-126 may be taken as zero: 2^-126 a segment, of which an input meets at most 128, so
+2^-119 in all.  bf16 results add their own rounding, 2^-8 of the value on either side."""
+import pytest
+import torch
+
+from helixml_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+INF, NAN = float("inf"), float("nan")
+TILE = 64        # channels that one warp owns: every special channel gets a tile of its own, with ordinary neighbours
+
+
+def walked(monkeypatch, call):
+    with monkeypatch.context() as m:
+        m.setattr(ops, "_gated_scan_workspace", lambda *a: None)
+        return call()
+
+
+def bound(a, v, start, reverse=False):
+    """2 (16 u W + 64 u M) + 2^-119 for every row, and behind the last one, in 64 bits."""
+    a, v = a.double().abs().nan_to_num(0, 0, 0), v.double().abs().nan_to_num(0, 0, 0)
+    m, w = start.double().abs().nan_to_num(0, 0, 0), torch.zeros_like(start, dtype=torch.float64)
+    rows = []
+    for t in (range(a.shape[1] - 1, -1, -1) if reverse else range(a.shape[1])):
+        if reverse:      # delta_t = dh_t + e_{t+1}, e_t = a_t delta_t
+            m = m + v[:, t]
+            rows.append(32 * U * w + 128 * U * m)
+            w, m = a[:, t] * (w + m), a[:, t] * m
+        else:
+            w = a[:, t] * (w + m)
+            m = a[:, t] * m + v[:, t]
+            rows.append(32 * U * w + 128 * U * m)
+    rows = torch.stack(rows[::-1] if reverse else rows, 1)
+    return rows + 2.0 ** -119, 32 * U * w + 128 * U * m + 2.0 ** -119
+
+
+def agree(got, want, tol, what):
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    assert torch.equal(torch.isinf(got), torch.isinf(want)), what
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]), what
+    ok = torch.isfinite(want)
+    eps = 0.0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps
+    err = (got.double() - want.double()).abs() - tol * (1 + eps) - eps * want.double().abs()
+    assert not (err[ok] > 0).any(), (what, err[ok].max().item())
+
+
+def decay_cases(L):
+    """name -> function that edits one channel's (a, v, h0) in place; 1-d tensors over time and a number."""
+    def two_large(a, v):
+        v[650] = v[651] = 3e38                       # overflows in the middle of a segment
+
+    def late_large(a, v):
+        v[L - 300], v[L - 299], a[L - 299] = 3e38, 3e38, 1.0
+
+    def large_then_halves(a, v):
+        a[:], v[:] = 0.5, 0.0
+        v[100] = 1e30                                # 160 halvings later 6.8e-19
+
+    def halves_of_start(a, v):
+        a[:], v[:] = 0.5, 0.0
+        return 1e30
+
+    def grows_over_zero(a, v):
+        a[:] = 2.0
+        v[:L - 100] = 0.0                            # the products overflow, the state is zero
+
+    def there_and_back(a, v):
+        a[:], v[:] = 1.0, 0.0
+        a[3:43], a[43:83] = 2.0, 0.5                 # 1e30 2^40 is infinite, the product of the decays is one
+        return 1e30
+
+    def shrinks_after_growth(a, v):
+        a[:], v[:] = 1.0, 0.0
+        a[10], a[20], a[21], a[500] = 1e20, 1e-25, 1e-25, 1e20   # 1e10 -> 1e30 -> 1e-20 -> 1; the products alone underflow
+        return 1e10
+
+    def grows_after_shrinking(a, v):
+        a[:], v[:] = 1.0, 0.0
+        a[10], a[20], a[21], a[30] = 1e-20, 1e-20, 1e20, 1e20    # 1 -> 1e-40 -> 1
+        return 1e3
+
+    def forgets(a, v):
+        v[5], a[40] = 1e37, 0.0
+
+    def infinite(a, v):
+        a[:] = 0.5
+        v[7] = INF
+
+    def infinite_forgotten(a, v):
+        v[7], a[900] = -INF, 0.0
+
+    def not_a_number(a, v):
+        v[300] = NAN
+
+    def gate_not_a_number(a, v):
+        a[1000] = NAN
+
+    def infinite_gate(a, v):
+        a[100] = INF
+        v[:101] = 0.0
+
+    def large_and_steady(a, v):
+        v *= 1e36
+
+    def over_the_largest(a, v):
+        v *= 8e37                                    # sums that overflow now and then
+
+    def alternates(a, v):
+        a[::2], a[1::2] = -1.0, 1.0
+
+    def small(a, v):
+        v *= 1e-36
+
+    def wild(a, v):
+        a.copy_(torch.randn(L, generator=torch.Generator().manual_seed(9)))
+
+    def sparse(a, v):
+        keep = v[::700].clone()
+        a[:], v[:] = 0.4, 0.0
+        v[::700] = keep * 1e20
+
+    return {f.__name__: f for f in (two_large, late_large, large_then_halves, halves_of_start, grows_over_zero, there_and_back,
+                                    shrinks_after_growth, grows_after_shrinking, forgets, infinite, infinite_forgotten, not_a_number,
+                                    gate_not_a_number, infinite_gate, large_and_steady, over_the_largest, alternates, small, wild, sparse)}
+
+
+def decay_inputs(B, L, dtype, reverse):
+    """a, v and the start; the case of tile k is in its third channel.  reverse: as the recurrence from the end meets them."""
+    cases = decay_cases(L)
+    D = TILE * (len(cases) + 1)
+    gen = torch.Generator().manual_seed(L)
+    a, v = 0.2 + 0.7 * torch.rand(B, L, D, generator=gen), torch.randn(B, L, D, generator=gen)
+    start = torch.randn(B, D, generator=gen)
+    for k, f in enumerate(cases.values()):
+        at, vt = a[0, :, TILE * k + 2].clone(), v[0, :, TILE * k + 2].clone()
+        s = f(at, vt)
+        start[0, TILE * k + 2] = 0.0 if s is None else s
+        a[0, :, TILE * k + 2], v[0, :, TILE * k + 2] = at, vt
+    if reverse:
+        a, v = a.flip(1), v.flip(1)
+    return a.to(DT[dtype]).cuda(), v.to(DT[dtype]).cuda(), start.cuda()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,lengths", [(1, 4096, None), (2, 4096, [4000, 1733]), (4, 4001, None)])
+def test_decays_forward(B, L, lengths, dtype, monkeypatch):
+    a, v, h0 = decay_inputs(B, L, dtype, False)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+    def call():
+        st = ops.gated_scan_states(B, L, a.shape[2])
+        st.zero_()   # rows of blocks behind a length are not written
+        return *ops.gated_scan(v, a, h0=h0, gate="decay", lengths=n, return_state=True, states=st), st
+
+    (h, last, st), (want, want_last, want_st) = call(), walked(monkeypatch, call)
+    if lengths is not None:
+        inside = (torch.arange(L, device="cuda")[None] < n[:, None])[:, :, None]
+        a, v = torch.where(inside, a, 1.0), torch.where(inside, v, 0.0)
+    tol, last_tol = bound(a, v, h0)
+    agree(h, want, tol, "h")
+    agree(last, want_last, last_tol, "h_last")
+    before = torch.cat([torch.full_like(tol[:, :1], 2.0 ** -119), tol[:, :-1]], 1)[:, ::16]
+    agree(st, want_st, before, "states")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,lengths", [(1, 4096, None), (2, 4096, [4096, 1733]), (4, 4001, None)])
+def test_decays_backward(B, L, lengths, dtype, monkeypatch):
+    a, dh, dh_last = decay_inputs(B, L, dtype, True)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    x = torch.randn(B, L, a.shape[2], generator=torch.Generator().manual_seed(1)).to(DT[dtype]).cuda()
+    st = ops.gated_scan_states(B, L, a.shape[2])
+    walked(monkeypatch, lambda: ops.gated_scan(x, a, gate="decay", lengths=n, states=st))
+    call = lambda: ops.gated_scan_bwd(dh, x, a, st, gate="decay", lengths=n, dh_last=dh_last)
+    (dx, dg, dh0), (want, want_dg, want0) = call(), walked(monkeypatch, call)
+    if lengths is not None:
+        inside = (torch.arange(L, device="cuda")[None] < n[:, None])[:, :, None]
+        a, dh = torch.where(inside, a, 1.0), torch.where(inside, dh, 0.0)
+    tol, tol0 = bound(a, dh, dh_last, reverse=True)
+    agree(dx, want, tol, "dx")
+    agree(dh0, want0, tol0, "dh0")
+    for same in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(same(dg), same(want_dg))
+
+
+def sigmoid_inputs(B, L, dtype):
+    D = TILE * 8
+    gen = torch.Generator().manual_seed(L)
+    g, x, h0 = torch.randn(B, L, D, generator=gen), torch.randn(B, L, D, generator=gen), torch.randn(B, D, generator=gen)
+    c = lambda k: TILE * k + 2
+    g[0, :, c(0)], x[0, :, c(0)], h0[0, c(0)] = 0.0, 0.0, 1e30         # halves of a large start
+    g[0, :, c(1)], x[0, :, c(1)], x[0, 100, c(1)] = 0.0, 0.0, 1e30     # of a large input
+    x[0, 200, c(2)] = INF
+    x[0, 333, c(3)] = NAN
+    g[0, 333, c(4)] = NAN
+    g[0, :, c(5)] = -30.0                                              # forgets everything within a step
+    x[0, 500, c(5)], h0[0, c(5)] = 1e37, 1e37
+    x[0, :, c(6)] *= 8e36
+    return g.to(DT[dtype]).cuda(), x.to(DT[dtype]).cuda(), h0.cuda()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L", [(1, 5000), (4, 4096)])
+def test_sigmoid(B, L, dtype, monkeypatch):
+    g, x, h0 = sigmoid_inputs(B, L, dtype)
+    call = lambda: ops.gated_scan(x, g, h0=h0, return_state=True)
+    (h, last), (want, want_last) = call(), walked(monkeypatch, call)
+    tol, last_tol = bound(torch.sigmoid(g.double()), torch.sigmoid(-g.double()) * x.double(), h0)
+    agree(h, want, tol, "h")
+    agree(last, want_last, last_tol, "h_last")
+    # the same numbers as gradients
+    st = ops.gated_scan_states(B, L, g.shape[2])
+    ones = torch.ones_like(x)
+    walked(monkeypatch, lambda: ops.gated_scan(ones, g, states=st))
+    call = lambda: ops.gated_scan_bwd(x.flip(1).contiguous(), ones, g, st, dh_last=h0)
+    (dx, dg, dh0), (want, want_dg, want0) = call(), walked(monkeypatch, call)
+    tol, tol0 = bound(torch.sigmoid(g.double()), x.flip(1), h0, reverse=True)
+    agree(dx, want, tol, "dx")
+    agree(dh0, want0, tol0, "dh0")
+    for same in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(same(dg), same(want_dg))
+
+
+def test_across_spans(monkeypatch):
+    """Inputs beyond the cache go span by span; the cases lie in the first and the last of them."""
+    L, D = 24000, 1024
+    gen = torch.Generator().manual_seed(5)
+    a, v = 0.2 + 0.7 * torch.rand(1, L, D, generator=gen), torch.randn(1, L, D, generator=gen)
+    h0 = torch.randn(1, D, generator=gen)
+    c = lambda k: TILE * k + 2
+    a[0, :, c(0)], v[0, :, c(0)], h0[0, c(0)] = 0.999, 0.0, 1e30
+    v[0, 650, c(1)] = v[0, 651, c(1)] = v[0, L - 651, c(2)] = v[0, L - 650, c(2)] = 3e38
+    a[0, :, c(3)], v[0, :, c(3)], v[0, L - 4000, c(3)] = 0.5, 0.0, 1e30
+    a[0, :, c(4)], v[0, :L - 90, c(4)], h0[0, c(4)] = 2.0, 0.0, 0.0
+    a, v, h0 = a.cuda(), v.cuda(), h0.cuda()
+    call = lambda: ops.gated_scan(v, a, h0=h0, gate="decay", return_state=True)
+    (h, last), (want, want_last) = call(), walked(monkeypatch, call)
+    assert torch.isinf(want[0, -1, [c(1), c(2)]]).all() and want[0, L - 3900, c(3)] != 0
+    tol, last_tol = bound(a, v, h0)
+    agree(h, want, tol, "h")
+    agree(last, want_last, last_tol, "h_last")
+    st = ops.gated_scan_states(1, L, D)
+    ones = torch.ones_like(v)
+    walked(monkeypatch, lambda: ops.gated_scan(ones, a, gate="decay", states=st))
+    call = lambda: ops.gated_scan_bwd(v, ones, a, st, gate="decay", dh_last=h0)
+    (dx, _, dh0), (want, _, want0) = call(), walked(monkeypatch, call)
+    tol, tol0 = bound(a, v, h0, reverse=True)
+    agree(dx, want, tol, "dx")
+    agree(dh0, want0, tol0, "dh0")
