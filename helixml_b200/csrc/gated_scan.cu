@@ -249,10 +249,11 @@ __device__ __forceinline__ float4 *map_at(float2 *maps, int seg, int b, int c, i
 //   overflow   A walk of the run from 0 that overflows leaves r, and then B, infinite or NaN.  What a state entering the run adds to it
 //              is at most lift |h| from before the segment and `reach` from its own runs; where both are below 2^102, half the last
 //              place of the largest number and less, the walk from h overflows where that from 0 does.
-//   underflow  lost_a and lost_b bound the absolute error that products below 2^-126 have left in A and B: half of 2^-149 a rounding,
-//              times the products that follow.
+//   underflow  lost_a and lost_b bound the absolute error that products below 2^-126 have left in A and B: 2^-149 a rounding, times
+//              the products that follow.  They are kept times 2^100, so that a bound does not underflow itself before the largest
+//              run result (2^102) makes less than 2^-126 of it.
 // A map is marked where lift or reach is too large, or where more is lost than 2^-24 of the value and than what odd() accepts.
-constexpr float kMostLift = 0x1p22f, kMostState = 0x1p80f, kMostReach = 0x1p102f, kNormal = 0x1p-126f;
+constexpr float kMostLift = 0x1p22f, kMostState = 0x1p80f, kMostReach = 0x1p102f, kNormal = 0x1p-126f, kStep = 0x1p-49f;   // 2^-149
 template <int GATE> struct Reach {
     float lift = 1.f, reach = 0.f, lost_a = 0.f, lost_b = 0.f;
     // before A and B take the run up; ep: the error of p
@@ -260,25 +261,25 @@ template <int GATE> struct Reach {
         lost_b = fmaf(lost_a, fabsf(r), lost_b);
         reach = fmaf(lift, fabsf(r), reach);
         if constexpr (GATE == HX_GATE_DECAY) lift = fmaxf(fmaxf(most, 1.f), lift * fabsf(p));   // a sigmoid's is 1
-        lost_a = fmaf(lost_a, fabsf(p), fmaf(fabsf(A), ep, A != 0.f && fabsf(A * p) < kNormal ? 0x1p-150f : 0.f));
+        lost_a = fmaf(lost_a, fabsf(p), fmaf(fabsf(A), ep, A != 0.f && fabsf(A * p) < kNormal ? kStep : 0.f));
     }
     __device__ __forceinline__ float mark(float A, float B) const {
-        const bool good = lift < kMostLift && reach < kMostReach && (lost_a <= 0x1p-140f || lost_a <= 0x1p-24f * fabsf(A)) &&
-                          (lost_b <= kNormal || lost_b <= 0x1p-24f * fabsf(B));
+        const bool good = lift < kMostLift && reach < kMostReach && (lost_a <= 0x1p-40f || lost_a <= 0x1p76f * fabsf(A)) &&
+                          (lost_b <= 0x1p-26f || lost_b <= 0x1p76f * fabsf(B));
         return good ? A : __int_as_float(0x7fc00000);
     }
 };
-// The run's error of p where products on the way are below 2^-126: nearly never with decays, and then worth a second look.  A sigmoid's
-// decays are at most 1, so that each rounding counts once.
-template <int GATE> __device__ __forceinline__ float lost_in_run(const float (&a)[kRun], float least) {
-    if (!(least < kNormal)) return 0.f;
+// The run's error of p where products on the way are below 2^-126: nearly never with decays, and then worth a second look, unless A is
+// zero already.  A sigmoid's decays are at most 1, so that each rounding counts once.
+template <int GATE> __device__ __forceinline__ float lost_in_run(const float (&a)[kRun], float least, float A) {
+    if (!(least < kNormal) || A == 0.f) return 0.f;
     if constexpr (GATE == HX_GATE_SIGMOID) {
-        return 0x1p-147f;
+        return kRun * kStep;
     } else {
         float p = 1.f, lost = 0.f;
         for (int s = 0; s < kRun; ++s) {
             const float next = p * a[s];
-            lost = fmaf(lost, fabsf(a[s]), p != 0.f && a[s] != 0.f && fabsf(next) < kNormal ? 0x1p-150f : 0.f);
+            lost = fmaf(lost, fabsf(a[s]), p != 0.f && a[s] != 0.f && fabsf(next) < kNormal ? kStep : 0.f);
             p = next;
         }
         return lost;
@@ -306,8 +307,8 @@ __device__ __forceinline__ void add_run(const float2 (&a)[kRun], const float2 (&
     float ax[kRun], ay[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) ax[i] = a[BACK ? kRun - 1 - i : i].x, ay[i] = a[BACK ? kRun - 1 - i : i].y;
-    reach[0].add(A.x, p.x, r.x, most.x, lost_in_run<GATE>(ax, least.x));
-    reach[1].add(A.y, p.y, r.y, most.y, lost_in_run<GATE>(ay, least.y));
+    reach[0].add(A.x, p.x, r.x, most.x, lost_in_run<GATE>(ax, least.x, A.x));
+    reach[1].add(A.y, p.y, r.y, most.y, lost_in_run<GATE>(ay, least.y, A.y));
     B = fma2(A, r, B);
     A = mul2(A, p);
 }
