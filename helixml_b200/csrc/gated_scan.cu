@@ -7,7 +7,7 @@
 // h -> A h + B (A the product of its decays, B its result from zero), a first launch writes the map of every segment but the last,
 // and the second folds the maps before its segment onto h0 and walks the segment with outputs.  That reads x and g twice, the second
 // time from L2 as far as they fit: the first launch walks every segment from its end (a map can be built from either side), so what
-// it read last is what the second needs first.  The order of the sums is a function of the shape alone.
+// it read last is what the second needs first.  The order of a channel's sums is a function of the shape and of its own numbers.
 // The backward pass is the same recurrence from the end, e_t = a_t (dh_t + e_{t+1}); h_{t-1} is recomputed from the state that the
 // forward pass saved every 16 steps, so h itself, rounded to the io type, is not needed.
 //
@@ -15,7 +15,7 @@
 // when its steps are walked, but a map knows the ends of a segment only, and what overflowed may have decayed by then; a product of
 // decays that underflows has lost what a large state, or growth before it, would have made of it.  So the first launch also bounds how
 // far a state can get within a segment and what its products have lost, marks a map that cannot stand for the walk (A is NaN), and the
-// warp walks the steps from there to its segment where it meets such a map or a state that the map is not made for (Reach, odd).
+// segment is walked instead, for the channels that meet such a map or a state that the map is not made for (Reach, odd).
 #include <algorithm>
 #include <initializer_list>
 
@@ -321,10 +321,12 @@ __device__ __forceinline__ bool odd(float A, float h, float next) {
     return h == h && (A != A || (ah > kMostState && !(ah > kLargest && A != 0.f)) || (fabsf(A) < 0x1p-116f && ah * 0x1p-116f > fabsf(next)));
 }
 
-// Folds `count` maps onto h, the k-th at `first + k * step`, kFold of them in one round trip to L2 and the next kFold under way.
-// Returns how many are folded: fewer where a map may not be applied for one of the warp's channels.
+// Folds `count` maps onto h, the k-th at `first + k * step`, kFold of them in one round trip to L2 and the next kFold under way.  Where
+// one may not be applied, its channel takes what walk(k, h), the walk of the k-th map's segment from h, gives instead.  A channel's
+// result depends on its own numbers alone, whatever the other channels of the warp hold.
 constexpr int kFold = 8;
-__device__ __forceinline__ int fold(const float4 *first, int64_t step, int count, bool real, float2 &h) {
+template <typename Walk>
+__device__ __forceinline__ void fold(const float4 *first, int64_t step, int count, bool real, float2 &h, Walk walk) {
     float4 m[2][kFold];
     auto load = [&](float4 (&b)[kFold], int k0) {
 #pragma unroll
@@ -354,11 +356,22 @@ __device__ __forceinline__ int fold(const float4 *first, int64_t step, int count
                     any |= odd(m[half][k].x, s.x, next.x) || odd(m[half][k].z, s.y, next.y);
                     s = next;
                 }
-                if (__any_sync(0xffffffffu, any)) return at;
+                if (__any_sync(0xffffffffu, any)) {   // one by one
+                    s = h;
+                    for (int k = at; k < min(at + kFold, count); ++k) {
+                        const float4 one = real ? __ldcg(first + k * step) : make_float4(1.f, 0.f, 1.f, 0.f);
+                        float2 next = make_float2(fmaf(one.x, s.x, one.y), fmaf(one.z, s.y, one.w));
+                        const bool x = odd(one.x, s.x, next.x), y = odd(one.z, s.y, next.y);
+                        if (__any_sync(0xffffffffu, x || y)) {
+                            const float2 w = walk(k, s);
+                            next = make_float2(x ? w.x : next.x, y ? w.y : next.y);
+                        }
+                        s = next;
+                    }
+                }
             }
             h = s;
         }
-    return count;
 }
 
 // ---------------------------------------------------------------- forward
@@ -415,24 +428,26 @@ gated_scan_kernel(const hx_gated_scan_args p, const Span span, float2 *maps, int
         if (span.in) h = load_carry(span.in + (int64_t)q.b * p.d_inner + q.c, q.n);
         if (segs > 1) {
             const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
-            const int j = fold(map_at(maps, 0, q.b, q.c, p.batch, p.d_inner), step, q.seg, q.n > 0, h);
-            if (j < q.seg)   // h is the state before segment j: walk on from there
-                for (int64_t t = span.begin + (int64_t)j * seg_len; t < q.t0; t += kRun) {
+            fold(map_at(maps, 0, q.b, q.c, p.batch, p.d_inner), step, q.seg, q.n > 0, h, [&](int j, float2 h) {
+                const int64_t end = min(span.begin + (int64_t)(j + 1) * seg_len, (int64_t)q.end);
+                for (int64_t t = span.begin + (int64_t)j * seg_len; t < end; t += kRun) {
                     float2 gv[kRun], xv[kRun];
 #pragma unroll
                     for (int s = 0; s < kRun; ++s) {
-                        const int n = t + s < q.t0 ? q.n : 0;
+                        const int n = t + s < end ? q.n : 0;
                         gv[s] = load_some(g + (t + s) * p.g_row_stride + 2 * q.lane, n);
                         xv[s] = load_some(x + (t + s) * p.x_row_stride + 2 * q.lane, n);
                     }
 #pragma unroll
                     for (int s = 0; s < kRun; ++s)
-                        if (t + s < q.t0) {
+                        if (t + s < end) {
                             float2 a, b, rest;
                             gate_step<GATE, FAST>(gv[s], xv[s], a, b, rest);
                             h = fma2(a, h, b);
                         }
                 }
+                return h;
+            });
         }
     }
     const T *slot_g = &ring[0][0][0][2 * q.lane], *const slot_end = slot_g + STAGES * 2 * kRun * P;
@@ -580,26 +595,26 @@ gated_scan_bwd_kernel(const hx_gated_scan_bwd_args p, const Span span, float2 *m
         float2 e = span.in ? load_carry(span.in + (int64_t)q.b * p.d_inner + q.c, q.n) : make_float2(0.f, 0.f);
         if (segs > 1) {
             const int64_t step = map_at(maps, 1, 0, 0, p.batch, p.d_inner) - map_at(maps, 0, 0, 0, p.batch, p.d_inner);
-            const int count = segs - 1 - q.seg;
-            const int folded = fold(map_at(maps, segs - 2, q.b, q.c, p.batch, p.d_inner), -step, count, q.n > 0, e);
-            const int j = segs - 1 - folded;
-            if (folded < count)   // e is the one behind segment j
-                for (int64_t t = min(span.begin + (int64_t)(j + 1) * seg_len, (int64_t)q.end) - 1; t >= q.t1; t -= kRun) {
+            fold(map_at(maps, segs - 2, q.b, q.c, p.batch, p.d_inner), -step, segs - 1 - q.seg, q.n > 0, e, [&](int k, float2 e) {
+                const int64_t begin = span.begin + (int64_t)(segs - 1 - k) * seg_len;   // of the k-th segment from the end
+                for (int64_t t = min(begin + seg_len, (int64_t)q.end) - 1; t >= begin; t -= kRun) {
                     float2 gv[kRun], dv[kRun];
 #pragma unroll
                     for (int s = 0; s < kRun; ++s) {
-                        const int n = t - s >= q.t1 ? q.n : 0;
+                        const int n = t - s >= begin ? q.n : 0;
                         gv[s] = load_some(g + (t - s) * p.g_row_stride + 2 * q.lane, n);
                         dv[s] = load_some(dh + (t - s) * p.dh_row_stride + 2 * q.lane, n);
                     }
 #pragma unroll
                     for (int s = 0; s < kRun; ++s)
-                        if (t - s >= q.t1) {
+                        if (t - s >= begin) {
                             float2 a, b, rest;
                             gate_step<GATE, FAST>(gv[s], dv[s], a, b, rest);
                             e = mul2(a, add2(e, dv[s]));
                         }
                 }
+                return e;
+            });
         }
         const bool whole = PIECE >= 2 * (int)sizeof(T) && q.n == 2;
         T *dx = static_cast<T *>(p.dx) + q.b * p.dx_batch_stride + q.c;

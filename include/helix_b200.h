@@ -305,9 +305,10 @@ HX_API hx_status hx_s4_diag_fwd(const void *u, const float *A, const float *Bp, 
  *   HX_GATE_DECAY     a_t = g[b,t,d]              h_t = a_t h_{t-1} + x[b,t,d]
  *   HX_GATE_SIGMOID   a_t = 1 / (1 + exp(-g))     h_t = a_t h_{t-1} + (1 - a_t) x[b,t,d]
  * h_{-1} = h0[b,d] (zero without h0).  State and arithmetic are fp32 whatever io_dtype is.  A decay may have any sign; sums
- * are associated over time in an order of the kernel's own (the same for every call of one shape), so with |a| > 1 rounding
- * grows as it does in any order.  Infinities and NaN, of the inputs or where sums of finite ones leave the format, are those of the
- * sequential recurrence, and so are numbers near the format's ends, but that a state below 2^-126 may be taken as zero.
+ * are associated over time in an order of the kernel's own (a function of the shape and of the channel's own numbers), so with
+ * |a| > 1 rounding grows as it does in any order.  Infinities and NaN, of the inputs or where sums of finite ones leave the
+ * format, are those of the sequential recurrence, and so are numbers near the format's ends, but that a state below 2^-126 may
+ * be taken as zero.
  *   lengths (int32 [batch] on the device, or NULL for seq_len everywhere; values are clamped to 0 .. seq_len): rows of a
  *   padded batch from len[b] on are not read as numbers (they may hold anything), their outputs are zeros, and h_last is the
  *   state after row len[b] - 1 (h0 where len[b] is 0).

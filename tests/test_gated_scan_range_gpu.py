@@ -256,3 +256,31 @@ def test_across_spans(monkeypatch):
     tol, tol0 = bound(a, v, h0, reverse=True)
     agree(dx, want, tol, "dx")
     agree(dh0, want0, tol0, "dh0")
+
+
+@pytest.mark.parametrize("gate", ["decay", "sigmoid"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_channel_does_not_depend_on_its_neighbours(dtype, gate):
+    """Infinities, NaN and numbers that leave the format in some channels of a tile leave every bit of the others as it was."""
+    B, L, D = 2, 3000, 130
+    gen = torch.Generator().manual_seed(8)
+    x, g, dh = (torch.randn(B, L, D, generator=gen) for _ in range(3))
+    if gate == "decay":
+        g = 0.9 + 0.1 * torch.rand(B, L, D, generator=gen)
+    h0, dh_last = torch.randn(B, D, generator=gen).cuda(), torch.randn(B, D, generator=gen).cuda()
+
+    def call(x, g, dh):
+        x, g, dh = (t.to(DT[dtype]).cuda() for t in (x, g, dh))
+        st = ops.gated_scan_states(B, L, D)
+        h, last = ops.gated_scan(x, g, h0=h0, gate=gate, states=st, return_state=True)
+        return h, last, st, *ops.gated_scan_bwd(dh, x, g, st, gate=gate, dh_last=dh_last)
+
+    want = call(x, g, dh)
+    bad = [5, 36, 127]
+    x[0, 9, 5], x[0, 1500, 36], x[1, 300, 127] = INF, NAN, -INF
+    dh[0, 2990, 5], dh[0, 1500, 36], dh[1, 2000, 127] = -INF, NAN, INF
+    x[1, 700:702, 5] = dh[1, 2000:2002, 5] = 3e38
+    others = [c for c in range(D) if c not in bad]
+    for name, got, w in zip(("h", "h_last", "states", "dx", "dg", "dh0"), call(x, g, dh), want):
+        assert torch.equal(got[..., others], w[..., others]), name
+        assert not torch.equal(got[..., bad], w[..., bad]), name
