@@ -332,46 +332,51 @@ __device__ __forceinline__ void fold(const float4 *first, int64_t step, int coun
 #pragma unroll
         for (int k = 0; k < kFold; ++k) b[k] = k0 + k < count && real ? __ldcg(first + (k0 + k) * step) : make_float4(1.f, 0.f, 1.f, 0.f);
     };
-    load(m[0], 0);
-    for (int k0 = 0; k0 < count; k0 += 2 * kFold)
+    int done = 0;
+    auto fast = [&]() {   // until all are folded, or up to eight of which one may not be
+        load(m[0], done);
+        while (true)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int at = k0 + half * kFold;
-            if (at >= count) break;
-            load(m[half ^ 1], at + kFold);
-            float2 s = h;
-            bool large = false;   // a marked map leaves NaN, so that nothing is odd where no state is large
-#pragma unroll
-            for (int k = 0; k < kFold; ++k) {
-                large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
-                s = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
-            }
-            large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
-            if (__any_sync(0xffffffffu, large)) {
-                bool any = false;
-                s = h;
+            for (int half = 0; half < 2; ++half) {
+                if (done >= count) return;
+                load(m[half ^ 1], done + kFold);
+                float2 s = h;
+                bool large = false;   // a marked map leaves NaN, so that nothing is odd where no state is large
 #pragma unroll
                 for (int k = 0; k < kFold; ++k) {
-                    const float2 next = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
-                    any |= odd(m[half][k].x, s.x, next.x) || odd(m[half][k].z, s.y, next.y);
-                    s = next;
+                    large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
+                    s = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
                 }
-                if (__any_sync(0xffffffffu, any)) {   // one by one
+                large |= !(fabsf(s.x) <= 0x1p14f) || !(fabsf(s.y) <= 0x1p14f);
+                if (__any_sync(0xffffffffu, large)) {
+                    bool any = false;
                     s = h;
-                    for (int k = at; k < min(at + kFold, count); ++k) {
-                        const float4 one = real ? __ldcg(first + k * step) : make_float4(1.f, 0.f, 1.f, 0.f);
-                        float2 next = make_float2(fmaf(one.x, s.x, one.y), fmaf(one.z, s.y, one.w));
-                        const bool x = odd(one.x, s.x, next.x), y = odd(one.z, s.y, next.y);
-                        if (__any_sync(0xffffffffu, x || y)) {
-                            const float2 w = walk(k, s);
-                            next = make_float2(x ? w.x : next.x, y ? w.y : next.y);
-                        }
+#pragma unroll
+                    for (int k = 0; k < kFold; ++k) {
+                        const float2 next = make_float2(fmaf(m[half][k].x, s.x, m[half][k].y), fmaf(m[half][k].z, s.y, m[half][k].w));
+                        any |= odd(m[half][k].x, s.x, next.x) || odd(m[half][k].z, s.y, next.y);
                         s = next;
                     }
+                    if (__any_sync(0xffffffffu, any)) return;
                 }
+                h = s;
+                done += kFold;
             }
-            h = s;
+    };
+    while (true) {
+        fast();
+        if (done >= count) return;
+        for (const int end = min(done + kFold, count); done < end; ++done) {   // one by one
+            const float4 one = real ? __ldcg(first + done * step) : make_float4(1.f, 0.f, 1.f, 0.f);
+            float2 next = make_float2(fmaf(one.x, h.x, one.y), fmaf(one.z, h.y, one.w));
+            const bool x = odd(one.x, h.x, next.x), y = odd(one.z, h.y, next.y);
+            if (__any_sync(0xffffffffu, x || y)) {
+                const float2 w = walk(done, h);
+                next = make_float2(x ? w.x : next.x, y ? w.y : next.y);
+            }
+            h = next;
         }
+    }
 }
 
 // ---------------------------------------------------------------- forward
