@@ -160,22 +160,29 @@ template <typename T> __device__ __forceinline__ void store_some(T *p, float2 v,
     if (n > 1) st_f32(p + 1, v.y);
 }
 
-// A pair of gates -> decays a = sigmoid(g) and 1 - a, both to full relative precision: with e = exp(-g), a = 1 / (1 + e) and
-// 1 - a = e a, neither of which cancels.  e is held to about 2^126, where a is the smallest normal number and 1 - a comes out as 1;
-// taking 2^-126 off a makes it the zero it should be there and is below the rounding of any a that matters.  A NaN goes through.
-// FAST, for bf16 results: one exp2 and one reciprocal of the special-function unit, off by (|g| + 9) 2^-24, far below 2^-9.
+// A pair of gates -> decays a = sigmoid(g) and 1 - a, both good relative to themselves: with e = exp(-g), a = 1 / (1 + e) and
+// 1 - a = e a, neither of which cancels.  e is held to about 2^126, where 1 - a comes out as 1 and a, which would be the smallest normal
+// number there and below it behind, is set to zero.  A NaN goes through.
+// FAST, for bf16 tensors: one exp2 and one reciprocal of the special-function unit, a off by at most (|g| + 9) 2^-24 of itself, 4 2^-24
+// where it is near one (e's error counts for e / (1 + e) of itself).  Along a memory of 1 / (1 - a) steps that adds up to
+// 4 2^-24 / (1 - a) of h, where rounding an exact a would leave 2^-24 / (1 - a): at g = 10 some 5e-3 and 1.3e-3.  The step takes the
+// other form for every type, and so may differ from the same row of a scan by as much.
 // Otherwise e = 2^t (1 + (t' - t) ln 2), t the rounded and t' the exact product -g log2(e), and one Newton step on the reciprocal.
 template <bool FAST> __device__ __forceinline__ void sigmoid2(float2 g, float2 &a, float2 &rest) {
-    float2 e;
+    float2 e, end;   // end: 1 where e is held
     if constexpr (FAST) {
         float2 t = mul2(g, make_float2(-kLog2e, -kLog2e));
         asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.x));   // 126
         asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.y));
+        asm("set.ge.f32.f32 %0, %1, 0f42FC0000;" : "=f"(end.x) : "f"(t.x));
+        asm("set.ge.f32.f32 %0, %1, 0f42FC0000;" : "=f"(end.y) : "f"(t.y));
         e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
     } else {
         constexpr float kLog2eLow = (float)(1.44269504088896340736 - (double)kLog2e);
         asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g.x));   // -126 ln 2
         asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g.y));
+        asm("set.le.f32.f32 %0, %1, 0fC2AEAC4F;" : "=f"(end.x) : "f"(g.x));
+        asm("set.le.f32.f32 %0, %1, 0fC2AEAC4F;" : "=f"(end.y) : "f"(g.y));
         asm("min.NaN.f32 %0, %0, 0f43480000;" : "+f"(g.x));   // 200: e is zero there, and t finite
         asm("min.NaN.f32 %0, %0, 0f43480000;" : "+f"(g.y));
         const float2 t = mul2(g, splat2(-kLog2e));
@@ -187,7 +194,7 @@ template <bool FAST> __device__ __forceinline__ void sigmoid2(float2 g, float2 &
     float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
     if constexpr (!FAST) r = fma2(r, fma2(make_float2(-d.x, -d.y), r, splat2(1.f)), r);
     rest = mul2(e, r);
-    a = add2(r, splat2(-0x1p-126f));
+    a = fma2(end, make_float2(-r.x, -r.y), r);
 }
 
 constexpr float kLargest = 3.402823466e38f;

@@ -284,3 +284,37 @@ def test_a_channel_does_not_depend_on_its_neighbours(dtype, gate):
     for name, got, w in zip(("h", "h_last", "states", "dx", "dg", "dh0"), call(x, g, dh), want):
         assert torch.equal(got[..., others], w[..., others]), name
         assert not torch.equal(got[..., bad], w[..., bad]), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_small_decays_of_large_states(dtype):
+    """sigmoid(g) of a strongly negative gate is good relative to itself, down to the smallest normal number: e = exp(-g) is off by
+    (|g| + 5) u, the sum, the reciprocal and the product with the state by 6 u at most, so a h by (|g| + 16) u of itself; below 2^-126
+    a may be zero.  A gate of minus infinity leaves nothing of an infinite state but NaN."""
+    g = torch.arange(-86.5, 0.0, 0.25)
+    D = g.numel()
+    g = g[None, None].expand(1, 200, -1).to(DT[dtype]).cuda()
+    h0 = torch.full((1, D), 3e38, device="cuda")
+    x = torch.zeros(1, 200, D, dtype=DT[dtype], device="cuda")
+    want = torch.sigmoid(g[:, 0].double()) * h0.double()
+    tol = (g[:, 0].double().abs() + 16) * U * want
+    _, last = ops.gated_scan(x[:, :1], g[:, :1], h0=h0, return_state=True)
+    assert ((last.double() - want).abs() <= tol).all()
+    _, last = ops.gated_scan(x, g, h0=h0, lengths=torch.ones(1, dtype=torch.int32, device="cuda"), return_state=True)
+    assert ((last.double() - want).abs() <= tol).all()
+    state = h0.clone()
+    ops.gated_scan_step(x[:, 0], g[:, 0], state)
+    assert ((state.double() - want).abs() <= tol).all()
+    st = ops.gated_scan_states(1, 1, D)
+    ops.gated_scan(x[:, :1], g[:, :1], states=st)
+    _, _, dh0 = ops.gated_scan_bwd(x[:, :1], x[:, :1], g[:, :1], st, dh_last=h0)
+    assert ((dh0.double() - want).abs() <= tol).all()
+    for gate in (-INF, -90.0, torch.finfo(DT[dtype]).min):
+        gt = torch.full((1, 1, 4), gate, dtype=DT[dtype], device="cuda")
+        one, inf = torch.ones_like(gt), torch.full((1, 4), INF, device="cuda")
+        _, last = ops.gated_scan(one, gt, h0=torch.full_like(inf, 3e38), return_state=True)
+        assert (last == 1).all()
+        _, last = ops.gated_scan(one, gt, h0=inf, return_state=True)
+        assert torch.isnan(last).all()
+        ops.gated_scan_step(one[:, 0], gt[:, 0], inf)
+        assert torch.isnan(inf).all()
