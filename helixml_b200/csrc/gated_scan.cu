@@ -20,6 +20,7 @@
 #include <initializer_list>
 
 #include "hx_common.cuh"
+#include "hx_overlap.h"
 #include "hx_tma.cuh"
 
 namespace hx {
@@ -844,6 +845,10 @@ template <typename Args> static hx_status choose_plan(const char *who, const Arg
     return HX_OK;
 }
 
+template <typename Args> static int64_t states_bytes(const Args &a) {
+    return (int64_t)a.batch * (((int64_t)a.seq_len + kBlock - 1) / kBlock) * a.d_inner * 4;
+}
+
 }  // namespace gated
 }  // namespace hx
 
@@ -888,6 +893,17 @@ hx_status hx_gated_scan_fwd(const hx_gated_scan_args *a, void *stream) {
     Plan plan;
     const hx_status ps = choose_plan("hx_gated_scan_fwd", *a, kSpanBytes, &plan);
     if (ps != HX_OK) return ps;
+    auto view = [&](const void *at, int64_t bs, int64_t rs) { return rows_of(at, a->batch, bs, a->seq_len, rs, a->d_inner, dtype_size(a->io_dtype)); };
+    const Operand outs[] = {{"h", view(a->h, a->h_batch_stride, a->h_row_stride)},
+                            {"h_last", dense_of(a->h_last, chains * 4)},
+                            {"states", dense_of(a->states, states_bytes(*a))},
+                            {"the workspace", dense_of(a->workspace, (int64_t)a->workspace_bytes)}};
+    const Operand ins[] = {{"x", view(a->x, a->x_batch_stride, a->x_row_stride)},
+                           {"g", view(a->g, a->g_batch_stride, a->g_row_stride)},
+                           {"h0", dense_of(a->h0, chains * 4)},
+                           {"lengths", dense_of(a->lengths, (int64_t)a->batch * 4)}};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_gated_scan_fwd: %s and %s share memory", one, other);
     HX_GATED_LAUNCH(launch_fwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
 }
 
@@ -923,6 +939,19 @@ hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *a, void *stream) {
     Plan plan;
     const hx_status ps = choose_plan("hx_gated_scan_bwd", *a, kSpanBytesBwd, &plan);
     if (ps != HX_OK) return ps;
+    auto view = [&](const void *at, int64_t bs, int64_t rs) { return rows_of(at, a->batch, bs, a->seq_len, rs, a->d_inner, dtype_size(a->io_dtype)); };
+    const Operand outs[] = {{"dx", view(a->dx, a->dx_batch_stride, a->dx_row_stride)},
+                            {"dg", view(a->dg, a->dg_batch_stride, a->dg_row_stride)},
+                            {"dh0", dense_of(a->dh0, chains * 4)},
+                            {"the workspace", dense_of(a->workspace, (int64_t)a->workspace_bytes)}};
+    const Operand ins[] = {{"x", view(a->x, a->x_batch_stride, a->x_row_stride)},
+                           {"g", view(a->g, a->g_batch_stride, a->g_row_stride)},
+                           {"dh", view(a->dh, a->dh_batch_stride, a->dh_row_stride)},
+                           {"states", dense_of(a->states, states_bytes(*a))},
+                           {"dh_last", dense_of(a->dh_last, chains * 4)},
+                           {"lengths", dense_of(a->lengths, (int64_t)a->batch * 4)}};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_gated_scan_bwd: %s and %s share memory", one, other);
     HX_GATED_LAUNCH(launch_bwd, a->gate, a->io_dtype, piece, *a, plan, (cudaStream_t)stream);
 }
 
@@ -940,6 +969,16 @@ hx_status hx_gated_scan_step(const void *x, int64_t x_row_stride, const void *g,
     const int64_t grid = ((int64_t)batch * ((d_inner + 1) / 2) + 127) / 128;
     HX_REQUIRE(grid <= 0x7fffffff, HX_ERR_INVALID_DIMENSION, "hx_gated_scan_step: batch * d_inner is too large for one launch");
     const size_t e = dtype_size(io_dtype);
+    // a thread reads its elements of every operand before it writes them, so that an output in an input's very place is right
+    auto same = [&](const void *in, int64_t stride) { return y == in && (stride == y_row_stride || batch == 1); };
+    auto view = [&](const void *at, int64_t rs) { return rows_of(at, batch, rs, 1, 0, d_inner, e); };
+    const Operand outs[] = {{"y", view(y, y_row_stride)}, {"h_out", dense_of(h_out, n * 4)}};
+    const Operand ins[] = {{"x", view(same(x, x_row_stride) ? nullptr : x, x_row_stride)},
+                           {"g", view(same(g, g_row_stride) ? nullptr : g, g_row_stride)}};
+    const Operand state[] = {{"h", dense_of(h == h_out ? nullptr : h, n * 4)}};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other) && !shared_operands(outs, state, one, other), HX_ERR_INVALID_INPUT,
+               "hx_gated_scan_step: %s and %s share memory", one, other);
     const uint64_t io = (uintptr_t)x | (uintptr_t)g | (uintptr_t)y | (uint64_t)(x_row_stride | g_row_stride | y_row_stride) * e;
     const bool pairs = d_inner % 2 == 0 && io % (2 * e) == 0 && ((uintptr_t)h | (uintptr_t)h_out) % 8 == 0;
 #define HX_GATED_STEP(T, GATE)                                                                                               \

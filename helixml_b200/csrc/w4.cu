@@ -2,6 +2,7 @@
 // entry points of the product.
 #include <type_traits>
 
+#include "hx_overlap.h"
 #include "hx_tma.cuh"
 #include "w4.cuh"
 
@@ -212,6 +213,11 @@ static hx_status check_matrix(const char *who, const hx_w4_matrix *m) {
     HX_REQUIRE(((uintptr_t)m->codes & 15) == 0, HX_ERR_INVALID_INPUT, "%s: codes must be 16-byte aligned", who);
     return HX_OK;
 }
+static int64_t codes_bytes(const hx_w4_matrix &m) { return (int64_t)m.rows * blocks_of(m.cols) * kBlockBytes; }
+static int64_t scale_bytes(const hx_w4_matrix &m) { return (int64_t)m.rows * (m.cols / m.group) * (int64_t)dtype_size(m.scale_dtype); }
+static int64_t zero_bytes(const hx_w4_matrix &m) { return (int64_t)m.rows * (m.cols / m.group); }
+#define HX_W4_PARTS(M) {"codes", dense_of((M).codes, codes_bytes(M))}, {"scale", dense_of((M).scale, scale_bytes(M))}, {"zero", dense_of((M).zero, zero_bytes(M))}
+
 // The grid of a kernel with one thread per item, if there is one.
 static hx_status grid_of(const char *who, int64_t items, unsigned *grid) {
     const int64_t g = (items + 255) / 256;
@@ -239,6 +245,9 @@ hx_status hx_w4_quantize(const void *W, int64_t ldw, int32_t w_dtype, const hx_w
     HX_REQUIRE(ldw >= 0, HX_ERR_INVALID_INPUT, "hx_w4_quantize: negative stride");
     const int blocks = blocks_of(m->cols);
     unsigned grid;
+    const Operand outs[] = {HX_W4_PARTS(*m)}, ins[] = {{"W", rows_of(W, m->rows, ldw, 1, 0, m->cols, dtype_size(w_dtype))}};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_w4_quantize: %s and %s share memory", one, other);
     const hx_status g = grid_of("hx_w4_quantize", (int64_t)m->rows * blocks * (16 / kEach), &grid);
     if (g != HX_OK) return g;
     const bool vec = aligned8(W, ldw, w_dtype);
@@ -264,6 +273,9 @@ hx_status hx_w4_pack(const uint8_t *in, int64_t ldc, const hx_w4_matrix *m, void
     HX_REQUIRE(ldc >= 0, HX_ERR_INVALID_INPUT, "hx_w4_pack: negative stride");
     const int blocks = blocks_of(m->cols);
     unsigned grid;
+    const Operand outs[] = {{"codes", dense_of(m->codes, codes_bytes(*m))}}, ins[] = {{"the codes given", rows_of(in, m->rows, ldc, 1, 0, m->cols, 1)}};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_w4_pack: %s and %s share memory", one, other);
     const hx_status g = grid_of("hx_w4_pack", (int64_t)m->rows * blocks * 16, &grid);
     if (g != HX_OK) return g;
     pack_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(in, ldc, *m, blocks);
@@ -278,6 +290,9 @@ hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t 
     HX_REQUIRE(W != nullptr, HX_ERR_INVALID_INPUT, "hx_w4_dequantize: W is NULL");
     HX_REQUIRE(m->rows == 1 || ldw >= m->cols, HX_ERR_SHAPE_MISMATCH, "hx_w4_dequantize: rows of W overlap (stride %lld)", (long long)ldw);
     unsigned grid;
+    const Operand outs[] = {{"W", rows_of(W, m->rows, ldw, 1, 0, m->cols, dtype_size(w_dtype))}}, ins[] = {HX_W4_PARTS(*m)};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_w4_dequantize: %s and %s share memory", one, other);
     const hx_status g = grid_of("hx_w4_dequantize", (int64_t)m->rows * (m->cols / 16), &grid);
     if (g != HX_OK) return g;
     const bool vec = aligned8(W, ldw, w_dtype);
@@ -302,6 +317,10 @@ hx_status hx_gemm_w4(const void *A, int64_t lda, int32_t a_dtype, const hx_w4_ma
     HX_REQUIRE(A && C, HX_ERR_INVALID_INPUT, "hx_gemm_w4: A and C must not be NULL");
     HX_REQUIRE(lda >= 0, HX_ERR_INVALID_INPUT, "hx_gemm_w4: negative stride");
     HX_REQUIRE(M == 1 || ldc >= m->rows, HX_ERR_SHAPE_MISMATCH, "hx_gemm_w4: rows of C overlap (stride %lld)", (long long)ldc);
+    const Operand outs[] = {{"C", rows_of(C, M, ldc, 1, 0, m->rows, dtype_size(c_dtype))}};
+    const Operand ins[] = {{"A", rows_of(A, M, lda, 1, 0, m->cols, dtype_size(a_dtype))}, {"the bias", dense_of(bias, (int64_t)m->rows * 4)}, HX_W4_PARTS(*m)};
+    const char *one, *other;
+    HX_REQUIRE(!shared_operands(outs, ins, one, other), HX_ERR_INVALID_INPUT, "hx_gemm_w4: %s and %s share memory", one, other);
     return a_dtype == HX_BF16 ? gemm_bf16(A, lda, *m, bias, C, ldc, c_dtype, M, epilogue, (cudaStream_t)stream)
                               : gemm_f32(A, lda, *m, bias, C, ldc, c_dtype, M, epilogue, (cudaStream_t)stream);
 }

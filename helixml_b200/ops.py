@@ -269,7 +269,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     """Gated linear recurrence (hx_gated_scan_fwd): h_t = g_t h_{t-1} + x_t ("decay"), or a_t h_{t-1} + (1 - a_t) x_t with
     a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
     lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
-    states: a gated_scan_states buffer, filled for gated_scan_bwd; out shares no memory with x or g.
+    states: a gated_scan_states buffer, filled for gated_scan_bwd; an out that shares memory with x or g is refused.
     Returns h, or (h, h_last [B, D] fp32) with return_state."""
     dev, shape = _cuda("x", x), x.shape
     xb, xr = _view3(x)
@@ -298,7 +298,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
 def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None, out=None):
     """Gradients of gated_scan (hx_gated_scan_bwd): (dx, dg, dh0) for dh = dL/dh [B, L, D] and dh_last = dL/dh_last [B, D]
     fp32 (None: zero).  x, g and lengths as given to gated_scan, states as it filled them; out: (dx, dg) to write into (halves
-    of one buffer, say)."""
+    of one buffer, say; memory of an input is refused)."""
     dev, shape = _cuda("x", x), x.shape
     xb, xr = _view3(x)
     dt = _float("x", x)
@@ -329,7 +329,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
 
 def gated_scan_step(x, g, h, gate="sigmoid", h_out=None, out=None):
     """One token of the gated recurrence for every sequence (hx_gated_scan_step): x, g [B, D] (row strides arbitrary),
-    h [B, D] fp32.  Returns y [B, D]; the new state goes to h_out, or replaces h."""
+    h [B, D] fp32.  Returns y [B, D]; the new state goes to h_out, or replaces h; out may be x or g itself."""
     dev, shape = _cuda("x", x), x.shape
     if len(shape) != 2:
         raise L.HxError(1, f"expected a [B, D] tensor, got {tuple(shape)}")
@@ -521,7 +521,7 @@ def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
 
 def gemm_w4(a, m: W4Matrix, bias=None, out_dtype=None, epilogue=L.EPI_NONE, out=None):
     """C = a @ W.T (+ bias) (+ activation) with W in 4 bits (hx_gemm_w4), for the few rows of a decode step.
-    a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's), no memory of a's."""
+    a [M, K] fp32 or bf16 (row stride arbitrary), bias [N] fp32; C [M, N] in out_dtype (default a's); an out that shares memory with a is refused."""
     dev, lda = _cuda("a", a), _rows2("a", a)
     adt = _float("a", a)
     M, K = a.shape

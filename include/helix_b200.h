@@ -312,8 +312,9 @@ HX_API hx_status hx_s4_diag_fwd(const void *u, const float *A, const float *Bp, 
  *   lengths (int32 [batch] on the device, or NULL for seq_len everywhere; values are clamped to 0 .. seq_len): rows of a
  *   padded batch from len[b] on are not read as numbers (they may hold anything), their outputs are zeros, and h_last is the
  *   state after row len[b] - 1 (h0 where len[b] is 0).
- * x, g and dh may be any views with a unit inner stride and strides >= 0; the rows of an output must not overlap one another
- * or an input. */
+ * x, g and dh may be any views with a unit inner stride and strides >= 0.  Rows of an output that overlap one another, and an
+ * output or a workspace that shares memory with another operand, are refused (parts of one buffer that lie between one another
+ * are apart). */
 typedef enum hx_gate_kind { HX_GATE_DECAY = 0, HX_GATE_SIGMOID = 1 } hx_gate_kind;
 /* Steps from one state kept for the backward pass to the next. */
 #define HX_GATED_SCAN_STATE_STEPS 16
@@ -369,7 +370,8 @@ typedef struct hx_gated_scan_bwd_args {
 HX_API hx_status hx_gated_scan_bwd(const hx_gated_scan_bwd_args *args, void *stream);
 
 /* One token per sequence: h_out = a h + x (or (1 - a) x), y = h_out in the io dtype.  x, g, y: [batch, d_inner] with row
- * strides; h, h_out: [batch, d_inner] fp32, dense; h_out may be h. */
+ * strides; h, h_out: [batch, d_inner] fp32, dense; h_out may be h, and y may be x or g (same address and row stride); operands
+ * that share memory in any other way are refused. */
 HX_API hx_status hx_gated_scan_step(const void *x, int64_t x_row_stride, const void *g, int64_t g_row_stride, const float *h,
                              float *h_out, void *y, int64_t y_row_stride, int32_t batch, int32_t d_inner, int32_t gate,
                              int32_t io_dtype, void *stream);
@@ -466,7 +468,7 @@ HX_API hx_status hx_w4_pack(const uint8_t *in, int64_t ldc, const hx_w4_matrix *
 /* The values the matrix stands for: W [rows, cols] fp32 or bf16, row stride ldw. */
 HX_API hx_status hx_w4_dequantize(const hx_w4_matrix *m, void *W, int64_t ldw, int32_t w_dtype, void *stream);
 /* C[M,N] = A[M,K] . W^T (+ bias[N]) (+ activation: 0 none, 1 SiLU, 2 softplus) with N = m->rows, K = m->cols; A and C fp32 or
- * bf16 with row strides in elements, bias fp32; C overlaps neither A nor the matrix.  Every product and sum is fp32 or wider
+ * bf16 with row strides in elements, bias fp32; a C that shares memory with another operand is refused.  Every product and sum is fp32 or wider
  * than its operands: codes are exact, the sum over a group is scaled in fp32.  Made for the few rows of a decode step (any M is
  * right; the weights are turned into operands once per 64 rows, so from about 200 rows on hx_w4_dequantize with hx_gemm_bf16 is
  * the faster way: N = K = 4096, 128 rows 24 us against 32, 512 rows 67 against 34). */

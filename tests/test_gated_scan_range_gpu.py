@@ -9,6 +9,7 @@ segment hands its state on, numbers below 2^-126 may be taken as zero: 2^-126 a 
 import pytest
 import torch
 
+from helixml_b200 import _lib as L_
 from helixml_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -318,3 +319,32 @@ def test_small_decays_of_large_states(dtype):
         assert torch.isnan(last).all()
         ops.gated_scan_step(one[:, 0], gt[:, 0], inf)
         assert torch.isnan(inf).all()
+
+
+def test_shared_memory_is_refused_and_parts_of_one_buffer_are_not():
+    B, L, D = 2, 900, 40
+    buf = torch.randn(B, L, 5 * D, generator=torch.Generator().manual_seed(2)).cuda()
+    part = lambda i: buf[:, :, i * D:(i + 1) * D]
+    want = ops.gated_scan(part(0), part(1))
+    st = ops.gated_scan_states(B, L, D)
+    assert torch.equal(ops.gated_scan(part(0), part(1), out=part(2), states=st), want)
+    x, g, dh = (part(i).clone() for i in (0, 1, 2))
+    dx, dg, _ = ops.gated_scan_bwd(dh, x, g, st)
+    ops.gated_scan_bwd(part(2), part(0), part(1), st, out=(part(3), part(4)))
+    assert torch.equal(part(3), dx) and torch.equal(part(4), dg)
+    first = x[:, :1].expand(B, L, D)      # an input without a stride, and an output among the rows around it
+    assert torch.equal(ops.gated_scan(buf[:, :1, :D].expand(B, L, D), g, out=part(4)), ops.gated_scan(first, g))
+    h = torch.randn(B, D, device="cuda")
+    y = ops.gated_scan_step(x[:, 0], g[:, 0], h.clone())
+    xt = x[:, 0].contiguous()
+    assert torch.equal(ops.gated_scan_step(xt, g[:, 0], h, out=xt), y) and torch.equal(xt, y)
+    before = buf.clone()
+    for call in (lambda: ops.gated_scan(part(0), part(1), out=part(0)), lambda: ops.gated_scan(part(0), part(1), out=part(1)),
+                 lambda: ops.gated_scan(part(0), part(1), out=buf[:, :, 3:D + 3]), lambda: ops.gated_scan(x, g, out=x),
+                 lambda: ops.gated_scan(x[:, 1:], g[:, 1:], out=x[:, :-1]), lambda: ops.gated_scan_bwd(dh, x, g, st, out=(dh, dg)),
+                 lambda: ops.gated_scan_bwd(dh, x, g, st, out=(dx, dx)), lambda: ops.gated_scan_bwd(dh, x, g, st, out=(dx, g)),
+                 lambda: ops.gated_scan_step(buf[:, 0, :D], g[:, 0], h, out=buf[:, 0, 1:D + 1])):
+        with pytest.raises(L_.HxError) as e:
+            call()
+        assert e.value.status == 10 and "share memory" in str(e.value)
+    assert torch.equal(buf, before)
