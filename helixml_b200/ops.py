@@ -185,6 +185,15 @@ def _float(name, t) -> int:
     return code
 
 
+def _fits(shape):
+    """The library takes sizes in 32 bits, and ctypes would cut a larger one down without a word."""
+    bits = 0
+    for n in shape:
+        bits |= n
+    if bits >> 31:
+        raise L.HxError(2, f"a size of {tuple(shape)} is above 2^31 - 1")
+
+
 def _cuda(name, t) -> int:
     dev = t.get_device()
     if dev < 0:
@@ -276,6 +285,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     dt = _float("x", x)
     _like("g", g, shape, x.dtype, dev)
     gb, gr = _view3(g)
+    _fits(shape)
     Bsz, Lq, Dm = shape
     if out is None:
         h = _same(x)
@@ -306,6 +316,7 @@ def gated_scan_bwd(dh, x, g, states, gate="sigmoid", lengths=None, dh_last=None,
     _like("dh", dh, shape, x.dtype, dev)
     gb, gr = _view3(g)
     db, dr = _view3(dh)
+    _fits(shape)
     Bsz, Lq, Dm = shape
     if out is None:
         dx, dg = _same(x), _same(x)
@@ -333,6 +344,7 @@ def gated_scan_step(x, g, h, gate="sigmoid", h_out=None, out=None):
     dev, shape = _cuda("x", x), x.shape
     if len(shape) != 2:
         raise L.HxError(1, f"expected a [B, D] tensor, got {tuple(shape)}")
+    _fits(shape)
     dt, code = _float("x", x), _gate(gate)
     _like("g", g, shape, x.dtype, dev)
     _dense_out("h", h, shape, torch.float32, dev)
@@ -456,6 +468,7 @@ class W4Matrix:
     def __init__(self, rows, cols, group, scale, zero):
         if group not in (32, 64, 128) or cols % group:
             raise L.HxError(1, f"{cols} columns in groups of {group}: groups are 32, 64 or 128 and divide the columns")
+        _fits((rows, cols))
         dev = _cuda("scale", scale)
         _float("scale", scale)
         self.rows, self.cols, self.group = rows, cols, group
@@ -469,9 +482,10 @@ class W4Matrix:
 
 
 def _rows2(name, t):
-    """Row stride in elements of a [rows, columns] view with unit inner stride."""
+    """Row stride in elements of a [rows, columns] view with unit inner stride, whose sizes the library can take."""
     if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
         raise L.HxError(1, f"{name}: expected a 2-D tensor with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
+    _fits(t.shape)
     return t.stride(0)
 
 

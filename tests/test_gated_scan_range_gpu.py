@@ -348,3 +348,16 @@ def test_shared_memory_is_refused_and_parts_of_one_buffer_are_not():
             call()
         assert e.value.status == 10 and "share memory" in str(e.value)
     assert torch.equal(buf, before)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Views that repeat one element 2^32 + 5 times: the sizes reach the library in 32 bits."""
+    many = (1 << 32) + 5
+    one = torch.zeros(1, 1, 1, device="cuda")
+    x = one.expand(1, many, 1)
+    for call in (lambda: ops.gated_scan(x, x), lambda: ops.gated_scan_bwd(x, x, x, ops.gated_scan_states(1, 5, 1)),
+                 lambda: ops.gated_scan(one.expand(many, 1, 1), one.expand(many, 1, 1)),
+                 lambda: ops.gated_scan_step(one[0].expand(many, 1), one[0].expand(many, 1), torch.zeros(5, 1, device="cuda"))):
+        with pytest.raises(L_.HxError) as e:
+            call()
+        assert e.value.status == 2
