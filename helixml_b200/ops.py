@@ -523,12 +523,12 @@ def w4_pack(codes, scale, zero=None) -> W4Matrix:
     return m
 
 
-def w4_dequantize(m: W4Matrix, dtype=torch.float32, out=None):
-    """The values a W4Matrix stands for, [N, K] fp32 or bf16 (hx_w4_dequantize)."""
+def w4_dequantize(m: W4Matrix, dtype=None, out=None):
+    """The values a W4Matrix stands for, [N, K] fp32 or bf16 (hx_w4_dequantize); dtype: out's, or fp32, unless named."""
     dev = m.codes.get_device()
-    w = _rows_like(m.rows, m.cols, dtype, dev) if out is None else out
+    w = _rows_like(m.rows, m.cols, dtype or torch.float32, dev) if out is None else out
     dt = _float("out", w)
-    _like("out", w, (m.rows, m.cols), dtype, dev)
+    _like("out", w, (m.rows, m.cols), dtype or w.dtype, dev)
     _call(dev, L.lib().hx_w4_dequantize, C.byref(m._args()), w.data_ptr(), _rows2("out", w), dt)
     return w
 

@@ -1,4 +1,5 @@
-"""4-bit weights at the edges of the calls: outputs in an operand's memory, sizes beyond 32 bits."""
+"""4-bit weights at the edges of the calls: outputs in an operand's memory, sizes beyond 32 bits, the
+type of an output that is given, matrices and rows that are not there."""
 import pytest
 import torch
 
@@ -34,3 +35,34 @@ def test_sizes_beyond_32_bits_are_refused():
         with pytest.raises(L.HxError) as e:
             call()
         assert e.value.status == 2
+
+
+def test_values_in_the_type_of_the_output_given():
+    m = ops.w4_quantize(torch.randn(7, 64, generator=torch.Generator().manual_seed(3)).cuda(), 32)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.empty(7, 64, device="cuda", dtype=dtype)
+        assert ops.w4_dequantize(m, out=out) is out and torch.equal(out, ops.w4_dequantize(m, dtype))
+    assert ops.w4_dequantize(m).dtype == torch.float32
+    for code, call in ((4, lambda: ops.w4_dequantize(m, torch.float32, out=torch.empty(7, 64, device="cuda", dtype=torch.bfloat16))),
+                       (4, lambda: ops.w4_dequantize(m, out=torch.empty(7, 64, device="cuda", dtype=torch.float16)))):
+        with pytest.raises(L.HxError) as e:
+            call()
+        assert e.value.status == code
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_nothing_to_do(zeros, dtype):
+    """No rows of weights, no rows of A, and a matrix without columns: it can be made and read back, a product with it is refused."""
+    none = ops.w4_quantize(torch.empty(0, 64, device="cuda", dtype=dtype), 32, zero_points=zeros)
+    assert none.codes.shape == (0, 64) and none.scale.shape == (0, 2) and ops.w4_dequantize(none).shape == (0, 64)
+    assert ops.gemm_w4(torch.ones(3, 64, device="cuda", dtype=dtype), none).shape == (3, 0)
+    packed = ops.w4_pack(torch.empty(0, 64, device="cuda", dtype=torch.uint8), torch.empty(0, 2, device="cuda", dtype=dtype))
+    assert packed.group == 32 and ops.w4_dequantize(packed, dtype).shape == (0, 64)
+    m = ops.w4_quantize(torch.ones(5, 64, device="cuda", dtype=dtype), 32, zero_points=zeros)
+    assert ops.gemm_w4(torch.empty(0, 64, device="cuda", dtype=dtype), m).shape == (0, 5)
+    narrow = ops.w4_quantize(torch.empty(5, 0, device="cuda", dtype=dtype), 32, zero_points=zeros)
+    assert ops.w4_dequantize(narrow, dtype).shape == (5, 0)
+    with pytest.raises(L.HxError) as e:
+        ops.gemm_w4(torch.empty(3, 0, device="cuda", dtype=dtype), narrow)
+    assert e.value.status == 2
