@@ -267,11 +267,10 @@ static hx_status launch_few(const void *A, int64_t lda, const hx_w4_matrix &m, c
 
 hx_status gemm_bf16(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                     cudaStream_t st) {
-    // up to eight rows: 1 x 16384 x 4096 13.3 us, 16.4 with the kernel for more; too long to be staged, 8 x 4096 x 16384, 17.1 with that one
+    // In us, this kernel and the one for more: 1 x 16384 x 4096 11.7, 13.5; 1 x 768 x 12288 6.7, 9.7; 4 x 2048 x 1536 4.2, 4.9; at eight rows
+    // they meet: 8 x 16384 x 4096 15.0, 14.6; 8 x 4096 x 4096 8.6, 7.0; 8 x 2048 x 1536 4.3, 5.1.
     if (M <= 8 && fits_staged(m, M)) return launch_few(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 16) return launch_rows<__nv_bfloat16, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 32) return launch_rows<__nv_bfloat16, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    return launch_rows<__nv_bfloat16, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_rows_for<__nv_bfloat16>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
 }
 
 }  // namespace w4

@@ -6,11 +6,7 @@ namespace w4 {
 
 hx_status gemm_f32(const void *A, int64_t lda, const hx_w4_matrix &m, const float *bias, void *C, int64_t ldc, int c_dtype, int M, int epilogue,
                    cudaStream_t st) {
-    if (M <= 8) return launch_rows<float, 1>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 16) return launch_rows<float, 2>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 24) return launch_rows<float, 3>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    if (M <= 32) return launch_rows<float, 4>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
-    return launch_rows<float, 8>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
+    return launch_rows_for<float>(A, lda, m, bias, C, ldc, c_dtype, M, epilogue, st);
 }
 
 }  // namespace w4

@@ -1,7 +1,8 @@
 """4-bit weights at the edges of the calls: outputs in an operand's memory, sizes beyond 32 bits, the
-type of an output that is given, matrices and rows that are not there."""
+type of an output that is given, matrices and rows that are not there, every count of row tiles."""
 import pytest
 import torch
+from test_w4_gpu import check_product, make, values
 
 from helixml_b200 import _lib as L
 from helixml_b200 import ops
@@ -66,3 +67,26 @@ def test_nothing_to_do(zeros, dtype):
     with pytest.raises(L.HxError) as e:
         ops.gemm_w4(torch.empty(3, 0, device="cuda", dtype=dtype), narrow)
     assert e.value.status == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,K,group", [(300, 416, 32), (2500, 256, 64), (70, 2048, 128)])
+def test_every_count_of_row_tiles(N, K, group, dtype):
+    """Rows of A up to, at and behind each multiple of 8 below 64, NaN in the memory behind the last one; the bound is check_product's."""
+    codes, scale, zero = make(N, N, K, group, dtype, True)
+    m, w = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda()), values(codes, scale, zero, group)
+    full = torch.full((72, K), float("nan"), device="cuda", dtype=dtype)
+    for M in (9, 16, 17, 24, 25, 32, 33, 39, 40, 41, 48, 49, 55, 56, 57, 64, 65):
+        full[:M] = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dtype).cuda()
+        out = torch.full((72, N), 7.0, device="cuda", dtype=torch.float32)
+        ops.gemm_w4(full[:M], m, out=out[:M])
+        check_product(out[:M], full[:M], w, None)
+        assert (out[M:] == 7).all()
+
+
+@pytest.mark.parametrize("M", [1, 8])
+def test_few_rows_too_long_to_be_staged(M):
+    codes, scale, zero = make(3, 40, 65536, 128, torch.bfloat16, True)
+    m = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda())
+    a = torch.randn(M, 65536, generator=torch.Generator().manual_seed(M)).bfloat16().cuda()
+    check_product(ops.gemm_w4(a, m, out_dtype=torch.float32), a, values(codes, scale, zero, 128), None)
