@@ -23,9 +23,9 @@ __device__ __forceinline__ void split(int64_t i, int across, int64_t &row, int &
 constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer, ties to even, and leaves that in the low bits
 constexpr float kNear = 0.5f - 1.52587890625e-5f;   // 1/2 - 2^-16
 
-// w / s rounded as exact arithmetic decides it, given fp32's q = w * (1 / s) and n, that rounded.  q is off by less than 2^-20 for
-// |w / s| < 17 (larger ones are clamped), so only a q within 2^-16 of a half can have gone to the wrong side, and there the sign of
-// w - half * s, which a fused multiply-add gives exactly, tells.
+// w / s rounded as exact arithmetic decides it, given fp32's q = w * (1 / s) and n, that rounded.  The reciprocal and the product round
+// once each, so q is off by at most 2^-23 of itself, less than 2^-18 for |w / s| < 17 (larger ones are clamped).  So only a q within
+// 2^-16 of a half can have gone to the wrong side, and there the sign of w - half * s, which a fused multiply-add gives exactly, tells.
 __device__ __forceinline__ float settle(float w, float s, float q, float n) {
     const float e = q - n;
     if (!(fabsf(e) > kNear)) return n;

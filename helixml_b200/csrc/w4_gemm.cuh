@@ -55,7 +55,7 @@ __device__ __forceinline__ void eight_weights(uint32_t word, uint32_t minus_zero
 constexpr float kSumScale = 64.f;   // what the sums have to be multiplied by in the end
 
 // fp32 rows of A go into the MMA as three bf16 parts that add up to them: the high 8 bits, the next 8, the rest.  The differences are
-// exact; an infinity has no rest, a NaN a NaN.
+// exact; an infinity has no rest, a NaN a NaN.  (Below 2^-110 the last part ends above the number's last bit: bf16 goes down to 2^-133.)
 template <typename TA> constexpr int kPartsOf = sizeof(TA) == 2 ? 1 : 3;
 __device__ __forceinline__ void cut(float v, uint32_t (&part)[3]) {
     part[0] = __float_as_uint(v) & 0xffff0000u;

@@ -279,6 +279,7 @@ def gated_scan(x, g, h0=None, gate="sigmoid", lengths=None, out=None, return_sta
     a_t = sigmoid(g_t) ("sigmoid").  x, g: [B, L, D] views with unit inner stride, both bf16 or fp32; h0 [B, D] fp32;
     lengths [B] int32: rows of a padded batch from lengths[b] on are not looked at and come out as zeros.
     states: a gated_scan_states buffer, filled for gated_scan_bwd; an out that shares memory with x or g is refused.
+    Like every call here it leaves no trace for torch's autograd, whatever its inputs require: gated_scan_bwd gives the gradients.
     Returns h, or (h, h_last [B, D] fp32) with return_state."""
     dev, shape = _cuda("x", x), x.shape
     xb, xr = _view3(x)

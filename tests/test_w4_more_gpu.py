@@ -1,5 +1,6 @@
 """4-bit weights at the edges of the calls: outputs in an operand's memory, sizes beyond 32 bits, the
-type of an output that is given, matrices and rows that are not there, every count of row tiles."""
+type of an output that is given, matrices and rows that are not there, every count of row tiles, and
+elements of A near the format's lower end."""
 import pytest
 import torch
 from test_w4_gpu import check_product, make, values
@@ -90,3 +91,17 @@ def test_few_rows_too_long_to_be_staged(M):
     m = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda())
     a = torch.randn(M, 65536, generator=torch.Generator().manual_seed(M)).bfloat16().cuda()
     check_product(ops.gemm_w4(a, m, out_dtype=torch.float32), a, values(codes, scale, zero, 128), None)
+
+
+def test_small_elements_of_fp32_rows():
+    """From 2^-110 on every bit of an element counts; below, what is left of it after cutting to a multiple of 2^-133."""
+    K, N = 128, 24
+    codes, _, zero = make(8, N, K, 64, torch.float32, True)
+    scale = torch.full((N, K // 64), 2.0 ** 100)
+    m, w = ops.w4_pack(codes.cuda(), scale.cuda(), zero.cuda()), values(codes, scale, zero, 64)
+    a = torch.randn(12, K, generator=torch.Generator().manual_seed(9)) * 2.0 ** -torch.arange(104.0, 140.0, 3.0)[:, None]
+    c = a.double() @ w.t()
+    tol = 2 * 2.0 ** -24 * (18 + K / 16) * (a.double().abs() @ w.abs().t())
+    tol += (a.abs() < 2.0 ** -110).double() @ w.abs().t() * 2.0 ** -133
+    for rows in (slice(0, 12), slice(3, 4)):
+        assert ((ops.gemm_w4(a[rows].cuda(), m).double().cpu() - c[rows]).abs() <= tol[rows]).all()
