@@ -47,8 +47,8 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     return r;
 }
 
-// A thread takes 16 columns, two words; a group's threads meet in shuffles.  What bounds it is instructions, about half of them a
-// thread's own and half a weight's: 8192 x 8192 fp32 59 us (78 % of a copy's rate), 16384 x 4096 bf16 with bf16 scales 50 (52 %).
+// A thread takes 16 columns, two words; a group's threads meet in shuffles.  8192 x 8192 fp32 48.5 us in a graph (95 % of a copy's rate);
+// 16384 x 4096 bf16 with bf16 scales 44.7 (57 %): half the bytes under the same instructions a thread, two thirds of the issue slots.
 template <typename T, bool ZERO>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int blocks, int shift, bool vec) {   // group = 2^shift
@@ -164,6 +164,8 @@ quantize_kernel(const T *__restrict__ W, int64_t ldw, const hx_w4_matrix m, int 
     for (int i = 0; i < kEach; ++i) row[word_at(part % (16 / kEach) * kEach + i)] = word[i];
 }
 
+// A word of eight codes a thread, read byte by byte at any alignment, once when a model is loaded: 16384 x 4096 34 us (45 % of a copy's
+// rate).
 __global__ void __launch_bounds__(256)
 pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, int blocks) {
     int64_t n;
@@ -180,8 +182,9 @@ pack_kernel(const uint8_t *__restrict__ in, int64_t ldc, const hx_w4_matrix m, i
     reinterpret_cast<uint32_t *>(m.codes)[(n * blocks + w / 16) * 16 + word_at(w & 15)] = word;
 }
 
-// A thread takes 16 columns, two words of one group; they are 64 or 32 bytes of W, written a sector at a time: 8192 x 8192 fp32 51 us
-// (91 % of a copy's rate; 74 in 16-byte stores of a word a thread), 16384 x 4096 bf16 37 (70 %; 49).
+// A thread takes 16 columns, two words of one group; they are 64 or 32 bytes of W, written a sector at a time: 8192 x 8192 fp32 47.3 us
+// in a graph (97 % of a copy's rate), 16384 x 4096 bf16 31.8 (80 %).  (As calls of their own, 51 and 37, where 16-byte stores of a word
+// a thread took 74 and 49.)
 template <typename T>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const hx_w4_matrix m, T *__restrict__ W, int64_t ldw, int blocks, int shift, bool vec) {

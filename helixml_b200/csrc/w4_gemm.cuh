@@ -11,8 +11,7 @@ namespace hx {
 namespace w4 {
 
 // ---------------------------------------------------------------- C = A W^T for a few rows
-// A stream over the codes: HBM gives an SM about 23 bytes = 46 codes a cycle, each of which has to become a tensor-core operand, so
-// instructions per code are what the kernel is made of.  W is the left operand (16 outputs x 16 columns), the rows of A the right one
+// A stream over the codes: HBM gives an SM about 23 bytes = 46 codes a cycle, each of which has to become a tensor-core operand.  W is the left operand (16 outputs x 16 columns), the rows of A the right one
 // (8 rows a tile).  Which column a k index of the MMA stands for does not matter as long as both operands agree; the layout of the
 // codes is such that lane (g, c) = (lane / 4, lane mod 4) finds in its 16 bytes of row g four words, word j holding the columns
 // 32 j + 8 c .. + 7 of the block, as the four k-pairs of two MMAs.  So the MMAs of word j cover columns 32 j .. 32 j + 31 whatever
@@ -99,9 +98,9 @@ static hx_status clusters_at_once(Kernel kernel, int threads, size_t smem, int s
 // The same products where a piece of A costs as much as the codes: more than one tile of 8 rows, or fp32 rows, which have to be cut
 // (1 x 16384 x 4096 fp32: 34.6 us where every warp cuts for itself, 20.0 here).  A CTA's warps take different outputs, 16 each, walk
 // the columns together and share the block of A they are at, staged in shared memory (fp32 rows already cut, once a CTA).  One barrier
-// a block; codes, A and scales of the next blocks are under way.  What bounds it is instructions (1.5 a cycle of the SM) around a
-// warp-level tensor pipe that is 35 to 40 % busy: 16 x 16384 x 4096 bf16 18.2 us, 32 rows 25.9, 64 rows 43.5; 24 x 5001 x 8192 fp32 in
-// groups of 32 with zero points 36.1.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
+// a block; codes, A and scales of the next blocks are under way.  No unit is full: 1.5 instructions a cycle of an SM's 4, the
+// warp-level tensor pipe 35 to 40 % busy, 21 % of the warp slots filled; a warp waits for its own chain and for the barrier of every
+// block.  16 x 16384 x 4096 bf16 17.9 us, 32 rows 25.6, 64 rows 43.1; 24 x 5001 x 8192 fp32 in groups of 32 with zero points 34.7.  Where tiles of 128 outputs are few, a cluster of CTAs shares the columns; each adds up a part of
 // the outputs out of the others' shared memory, in the order of the ranks.
 template <typename TA, int NT> constexpr int row_warps() { return 8; }
 constexpr int kRowPitch = kBlockCols * 2 + 64;   // bytes from one staged row to the next: rows g and g + 1 fall on different banks

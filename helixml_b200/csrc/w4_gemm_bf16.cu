@@ -11,8 +11,9 @@ namespace w4 {
 // scoreboard: loads that miss and loads that hit would share one.  The four lanes of a row need the same scales, so lane c loads
 // those of block c of the chunk and the others get them by shuffle.  The warps' partial sums are added in the order of the warps.
 // Where the tiles are fewer than the SMs, a cluster of CTAs shares a tile's columns and the first one adds the others' sums out of
-// their shared memory.  16384 x 4096, groups of 128: one row 13.3 us (40 % of HBM's rate; the loads alone take 8.7, the rest is
-// instructions), eight rows 16.7.
+// their shared memory.  16384 x 4096, groups of 128: one row 12.7 us out of HBM (42 % of its rate; the loads alone take 8.7), eight
+// rows 15.8.  No unit is full: half of the issue slots, 18 % of the warp-level tensor pipe, 22 % of the warp slots (16 warps an SM, by
+// their registers).  What a warp waits for is its own chain of convert, multiply and scale, and a stream that starts cold.
 constexpr int kMostWarps = 16;   // of a CTA, by its registers
 
 // Where a warp's partial sum of output n of the tile and row `row` of A lies: [lane][i].
