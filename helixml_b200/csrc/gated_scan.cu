@@ -273,7 +273,7 @@ template <int GATE> struct Reach {
         lost_b = fmaf(lost_a, fabsf(r), lost_b);
         reach = fmaf(lift, fabsf(r), reach);
         if constexpr (GATE == HX_GATE_DECAY) lift = fmaxf(fmaxf(most, 1.f), lift * fabsf(p));   // a sigmoid's is 1
-        lost_a = fmaf(lost_a, fabsf(p), fmaf(fabsf(A), ep, A != 0.f && fabsf(A * p) < kNormal ? kStep : 0.f));
+        lost_a = fmaf(lost_a, fmaf(ep, 0x1p-100f, fabsf(p)), fmaf(fabsf(A), ep, A != 0.f && fabsf(A * p) < kNormal ? kStep : 0.f));
     }
     __device__ __forceinline__ float mark(float A, float B) const {
         const bool good = lift < kMostLift && reach < kMostReach && (lost_a <= 0x1p-40f || lost_a <= 0x1p76f * fabsf(A)) &&
@@ -281,10 +281,10 @@ template <int GATE> struct Reach {
         return good ? A : __int_as_float(0x7fc00000);
     }
 };
-// The run's error of p where products on the way are below 2^-126: nearly never with decays, and then worth a second look, unless A is
-// zero already.  A sigmoid's decays are at most 1, so that each rounding counts once.
-template <int GATE> __device__ __forceinline__ float lost_in_run(const float (&a)[kRun], float least, float A) {
-    if (!(least < kNormal) || A == 0.f) return 0.f;
+// The run's error of p where products on the way are below 2^-126: nearly never with decays, and then worth a second look, unless
+// nothing that it multiplies is left (A is zero, and exactly so).  A sigmoid's decays are at most 1, so that each rounding counts once.
+template <int GATE> __device__ __forceinline__ float lost_in_run(const float (&a)[kRun], float least, float A, float lost_a) {
+    if (!(least < kNormal) || (A == 0.f && lost_a == 0.f)) return 0.f;
     if constexpr (GATE == HX_GATE_SIGMOID) {
         return kRun * kStep;
     } else {
@@ -319,8 +319,8 @@ __device__ __forceinline__ void add_run(const float2 (&a)[kRun], const float2 (&
     float ax[kRun], ay[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) ax[i] = a[BACK ? kRun - 1 - i : i].x, ay[i] = a[BACK ? kRun - 1 - i : i].y;
-    reach[0].add(A.x, p.x, r.x, most.x, lost_in_run<GATE>(ax, least.x, A.x));
-    reach[1].add(A.y, p.y, r.y, most.y, lost_in_run<GATE>(ay, least.y, A.y));
+    reach[0].add(A.x, p.x, r.x, most.x, lost_in_run<GATE>(ax, least.x, A.x, reach[0].lost_a));
+    reach[1].add(A.y, p.y, r.y, most.y, lost_in_run<GATE>(ay, least.y, A.y, reach[1].lost_a));
     B = fma2(A, r, B);
     A = mul2(A, p);
 }

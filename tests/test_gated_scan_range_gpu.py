@@ -129,9 +129,15 @@ def decay_cases(L):
         a[:], v[:] = 0.4, 0.0
         v[::700] = keep * 1e20
 
+    def regrows(a, v):
+        a[:], v[:], v[10] = 1.0, 0.0, 1e30
+        a[24], a[25], a[26], a[27] = 1e-30, 1e-30, 1e30, 1e30    # 1e30 -> 1 -> 1e-30 -> 1 -> 1e30
+        a[30:110] = 0.25                                         # 6.8e-19 from there on
+
     return {f.__name__: f for f in (two_large, late_large, large_then_halves, halves_of_start, grows_over_zero, there_and_back,
                                     shrinks_after_growth, grows_after_shrinking, forgets, infinite, infinite_forgotten, not_a_number,
-                                    gate_not_a_number, infinite_gate, large_and_steady, over_the_largest, alternates, small, wild, sparse)}
+                                    gate_not_a_number, infinite_gate, large_and_steady, over_the_largest, alternates, small, wild, sparse,
+                                    regrows)}
 
 
 def decay_inputs(B, L, dtype, reverse):
