@@ -367,3 +367,55 @@ def test_sizes_beyond_32_bits_are_refused():
         with pytest.raises(L_.HxError) as e:
             call()
         assert e.value.status == 2
+
+
+def random_extremes(seed, B, L, D):
+    """Stretches of constant decay, growth by up to 1e30 that is taken back within 50 steps, and inputs and starts over the whole range."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.rand(*s, generator=gen, device="cuda")
+    choice = torch.tensor([1.0, 0.5, 0.25, 0.9, 0.99, 0.75, 1.0, 0.05], device="cuda")
+    stretch = (r(B, L, D) < 0.01).cumsum(1)
+    a = choice[(r(1, 1, D) * 8 + stretch * (1 + (r(1, 1, D) * 7).long())).long() % 8]
+    for _ in range(6 * (seed % 2)):
+        t, k = (r(B, 1, D) * (L - 60)).long(), 1 + (r(B, 1, D) * 50).long()
+        u = (60 * r(B, 1, D) - 30) * (r(B, 1, D) < 0.5)
+        a.scatter_(1, t, 10 ** u)
+        a.scatter_(1, t + k, 10 ** -u)
+    size = 38.4 * r(1, 1, D)
+    v = torch.where(r(B, L, D) < 10 ** (-1 - 2.3 * r(1, 1, D)), 10 ** (size * (r(B, L, D) * 1.5 - 0.5)) * torch.sign(r(B, L, D) - 0.5), 0.0)
+    v = torch.where(r(1, 1, D) < 0.3, v + torch.randn(B, L, D, generator=gen, device="cuda"), v)
+    start = 10 ** (38 * (2 * r(B, D) - 1)) * torch.sign(r(B, D) - 0.5)
+    return a, v.clamp(-3e38, 3e38), start
+
+
+def hold(got, want, a, v, start, reverse=False):
+    """2 (16 u W + 64 u M) as above, and 2^-125 a step for what may be taken as zero, under the decays behind it.  Where that reaches the
+    largest number, either way of summing may overflow; what comes after is not compared."""
+    a, v = a.double().abs(), v.double().abs()
+    m, w, z = start.double().abs(), torch.zeros_like(start, dtype=torch.float64), torch.full_like(start, 2.0 ** -125, dtype=torch.float64)
+    border = torch.zeros_like(start, dtype=torch.bool)
+    wrong = compared = torch.zeros((), dtype=torch.int64, device="cuda")
+    for t in (range(a.shape[1] - 1, -1, -1) if reverse else range(a.shape[1])):
+        if reverse:
+            m = m + v[:, t]
+        else:
+            w, m, z = a[:, t] * (w + m), a[:, t] * m + v[:, t], a[:, t] * z + 2.0 ** -125
+        tol = 32 * U * w + 128 * U * m + z
+        g, h = got[:, t].double(), want[:, t].double()
+        border = border | (tol + h.abs().nan_to_num(0, 0, 0) >= 0.999 * torch.finfo(torch.float32).max)
+        same = torch.where(torch.isfinite(h), (g - h).abs() <= tol, (g == h) | (torch.isnan(g) & torch.isnan(h)))
+        wrong, compared = wrong + (~same & ~border).sum(), compared + (~border).sum()
+        if reverse:
+            w, m, z = a[:, t] * (w + m), a[:, t] * m, a[:, t] * z + 2.0 ** -125
+    assert wrong.item() == 0 and compared.item() > 0.4 * got.numel(), (wrong.item(), compared.item())
+
+
+@pytest.mark.parametrize("seed,B,L,D", [(0, 2, 3000, 1024), (1, 1, 1500, 2048), (2, 4, 2001, 1408), (3, 1, 6000, 512)])
+def test_random_extremes(seed, B, L, D, monkeypatch):
+    a, v, start = random_extremes(seed, B, L, D)
+    call = lambda: ops.gated_scan(v, a, h0=start, gate="decay")
+    hold(call(), walked(monkeypatch, call), a, v, start)
+    zeros = torch.zeros_like(v)
+    st = ops.gated_scan_states(B, L, D).zero_()
+    call = lambda: ops.gated_scan_bwd(v, zeros, a, st, gate="decay", dh_last=start)[0]
+    hold(call(), walked(monkeypatch, call), a, v, start, reverse=True)
