@@ -166,10 +166,11 @@ template <typename T> __device__ __forceinline__ void store_some(T *p, float2 v,
 // A pair of gates -> decays a = sigmoid(g) and 1 - a, both good relative to themselves: with e = exp(-g), a = 1 / (1 + e) and
 // 1 - a = e a, neither of which cancels.  e is held to about 2^126, where 1 - a comes out as 1 and a, which would be the smallest normal
 // number there and below it behind, is set to zero.  A NaN goes through.
-// FAST, for bf16 tensors: one exp2 and one reciprocal of the special-function unit, a off by at most (|g| + 9) 2^-24 of itself, 4 2^-24
-// where it is near one (e's error counts for e / (1 + e) of itself).  Along a memory of 1 / (1 - a) steps that adds up to
-// 4 2^-24 / (1 - a) of h, where rounding an exact a would leave 2^-24 / (1 - a): at g = 10 some 5e-3 and 1.3e-3.  The step takes the
-// other form for every type, and so may differ from the same row of a scan by as much.
+// FAST, for bf16 tensors: one exp2 and one reciprocal of the special-function unit, a off by at most (|g| + 9) 2^-24 of itself, a few
+// 2^-24 where it is near one (e's error counts for e / (1 + e) of itself).  The step takes the other form for every type.
+// Along a memory of 1 / (1 - a) steps an error of a counts that often: constant inputs settle at 1 + (a's error) / (1 - a) times what
+// they should, in either form, because 1 + e is rounded: off by 1e-4 at g = 7.5, 6e-4 at 10, 4e-3 at 13, where an exact a rounded to
+// fp32 leaves 1e-5, 5e-4 and 4e-4.
 // Otherwise e = 2^t (1 + (t' - t) ln 2), t the rounded and t' the exact product -g log2(e), and one Newton step on the reciprocal.
 template <bool FAST> __device__ __forceinline__ void sigmoid2(float2 g, float2 &a, float2 &rest) {
     float2 e, end;   // end: 1 where e is held
